@@ -25,6 +25,8 @@ FO_B_KN, FO_B_NK = 0, 1
 (FO_EPI_NONE, FO_EPI_BIAS, FO_EPI_BIAS_RELU, FO_EPI_BIAS_GELU_TANH, FO_EPI_BIAS_GELU_ERF,
  FO_EPI_BIAS_LN, FO_EPI_RELU, FO_EPI_BIAS_RESIDUAL_LN, FO_EPI_BN, FO_EPI_BN_RELU, FO_EPI_BN_ADD_RELU) = range(11)
 FO_NOALLOC_LN_SCRATCH_BYTES = 8 << 20
+FO_NORM_RMS, FO_NORM_LAYER = 0, 1
+FO_GATE_NONE, FO_GATE_SILU, FO_GATE_GELU_TANH, FO_GATE_GELU_ERF, FO_GATE_RELU = range(5)
 
 # Every symbol include/b200fo.h declares; tests check the library exports all of them.
 EXPORTED = (
@@ -32,6 +34,8 @@ EXPORTED = (
     "fo_config_smem_bytes", "fo_device_status", "fo_set_wait_timeout_ns",
     "fo_selftest_wait_timeout", "fo_last_error", "fo_version", "fo_launch_count",
     "fo_gemm_bias_layernorm_noalloc", "fo_conv2d_workspace_size",
+    "fo_block_norm", "fo_block_norm_backward", "fo_block_norm_backward_workspace_size",
+    "fo_matvec_w4",
 )
 
 
@@ -66,6 +70,29 @@ class FoConvDesc(ctypes.Structure):
                 ("bn_eps", ctypes.c_float), ("residual", ctypes.c_void_p)]
 
 
+class FoBlockNormDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int64) for n in ("T", "D")] +
+                [(n, ctypes.c_void_p) for n in
+                 ("y", "x", "r", "z", "dr", "dz", "dy", "dx", "w_post", "b_post", "w_pre", "b_pre", "gate", "dw_post",
+                  "db_post", "dw_pre", "db_pre", "dgate")] +
+                [(n, ctypes.c_int64) for n in
+                 ("ldy", "ldx", "ldr", "ldz", "lddr", "lddz", "lddy", "lddx", "ldgate", "gate_rows")] +
+                [(n, ctypes.c_int32) for n in ("dtype", "vec_dtype", "norm")] +
+                [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float), ("workspace", ctypes.c_void_p),
+                 ("workspace_bytes", ctypes.c_size_t)])
+
+
+class FoW4(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "scales", "zeros")] +
+                [(n, ctypes.c_int64) for n in ("ldq", "lds", "ldz")] + [("group", ctypes.c_int32)])
+
+
+class FoMatvecW4Desc(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("w", FoW4), ("w_up", FoW4), ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32)]
+
+
 class FoError(RuntimeError):
     """A libb200fo call returned a non-zero code; `code` is the FO_E* value."""
 
@@ -90,6 +117,11 @@ def _declare(l: ctypes.CDLL) -> None:
     l.fo_conv2d.restype = ctypes.c_int
     l.fo_conv2d_workspace_size.argtypes = [P(FoConvDesc), P(FoTileCfg)]
     l.fo_conv2d_workspace_size.restype = ctypes.c_size_t
+    for f in (l.fo_block_norm, l.fo_block_norm_backward):
+        f.argtypes, f.restype = [P(FoBlockNormDesc), ctypes.c_void_p], ctypes.c_int
+    l.fo_block_norm_backward_workspace_size.argtypes = [P(FoBlockNormDesc)]
+    l.fo_block_norm_backward_workspace_size.restype = ctypes.c_size_t
+    l.fo_matvec_w4.argtypes, l.fo_matvec_w4.restype = [P(FoMatvecW4Desc), ctypes.c_void_p], ctypes.c_int
     l.fo_query_config_legal.argtypes = [ctypes.c_int32, ctypes.c_int32, P(FoTileCfg),
                                         ctypes.c_char_p, ctypes.c_size_t]
     l.fo_query_config_legal.restype = ctypes.c_int

@@ -29,6 +29,8 @@ SOURCES = [
     ("fo_family_conv.cu", "fo_family_conv", []),
     ("fo_family_direct.cu", "fo_family_direct", []),
     ("fo_noalloc.cu", "fo_noalloc", []),
+    ("fo_norm.cu", "fo_norm", []),
+    ("fo_skinny.cu", "fo_skinny", []),
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",

@@ -16,6 +16,7 @@
 #include "../../include/b200fo.h"
 #include "fo_launch.cuh"
 #include "fo_direct.cuh"
+#include "fo_host.cuh"
 
 namespace {
 
@@ -1038,3 +1039,33 @@ extern "C" int fo_selftest_wait_timeout(uint64_t timeout_ns, void* stream) {
                                               static_cast<unsigned long long>(timeout_ns));
   return ok();
 }
+
+// ---------------------------------------------------------------------- fo_host.cuh
+namespace fo {
+
+int host_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+
+int host_ok() { return ok(); }
+
+int host_device(HostDevice* out) {
+  DevInfo di;
+  if (int rc = device_info(&di)) return rc;
+  *out = {di.dev, di.sms, di.status, g_timeout_ns.load()};
+  return FO_OK;
+}
+
+int host_tmap(CUtensorMap* m, int dt, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+              uint32_t box_inner, uint32_t box_outer, const char* what) {
+  return make_tmap(m, dt, base, inner, outer, row_bytes, box_inner, box_outer, what);
+}
+
+void host_count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n)); }
+
+}  // namespace fo

@@ -5,18 +5,10 @@
 
 #include <atomic>
 
+#include "fo_host.cuh"
 #include "fo_kernel.cuh"
 
 namespace fo {
-
-// Function attributes and occupancy queries enqueue nothing, but a global-mode stream
-// capture on another thread would refuse them: switch this thread to relaxed mode for
-// the one-time setup of a kernel so that a first call under capture stays legal.
-struct RelaxedCapture {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
 
 struct LaunchArgs {
   CUtensorMap tmA, tmB, tmC;

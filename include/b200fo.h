@@ -175,6 +175,90 @@ int fo_conv2d(const FoConvDesc* desc, const FoTileCfg* cfg, void* stream);
  * along K (zero-filled before first use, left zeroed); 0 when no split applies. */
 size_t fo_conv2d_workspace_size(const FoConvDesc* desc, const FoTileCfg* cfg);
 
+/* ---- norms around a block ---------------------------------------------------------- */
+#define FO_NORM_RMS 0   /* v * rsqrt(mean(v^2) + eps) * w                                */
+#define FO_NORM_LAYER 1 /* (v - mean) * rsqrt(var + eps) * w + b                         */
+
+/* The norms after and before a block, fused with the block's gate and the residual scale.
+ * y: the block's output, x: the residual stream, both [T, D]:
+ *   n = norm_post(y) (w_post NULL: n = y),  r = residual_scale * x + gate * n,
+ *   z = norm_pre(r), computed from the unrounded r.
+ * gate: NULL (gate_rows 0) or [gate_rows, D] with row stride ldgate, each row shared by
+ * T / gate_rows consecutive rows.  Parameters and their gradients are of vec_dtype; biases
+ * (may be NULL) belong to FO_NORM_LAYER.  Backward reads y, r, dr (may be NULL: zero) and
+ * dz and writes dy, dx, dw_pre, dw_post (with w_post), db_pre and db_post (where not NULL)
+ * and dgate ([gate_rows, D], contiguous).  Sums over rows run in a fixed order.
+ * D <= 16384 forward, 8192 backward (FO_EUNSUPPORTED above). */
+typedef struct FoBlockNormDesc {
+  int64_t T, D;
+  const void* y;
+  const void* x;   /* forward */
+  void* r;         /* written forward, read backward */
+  void* z;
+  const void* dr;
+  const void* dz;
+  void* dy;
+  void* dx;
+  const void* w_post;
+  const void* b_post;
+  const void* w_pre;
+  const void* b_pre;
+  const void* gate;
+  void* dw_post;
+  void* db_post;
+  void* dw_pre;
+  void* db_pre;
+  void* dgate;
+  int64_t ldy, ldx, ldr, ldz, lddr, lddz, lddy, lddx, ldgate;
+  int64_t gate_rows;
+  int32_t dtype;     /* FO_DT_F16 or FO_DT_BF16: y, x, r, z and their gradients            */
+  int32_t vec_dtype; /* parameters and their gradients                                     */
+  int32_t norm;      /* FO_NORM_*                                                          */
+  float residual_scale, eps;
+  void* workspace;   /* backward: fo_block_norm_backward_workspace_size bytes, any content */
+  size_t workspace_bytes;
+} FoBlockNormDesc;
+
+int fo_block_norm(const FoBlockNormDesc* desc, void* stream);
+int fo_block_norm_backward(const FoBlockNormDesc* desc, void* stream);
+size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* desc);
+
+/* ---- few-token products with 4-bit weights ------------------------------------------ */
+/* Activations of the gated products, act(x Wg) * (x Wu). */
+#define FO_GATE_NONE 0
+#define FO_GATE_SILU 1      /* g / (1 + e^-g)                                            */
+#define FO_GATE_GELU_TANH 2
+#define FO_GATE_GELU_ERF 3
+#define FO_GATE_RELU 4
+
+/* w[n, k] = scales[n, k / group] * (q[n, k] - zeros[n, k / group]).  q: two weights to a
+ * byte, the lower nibble the even k, rows ldq bytes apart (a multiple of 16, 16-byte aligned
+ * base); scales: dtype of x, rows lds apart; zeros: one byte each, rows ldz apart, or NULL
+ * (every zero is 8).  group: a multiple of 32; the last group of a row may be short. */
+typedef struct FoW4 {
+  const void* q;
+  const void* scales;
+  const void* zeros;
+  int64_t ldq, lds, ldz;
+  int32_t group;
+} FoW4;
+
+/* act FO_GATE_NONE: out[T, N] = x[T, K] w^T (+ bias).  Otherwise out = act(x w^T) * (x w_up^T).
+ * K a multiple of 32 and at most 1024 groups.  Any T; the weights are read once for every
+ * 64 tokens, so it pays for few. */
+typedef struct FoMatvecW4Desc {
+  int64_t T, N, K;
+  const void* x;
+  FoW4 w, w_up;
+  const void* bias; /* [N] of dtype or NULL                                                */
+  void* out;
+  int64_t ldx, ldo;
+  int32_t dtype; /* FO_DT_F16 or FO_DT_BF16: x, scales, bias and out                       */
+  int32_t act;   /* FO_GATE_*                                                              */
+} FoMatvecW4Desc;
+
+int fo_matvec_w4(const FoMatvecW4Desc* desc, void* stream);
+
 /* Legality of a tile config for an op (0 = gemm family, 1 = conv2d) and output dtype:
  * shared memory <= 227 KB, TMEM columns <= 512, tcgen05 shape rules.  Returns FO_OK or
  * FO_EINVAL with the reason in `why`.  Host-only; needs no GPU.  Used by the autotuner's
