@@ -35,7 +35,7 @@ EXPORTED = (
     "fo_selftest_wait_timeout", "fo_last_error", "fo_version", "fo_launch_count",
     "fo_gemm_bias_layernorm_noalloc", "fo_conv2d_workspace_size",
     "fo_block_norm", "fo_block_norm_backward", "fo_block_norm_backward_workspace_size",
-    "fo_matvec_w4",
+    "fo_matvec_w4", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
 )
 
 
@@ -82,6 +82,16 @@ class FoBlockNormDesc(ctypes.Structure):
                  ("workspace_bytes", ctypes.c_size_t)])
 
 
+class FoGatedFfnDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int64) for n in ("T", "D", "F", "N")] +
+                [(n, ctypes.c_void_p) for n in
+                 ("x", "w_gate", "w_up", "w_down", "y", "g", "u", "dy", "dx", "dw_gate", "dw_up", "dw_down")] +
+                [(n, ctypes.c_int64) for n in
+                 ("ldx", "ldwg", "ldwu", "ldwd", "ldy", "ldg", "ldu", "lddy", "lddx", "lddwg", "lddwu", "lddwd")] +
+                [(n, ctypes.c_int32) for n in ("dtype", "b_layout", "act")] +
+                [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
+
+
 class FoW4(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "scales", "zeros")] +
                 [(n, ctypes.c_int64) for n in ("ldq", "lds", "ldz")] + [("group", ctypes.c_int32)])
@@ -121,6 +131,10 @@ def _declare(l: ctypes.CDLL) -> None:
         f.argtypes, f.restype = [P(FoBlockNormDesc), ctypes.c_void_p], ctypes.c_int
     l.fo_block_norm_backward_workspace_size.argtypes = [P(FoBlockNormDesc)]
     l.fo_block_norm_backward_workspace_size.restype = ctypes.c_size_t
+    for f in (l.fo_gated_ffn, l.fo_gated_ffn_backward):
+        f.argtypes, f.restype = [P(FoGatedFfnDesc), ctypes.c_void_p], ctypes.c_int
+    l.fo_gated_ffn_workspace_size.argtypes = [P(FoGatedFfnDesc), ctypes.c_int32]
+    l.fo_gated_ffn_workspace_size.restype = ctypes.c_size_t
     l.fo_matvec_w4.argtypes, l.fo_matvec_w4.restype = [P(FoMatvecW4Desc), ctypes.c_void_p], ctypes.c_int
     l.fo_query_config_legal.argtypes = [ctypes.c_int32, ctypes.c_int32, P(FoTileCfg),
                                         ctypes.c_char_p, ctypes.c_size_t]

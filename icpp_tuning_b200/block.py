@@ -1,5 +1,6 @@
 """Operators of a decoder block's feed-forward half over libb200fo.so, for torch CUDA tensors.
 
+  gated_ffn, gated_ffn_backward     the gated feed-forward block (act(x Wg) * (x Wu)) Wd
   block_norm, block_norm_backward   the norms after and before a block, fused with its gate
                                     and the residual scale
   matvec_w4, gated_ffn_w4           products of a few tokens with 4-bit weights (W4), plain and
@@ -46,6 +47,83 @@ def _sixteen_bit(dt: torch.dtype, name: str) -> int:
     if dt not in (torch.float16, torch.bfloat16):
         raise ValueError(f"{name} must be float16 or bfloat16, got {dt}")
     return dtype_code(dt)
+
+
+# ---------------------------------------------------------------------- gated feed-forward block
+def _matrix(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised [rows, cols] whose row stride is a multiple of 8 elements."""
+    t = torch.empty((rows, (cols + 7) // 8 * 8), dtype=like.dtype, device=like.device)
+    return t if cols % 8 == 0 else t[:, :cols]
+
+
+def _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, others) -> N.FoGatedFfnDesc:
+    if act not in GATE_ACTS:
+        raise ValueError(f"act must be one of {sorted(GATE_ACTS)}")
+    if b_layout not in ("kn", "nk"):
+        raise ValueError("b_layout must be 'kn' or 'nk'")
+    kn = b_layout == "kn"
+    d = N.FoGatedFfnDesc()
+    d.dtype, d.act, d.b_layout = _sixteen_bit(x.dtype, "x"), GATE_ACTS[act], N.FO_B_KN if kn else N.FO_B_NK
+    for t in (w_gate, w_up, w_down, *others):
+        if t.dtype != x.dtype:
+            raise ValueError("every matrix of the block must share x's dtype")
+    d.x, d.ldx = x.data_ptr(), _rows(x, "x")
+    d.T, d.D = x.shape
+    d.ldwd = _rows(w_down, "w_down")
+    d.F, d.N = w_down.shape if kn else reversed(w_down.shape)
+    up = (d.D, d.F) if kn else (d.F, d.D)
+    d.ldwg, d.ldwu = _like(w_gate, up, "w_gate"), _like(w_up, up, "w_up")
+    d.w_gate, d.w_up, d.w_down = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
+    return d
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, *, act: str = "silu",
+              b_layout: str = "kn", save: bool = False, stream=None):
+    """y = (act(x Wg) * (x Wu)) Wd, the two products accumulated in fp32.
+
+    x [T, D] float16 / bfloat16; w_gate, w_up [D, F] and w_down [F, N] when b_layout == "kn",
+    [F, D] and [N, F] when "nk" (nn.Linear).  act: one of GATE_ACTS.  Returns y [T, N], or with
+    save=True (y, g, u): the products before the activation, for gated_ffn_backward.  The
+    intermediate act(g) * u is rounded to x's dtype.  Row strides must be multiples of 8."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return gated_ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout, save=save)
+    dev = _require_cuda(x, w_gate, w_up, w_down)
+    d = _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, ())
+    y = _matrix(d.T, d.N, x)
+    d.y, d.ldy = y.data_ptr(), y.stride(0)
+    if save:
+        g, u = _matrix(d.T, d.F, x), _matrix(d.T, d.F, x)
+        d.g, d.ldg, d.u, d.ldu = g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0)
+    lib = N.lib()
+    need = lib.fo_gated_ffn_workspace_size(ctypes.byref(d), 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _run(dev, lib.fo_gated_ffn, ctypes.byref(d))
+    return (y, g, u) if save else y
+
+
+def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                       g: torch.Tensor, u: torch.Tensor, *, act: str = "silu", b_layout: str = "kn",
+                       stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw_gate, dw_up, dw_down) of gated_ffn from dy [T, N] and the g, u it saved."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return gated_ffn_backward(dy, x, w_gate, w_up, w_down, g, u, act=act, b_layout=b_layout)
+    dev = _require_cuda(x, dy, w_gate, w_up, w_down, g, u)
+    d = _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, (dy, g, u))
+    d.dy, d.lddy = dy.data_ptr(), _like(dy, (d.T, d.N), "dy")
+    d.g, d.ldg = g.data_ptr(), _like(g, (d.T, d.F), "g")
+    d.u, d.ldu = u.data_ptr(), _like(u, (d.T, d.F), "u")
+    dx, dwg, dwu, dwd = (_matrix(*t.shape, x) for t in (x, w_gate, w_up, w_down))
+    d.dx, d.dw_gate, d.dw_up, d.dw_down = dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()
+    d.lddx, d.lddwg, d.lddwu, d.lddwd = dx.stride(0), dwg.stride(0), dwu.stride(0), dwd.stride(0)
+    lib = N.lib()
+    need = lib.fo_gated_ffn_workspace_size(ctypes.byref(d), 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _run(dev, lib.fo_gated_ffn_backward, ctypes.byref(d))
+    return dx, dwg, dwu, dwd
 
 
 # ---------------------------------------------------------------------- norms around a block

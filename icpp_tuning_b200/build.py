@@ -29,6 +29,7 @@ SOURCES = [
     ("fo_family_conv.cu", "fo_family_conv", []),
     ("fo_family_direct.cu", "fo_family_direct", []),
     ("fo_noalloc.cu", "fo_noalloc", []),
+    ("fo_ffn.cu", "fo_ffn", []),
     ("fo_norm.cu", "fo_norm", []),
     ("fo_skinny.cu", "fo_skinny", []),
 ]

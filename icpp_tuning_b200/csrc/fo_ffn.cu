@@ -1,0 +1,278 @@
+// fo_ffn.cu -- launches and C entries of the gated feed-forward block.
+#include <cstring>
+
+#include "fo_ffn.cuh"
+#include "fo_host.cuh"
+#include "../../include/b200fo.h"
+
+namespace fo {
+namespace {
+
+template <int EPI, int ACT, int DT>
+cudaError_t launch_ffn(const FfnMaps& maps, const FfnParams& p, int pairs, cudaStream_t stream) {
+  static std::atomic<uint64_t> opted{0};
+  return launch_pdl(fo_ffn_kernel<EPI, ACT, DT>, opted, dim3(2 * (p.units < pairs ? p.units : pairs)), dim3(320), kFfnSmem, 2, stream,
+                    maps, p);
+}
+
+template <int EPI, int DT>
+cudaError_t by_act(int act, const FfnMaps& m, const FfnParams& p, int pairs, cudaStream_t s) {
+  switch (act) {
+    case FO_GATE_SILU: return launch_ffn<EPI, ACT_SILU, DT>(m, p, pairs, s);
+    case FO_GATE_GELU_TANH: return launch_ffn<EPI, ACT_GELU_TANH, DT>(m, p, pairs, s);
+    case FO_GATE_GELU_ERF: return launch_ffn<EPI, ACT_GELU_ERF, DT>(m, p, pairs, s);
+    default: return launch_ffn<EPI, ACT_RELU, DT>(m, p, pairs, s);
+  }
+}
+
+cudaError_t launch(int epi, int act, const FfnMaps& m, const FfnParams& p, int pairs, cudaStream_t s) {
+  if (epi == FFN_GRADS)
+    return p.bf16 ? launch_ffn<FFN_GRADS, ACT_NONE, DT_BF16>(m, p, pairs, s) : launch_ffn<FFN_GRADS, ACT_NONE, DT_F16>(m, p, pairs, s);
+  if (epi == FFN_GATED) return p.bf16 ? by_act<FFN_GATED, DT_BF16>(act, m, p, pairs, s) : by_act<FFN_GATED, DT_F16>(act, m, p, pairs, s);
+  return p.bf16 ? by_act<FFN_DGATE, DT_BF16>(act, m, p, pairs, s) : by_act<FFN_DGATE, DT_F16>(act, m, p, pairs, s);
+}
+
+// A stored matrix [rows, cols], row-major.
+struct Mat {
+  const void* p;
+  int64_t rows, cols, ld;
+};
+
+// One launch being put together: problems in order, then the schedule.
+struct Build {
+  FfnMaps maps;
+  FfnParams p;
+  int dt;
+  int rc = FO_OK;
+
+  explicit Build(int dtype, const HostDevice& hd) : dt(dtype) {
+    memset(&maps, 0, sizeof(maps));
+    memset(&p, 0, sizeof(p));
+    p.bf16 = dtype == FO_DT_BF16;
+    p.group_m = 8;
+    p.status = hd.status;
+    p.timeout_ns = hd.timeout_ns;
+  }
+
+  void map(CUtensorMap* m, const Mat& t, uint32_t box_rows, const char* what) {
+    if (rc == FO_OK) rc = host_tmap(m, dt, t.p, t.cols, t.rows, static_cast<uint64_t>(t.ld) * 2, 64, box_rows, what);
+  }
+  // An operand whose rows (kt = false) or columns (kt = true: read transposed) run along the
+  // product's M or N.
+  void operand(CUtensorMap* m, const Mat& t, bool kt, const char* what) { map(m, t, kt ? 64 : 128, what); }
+
+  FfnProblem& add(int64_t M, int64_t N, int64_t K, int tile_n, int segments) {
+    FfnProblem& q = p.prob[p.nprob++];
+    q.M = static_cast<int>(M), q.N = static_cast<int>(N);
+    q.tiles_m = (q.M + kFfnTile - 1) / kFfnTile;
+    q.tiles_n = (q.N + tile_n - 1) / tile_n;
+    q.kb0 = static_cast<int>((K + kBK - 1) / kBK);
+    q.kb = segments * q.kb0;
+    q.unit0 = p.units;
+    p.units += q.tiles_m * q.tiles_n;
+    return q;
+  }
+
+  // C [M, N] = op(A) op(B) over K (a second pair of operands: a second K segment).
+  void product(int64_t M, int64_t N, int64_t K, const Mat& a, bool a_t, const Mat& b, bool b_t, const Mat& c,
+               const Mat* a1 = nullptr, const Mat* b1 = nullptr) {
+    FfnProblem& q = add(M, N, K, kFfnTile, a1 != nullptr ? 2 : 1);
+    const int i = p.nprob - 1;
+    q.a_mn = a_t, q.b_mn = b_t;
+    operand(&maps.a[i][0], a, a_t, "a product's first operand");
+    operand(&maps.b[i][0], b, b_t, "a product's second operand");
+    if (a1 != nullptr) {
+      operand(&maps.a[i][1], *a1, a_t, "a product's first operand");
+      operand(&maps.b[i][1], *b1, b_t, "a product's second operand");
+    }
+    map(&maps.c[i], c, 32, "a product's output");
+  }
+
+  // Names each unit's pair when the problems' K differ: longest first, to the pair with the
+  // least work so far (dx of a short batch has few, long tiles; the weight gradients many,
+  // short ones).  Above kFfnOwners units the tiles per pair are many enough to walk them in
+  // turn.
+  void schedule(int pairs) {
+    if (p.nprob < 2 || p.units > kFfnOwners) return;
+    int load[256] = {0};
+    if (pairs > 256) pairs = 256;
+    if (pairs > p.units) pairs = p.units;
+    p.owned = 1;
+    for (int i = 0; i < p.nprob; ++i) {
+      const FfnProblem& q = p.prob[i];
+      for (int t = 0; t < q.tiles_m * q.tiles_n; ++t) {
+        int best = 0;
+        for (int c = 1; c < pairs; ++c)
+          if (load[c] < load[best]) best = c;
+        p.owner[q.unit0 + t] = static_cast<unsigned char>(best);
+        load[best] += q.kb + 8;  // the tile's K blocks and about its epilogue
+      }
+    }
+  }
+};
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+int check_mat(const void* p, int64_t ld, int64_t cols, const char* name) {
+  if (p == nullptr || !host_aligned16(p)) return host_fail(FO_EINVAL, "%s must be a 16-byte aligned device pointer", name);
+  if (ld % 8 != 0 || ld < cols)
+    return host_fail(FO_EINVAL, "the row stride of %s must be a multiple of 8 and >= %lld, got %lld", name, static_cast<long long>(cols),
+                     static_cast<long long>(ld));
+  return FO_OK;
+}
+
+int check(const FoGatedFfnDesc* d) {
+  if (d == nullptr) return host_fail(FO_EINVAL, "null descriptor");
+  if (d->T < 0 || d->D < 0 || d->F < 0 || d->N < 0) return host_fail(FO_EINVAL, "negative problem size");
+  for (int64_t v : {d->T, d->D, d->F, d->N})
+    if (v > (1ll << 27)) return host_fail(FO_EINVAL, "problem too large");
+  if (d->dtype != FO_DT_F16 && d->dtype != FO_DT_BF16) return host_fail(FO_EINVAL, "dtype must be FO_DT_F16 or FO_DT_BF16");
+  if (d->b_layout != FO_B_KN && d->b_layout != FO_B_NK) return host_fail(FO_EINVAL, "bad b_layout %d", d->b_layout);
+  if (d->act < FO_GATE_SILU || d->act > FO_GATE_RELU) return host_fail(FO_EINVAL, "bad activation %d", d->act);
+  return FO_OK;
+}
+
+int check_weights(const FoGatedFfnDesc* d, bool kn) {
+  if (int rc = check_mat(d->x, d->ldx, d->D, "x")) return rc;
+  if (int rc = check_mat(d->w_gate, d->ldwg, kn ? d->F : d->D, "w_gate")) return rc;
+  if (int rc = check_mat(d->w_up, d->ldwu, kn ? d->F : d->D, "w_up")) return rc;
+  return check_mat(d->w_down, d->ldwd, kn ? d->N : d->F, "w_down");
+}
+
+int fail_launch(cudaError_t e) { return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e)); }
+
+}  // namespace
+}  // namespace fo
+
+extern "C" size_t fo_gated_ffn_workspace_size(const FoGatedFfnDesc* d, int32_t backward) {
+  if (d == nullptr || d->T <= 0 || d->F <= 0) return 0;
+  return static_cast<size_t>(d->T) * fo::pad8(d->F) * 2 * (backward ? 3 : 1);
+}
+
+extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
+  using namespace fo;
+  if (int rc = check(d)) return rc;
+  if (d->T == 0 || d->N == 0) return host_ok();
+  if (d->D == 0 || d->F == 0) return host_fail(FO_EINVAL, "D and F must be positive");
+  const bool kn = d->b_layout == FO_B_KN;
+  if (int rc = check_weights(d, kn)) return rc;
+  if (int rc = check_mat(d->y, d->ldy, d->N, "y")) return rc;
+  const bool save = d->g != nullptr;
+  if (save != (d->u != nullptr)) return host_fail(FO_EINVAL, "g and u are saved together");
+  if (save) {
+    if (int rc = check_mat(d->g, d->ldg, d->F, "g")) return rc;
+    if (int rc = check_mat(d->u, d->ldu, d->F, "u")) return rc;
+  }
+  const size_t need = fo_gated_ffn_workspace_size(d, 0);
+  if (d->workspace == nullptr || d->workspace_bytes < need || !host_aligned16(d->workspace))
+    return host_fail(FO_EINVAL, "the block needs a 16-byte aligned workspace of %zu bytes", need);
+  HostDevice hd;
+  if (int rc = host_device(&hd)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Mat h{d->workspace, d->T, d->F, pad8(d->F)};
+
+  Build b(d->dtype, hd);
+  FfnProblem& q = b.add(d->T, d->F, d->D, kFfnTile / 2, 1);
+  q.b_mn = kn;
+  const Mat x{d->x, d->T, d->D, d->ldx};
+  const Mat wg{d->w_gate, kn ? d->D : d->F, kn ? d->F : d->D, d->ldwg}, wu{d->w_up, wg.rows, wg.cols, d->ldwu};
+  b.operand(&b.maps.a[0][0], x, false, "x");
+  b.operand(&b.maps.b[0][0], wg, kn, "w_gate");
+  b.operand(&b.maps.b[0][1], wu, kn, "w_up");
+  b.map(&b.maps.c[0], h, 32, "h");
+  b.p.save = save;
+  if (save) {
+    b.map(&b.maps.c[1], {d->g, d->T, d->F, d->ldg}, 32, "g");
+    b.map(&b.maps.c[2], {d->u, d->T, d->F, d->ldu}, 32, "u");
+  }
+  if (b.rc) return b.rc;
+  cudaError_t e = launch(FFN_GATED, d->act, b.maps, b.p, hd.sms / 2, st);
+  if (e != cudaSuccess) return fail_launch(e);
+
+  Build y(d->dtype, hd);
+  y.product(d->T, d->N, d->F, h, false, {d->w_down, kn ? d->F : d->N, kn ? d->N : d->F, d->ldwd}, kn, {d->y, d->T, d->N, d->ldy});
+  if (y.rc) return y.rc;
+  e = launch(FFN_GRADS, 0, y.maps, y.p, hd.sms / 2, st);
+  if (e != cudaSuccess) return fail_launch(e);
+  host_count_launches(2);
+  return host_ok();
+}
+
+extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
+  using namespace fo;
+  if (int rc = check(d)) return rc;
+  if (d->D == 0 || d->F == 0 || d->N == 0) return host_fail(FO_EINVAL, "D, F and N must be positive");
+  const bool kn = d->b_layout == FO_B_KN;
+  if (int rc = check_weights(d, kn)) return rc;
+  if (int rc = check_mat(d->dw_gate, d->lddwg, kn ? d->F : d->D, "dw_gate")) return rc;
+  if (int rc = check_mat(d->dw_up, d->lddwu, kn ? d->F : d->D, "dw_up")) return rc;
+  if (int rc = check_mat(d->dw_down, d->lddwd, kn ? d->N : d->F, "dw_down")) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  HostDevice hd;
+  const int64_t up_rows = kn ? d->D : d->F, up_cols = kn ? d->F : d->D;
+  const int64_t down_rows = kn ? d->F : d->N, down_cols = kn ? d->N : d->F;
+  if (d->T == 0) {  // no tokens: the weight gradients are empty sums
+    if (int rc = host_device(&hd)) return rc;
+    if (cudaMemset2DAsync(d->dw_gate, d->lddwg * 2, 0, up_cols * 2, up_rows, st) != cudaSuccess ||
+        cudaMemset2DAsync(d->dw_up, d->lddwu * 2, 0, up_cols * 2, up_rows, st) != cudaSuccess ||
+        cudaMemset2DAsync(d->dw_down, d->lddwd * 2, 0, down_cols * 2, down_rows, st) != cudaSuccess)
+      return host_fail(FO_ECUDA, "clearing a weight gradient failed");
+    return host_ok();
+  }
+  if (int rc = check_mat(d->dy, d->lddy, d->N, "dy")) return rc;
+  if (int rc = check_mat(d->g, d->ldg, d->F, "g")) return rc;
+  if (int rc = check_mat(d->u, d->ldu, d->F, "u")) return rc;
+  if (int rc = check_mat(d->dx, d->lddx, d->D, "dx")) return rc;
+  const size_t need = fo_gated_ffn_workspace_size(d, 1);
+  if (d->workspace == nullptr || d->workspace_bytes < need || !host_aligned16(d->workspace))
+    return host_fail(FO_EINVAL, "the backward pass needs a 16-byte aligned workspace of %zu bytes", need);
+  if (int rc = host_device(&hd)) return rc;
+  const int64_t ldf = pad8(d->F);
+  char* ws = static_cast<char*>(d->workspace);
+  const Mat dg{ws, d->T, d->F, ldf}, du{ws + d->T * ldf * 2, d->T, d->F, ldf}, h{ws + 2 * d->T * ldf * 2, d->T, d->F, ldf};
+  const Mat x{d->x, d->T, d->D, d->ldx}, dy{d->dy, d->T, d->N, d->lddy};
+  const Mat wg{d->w_gate, up_rows, up_cols, d->ldwg}, wu{d->w_up, up_rows, up_cols, d->ldwu};
+  const Mat wd{d->w_down, down_rows, down_cols, d->ldwd};
+
+  Build b(d->dtype, hd);
+  FfnProblem& q = b.add(d->T, d->F, d->N, kFfnTile, 1);
+  q.b_mn = !kn;
+  b.operand(&b.maps.a[0][0], dy, false, "dy");
+  b.operand(&b.maps.b[0][0], wd, !kn, "w_down");
+  b.map(&b.maps.c[0], dg, 32, "dg");
+  b.map(&b.maps.c[1], du, 32, "du");
+  b.map(&b.maps.c[2], h, 32, "h");
+  b.p.g = d->g, b.p.u = d->u, b.p.ldg = d->ldg, b.p.ldu = d->ldu;
+  if (b.rc) return b.rc;
+  cudaError_t e = launch(FFN_DGATE, d->act, b.maps, b.p, hd.sms / 2, st);
+  if (e != cudaSuccess) return fail_launch(e);
+
+  Build w(d->dtype, hd);
+  auto add_dx = [&] { w.product(d->T, d->D, d->F, dg, false, wg, !kn, {d->dx, d->T, d->D, d->lddx}, &du, &wu); };
+  auto add_weights = [&] {
+    const Mat owg{d->dw_gate, up_rows, up_cols, d->lddwg}, owu{d->dw_up, up_rows, up_cols, d->lddwu};
+    const Mat owd{d->dw_down, down_rows, down_cols, d->lddwd};
+    if (kn) {
+      w.product(d->D, d->F, d->T, x, true, dg, true, owg);
+      w.product(d->D, d->F, d->T, x, true, du, true, owu);
+      w.product(d->F, d->N, d->T, h, true, dy, true, owd);
+    } else {
+      w.product(d->F, d->D, d->T, dg, true, x, true, owg);
+      w.product(d->F, d->D, d->T, du, true, x, true, owu);
+      w.product(d->N, d->F, d->T, dy, true, h, true, owd);
+    }
+  };
+  if (2 * d->F >= d->T) {  // longest tiles first
+    add_dx();
+    add_weights();
+  } else {
+    add_weights();
+    add_dx();
+  }
+  if (w.rc) return w.rc;
+  w.schedule(hd.sms / 2);
+  e = launch(FFN_GRADS, 0, w.maps, w.p, hd.sms / 2, st);
+  if (e != cudaSuccess) return fail_launch(e);
+  host_count_launches(2);
+  return host_ok();
+}

@@ -45,11 +45,19 @@ struct SkinnyParams {
 // forms need one exponential and one reciprocal (gelu_tanh(x) = x sigmoid(2 u)).
 __device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
-__device__ __forceinline__ float gate_act(int act, float x) {
-  if (act == ACT_SILU) return x * sigmoid_fast(x);
-  if (act == ACT_GELU_TANH) return x * sigmoid_fast(1.5957691216057308f * fmaf(0.044715f * x, x * x, x));
-  if (act == ACT_GELU_ERF) return 0.5f * x * (1.0f + erf_as7128(x * 0.7071067811865476f));
+template <int ACT>
+__device__ __forceinline__ float gate_act(float x) {
+  if constexpr (ACT == ACT_SILU) return x * sigmoid_fast(x);
+  if constexpr (ACT == ACT_GELU_TANH) return x * sigmoid_fast(1.5957691216057308f * fmaf(0.044715f * x, x * x, x));
+  if constexpr (ACT == ACT_GELU_ERF) return 0.5f * x * (1.0f + erf_as7128(x * 0.7071067811865476f));
   return x < 0.f ? 0.f : x;
+}
+
+__device__ __forceinline__ float gate_act(int act, float x) {
+  if (act == ACT_SILU) return gate_act<ACT_SILU>(x);
+  if (act == ACT_GELU_TANH) return gate_act<ACT_GELU_TANH>(x);
+  if (act == ACT_GELU_ERF) return gate_act<ACT_GELU_ERF>(x);
+  return gate_act<ACT_RELU>(x);
 }
 
 template <int DT>

@@ -223,7 +223,7 @@ int fo_block_norm(const FoBlockNormDesc* desc, void* stream);
 int fo_block_norm_backward(const FoBlockNormDesc* desc, void* stream);
 size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* desc);
 
-/* ---- few-token products with 4-bit weights ------------------------------------------ */
+/* ---- the gated feed-forward block ---------------------------------------------------- */
 /* Activations of the gated products, act(x Wg) * (x Wu). */
 #define FO_GATE_NONE 0
 #define FO_GATE_SILU 1      /* g / (1 + e^-g)                                            */
@@ -231,6 +231,41 @@ size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* desc);
 #define FO_GATE_GELU_ERF 3
 #define FO_GATE_RELU 4
 
+/* Forward: g = x Wg, u = x Wu, h = act(g) * u, y = h Wd.  x [T, D], y [T, N]; weights as
+ * b_layout says: FO_B_KN Wg, Wu [D, F] and Wd [F, N], FO_B_NK [F, D] and [N, F].  g and u
+ * [T, F] are written when both pointers are given (what the backward pass needs).  h is
+ * rounded to dtype between the two products.
+ * Backward, from dy and the saved g, u: dh = dy Wd^T, dg = dh u act'(g), du = dh act(g),
+ * dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du, dWd = h^T dy; dh stays in fp32, dg, du
+ * and h are rounded to dtype.  relu'(0) = 0.
+ * Every matrix: 16-byte aligned, row stride a multiple of 8 elements. */
+typedef struct FoGatedFfnDesc {
+  int64_t T, D, F, N;
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  void* y;
+  void* g; /* written forward (or NULL), read backward                                     */
+  void* u;
+  const void* dy;
+  void* dx;
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  int64_t ldx, ldwg, ldwu, ldwd, ldy, ldg, ldu, lddy, lddx, lddwg, lddwu, lddwd;
+  int32_t dtype;    /* FO_DT_F16 or FO_DT_BF16, of every matrix                            */
+  int32_t b_layout; /* FO_B_KN or FO_B_NK                                                  */
+  int32_t act;      /* FO_GATE_SILU .. FO_GATE_RELU                                        */
+  void* workspace;  /* fo_gated_ffn_workspace_size bytes, any content                      */
+  size_t workspace_bytes;
+} FoGatedFfnDesc;
+
+int fo_gated_ffn(const FoGatedFfnDesc* desc, void* stream);
+int fo_gated_ffn_backward(const FoGatedFfnDesc* desc, void* stream);
+size_t fo_gated_ffn_workspace_size(const FoGatedFfnDesc* desc, int32_t backward);
+
+/* ---- few-token products with 4-bit weights ------------------------------------------ */
 /* w[n, k] = scales[n, k / group] * (q[n, k] - zeros[n, k / group]).  q: two weights to a
  * byte, the lower nibble the even k, rows ldq bytes apart (a multiple of 16, 16-byte aligned
  * base); scales: dtype of x, rows lds apart; zeros: one byte each, rows ldz apart, or NULL
