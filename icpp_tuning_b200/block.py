@@ -19,60 +19,88 @@ from typing import Dict, NamedTuple, Optional, Tuple
 import torch
 
 from . import _native as N
-from .fused import _require_cuda, _rows, _vec, dtype_code
+from .fused import _require_cuda, _vec, dtype_code
 
 GATE_ACTS = {"silu": N.FO_GATE_SILU, "gelu_tanh": N.FO_GATE_GELU_TANH, "gelu_erf": N.FO_GATE_GELU_ERF,
              "relu": N.FO_GATE_RELU}
 NORMS = {"rms": N.FO_NORM_RMS, "layer": N.FO_NORM_LAYER}
 
 
-def _run(dev: torch.device, fn, *args) -> None:
+def _run(dev: torch.device, fn, desc) -> None:
     """Calls a C entry on `dev`'s current stream."""
-    s = torch.cuda.current_stream(dev).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)  # current_stream(dev).cuda_stream without the Stream object
     if torch.cuda.current_device() == dev.index:
-        N.check(fn(*args, s))
+        rc = fn(desc, stream)
     else:
         with torch.cuda.device(dev):
-            N.check(fn(*args, s))
+            rc = fn(desc, stream)
+    if rc:
+        N.check(rc)
 
 
-def _like(t: torch.Tensor, shape: Tuple[int, int], name: str) -> int:
-    """Row stride of a 2-D operand that must have this shape."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    return _rows(t, name)
+def _cuda(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The one CUDA device of these tensors (None: not given)."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            return _require_cuda(*ts)  # raises
+    return dev if dev.type == "cuda" else _require_cuda(*ts)
+
+
+def _ld(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    """Row stride of a 2-D operand that must be [rows, cols] with unit column stride."""
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
+    st = t.stride()
+    if st[1] != 1 and cols != 1:
+        raise ValueError(f"{name} must be a 2-D tensor with unit column stride")
+    return st[0]
+
+
+def _shape2(t: torch.Tensor, name: str) -> Tuple[int, int]:
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D tensor with unit column stride")
+    return t.shape
 
 
 def _sixteen_bit(dt: torch.dtype, name: str) -> int:
-    if dt not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{name} must be float16 or bfloat16, got {dt}")
-    return dtype_code(dt)
+    if dt is torch.bfloat16:
+        return N.FO_DT_BF16
+    if dt is torch.float16:
+        return N.FO_DT_F16
+    raise ValueError(f"{name} must be float16 or bfloat16, got {dt}")
 
 
 # ---------------------------------------------------------------------- gated feed-forward block
 def _matrix(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """An uninitialised [rows, cols] whose row stride is a multiple of 8 elements."""
-    t = torch.empty((rows, (cols + 7) // 8 * 8), dtype=like.dtype, device=like.device)
-    return t if cols % 8 == 0 else t[:, :cols]
+    if cols % 8 == 0:
+        return like.new_empty((rows, cols))
+    return like.new_empty((rows, (cols + 7) // 8 * 8))[:, :cols]
 
 
 def _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, others) -> N.FoGatedFfnDesc:
-    if act not in GATE_ACTS:
+    code = GATE_ACTS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(GATE_ACTS)}")
     if b_layout not in ("kn", "nk"):
         raise ValueError("b_layout must be 'kn' or 'nk'")
     kn = b_layout == "kn"
-    d = N.FoGatedFfnDesc()
-    d.dtype, d.act, d.b_layout = _sixteen_bit(x.dtype, "x"), GATE_ACTS[act], N.FO_B_KN if kn else N.FO_B_NK
+    dt = x.dtype
     for t in (w_gate, w_up, w_down, *others):
-        if t.dtype != x.dtype:
+        if t.dtype is not dt:
             raise ValueError("every matrix of the block must share x's dtype")
-    d.x, d.ldx = x.data_ptr(), _rows(x, "x")
-    d.T, d.D = x.shape
-    d.ldwd = _rows(w_down, "w_down")
-    d.F, d.N = w_down.shape if kn else reversed(w_down.shape)
-    up = (d.D, d.F) if kn else (d.F, d.D)
-    d.ldwg, d.ldwu = _like(w_gate, up, "w_gate"), _like(w_up, up, "w_up")
+    T, D = _shape2(x, "x")
+    d = N.FoGatedFfnDesc()
+    d.dtype, d.act, d.b_layout = _sixteen_bit(dt, "x"), code, N.FO_B_KN if kn else N.FO_B_NK
+    if kn:
+        F, Nn = _shape2(w_down, "w_down")
+        d.ldwg, d.ldwu, d.ldwd = _ld(w_gate, D, F, "w_gate"), _ld(w_up, D, F, "w_up"), _ld(w_down, F, Nn, "w_down")
+    else:
+        Nn, F = _shape2(w_down, "w_down")
+        d.ldwg, d.ldwu, d.ldwd = _ld(w_gate, F, D, "w_gate"), _ld(w_up, F, D, "w_up"), _ld(w_down, Nn, F, "w_down")
+    d.T, d.D, d.F, d.N = T, D, F, Nn
+    d.x, d.ldx = x.data_ptr(), _ld(x, T, D, "x")
     d.w_gate, d.w_up, d.w_down = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
     return d
 
@@ -88,18 +116,20 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout, save=save)
-    dev = _require_cuda(x, w_gate, w_up, w_down)
+    dev = _cuda(x, w_gate, w_up, w_down)
     d = _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, ())
-    y = _matrix(d.T, d.N, x)
+    T, F, Nn = d.T, d.F, d.N
+    y = _matrix(T, Nn, x)
     d.y, d.ldy = y.data_ptr(), y.stride(0)
     if save:
-        g, u = _matrix(d.T, d.F, x), _matrix(d.T, d.F, x)
+        g, u = _matrix(T, F, x), _matrix(T, F, x)
         d.g, d.ldg, d.u, d.ldu = g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0)
     lib = N.lib()
-    need = lib.fo_gated_ffn_workspace_size(ctypes.byref(d), 0)
+    ref = ctypes.byref(d)
+    need = lib.fo_gated_ffn_workspace_size(ref, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    _run(dev, lib.fo_gated_ffn, ctypes.byref(d))
+    _run(dev, lib.fo_gated_ffn, ref)
     return (y, g, u) if save else y
 
 
@@ -110,48 +140,56 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn_backward(dy, x, w_gate, w_up, w_down, g, u, act=act, b_layout=b_layout)
-    dev = _require_cuda(x, dy, w_gate, w_up, w_down, g, u)
+    dev = _cuda(x, dy, w_gate, w_up, w_down, g, u)
     d = _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, (dy, g, u))
-    d.dy, d.lddy = dy.data_ptr(), _like(dy, (d.T, d.N), "dy")
-    d.g, d.ldg = g.data_ptr(), _like(g, (d.T, d.F), "g")
-    d.u, d.ldu = u.data_ptr(), _like(u, (d.T, d.F), "u")
+    T, F = d.T, d.F
+    d.dy, d.lddy = dy.data_ptr(), _ld(dy, T, d.N, "dy")
+    d.g, d.ldg = g.data_ptr(), _ld(g, T, F, "g")
+    d.u, d.ldu = u.data_ptr(), _ld(u, T, F, "u")
     dx, dwg, dwu, dwd = (_matrix(*t.shape, x) for t in (x, w_gate, w_up, w_down))
     d.dx, d.dw_gate, d.dw_up, d.dw_down = dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr()
     d.lddx, d.lddwg, d.lddwu, d.lddwd = dx.stride(0), dwg.stride(0), dwu.stride(0), dwd.stride(0)
     lib = N.lib()
-    need = lib.fo_gated_ffn_workspace_size(ctypes.byref(d), 1)
+    ref = ctypes.byref(d)
+    need = lib.fo_gated_ffn_workspace_size(ref, 1)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    _run(dev, lib.fo_gated_ffn_backward, ctypes.byref(d))
+    _run(dev, lib.fo_gated_ffn_backward, ref)
     return dx, dwg, dwu, dwd
 
 
 # ---------------------------------------------------------------------- norms around a block
+def _param(v: Optional[torch.Tensor], D: int, dt: torch.dtype, name: str) -> Optional[int]:
+    if v is None:
+        return None
+    if v.dtype is not dt:
+        raise ValueError("the norms' parameters and the gate must share one dtype")
+    return _vec(v, D, name).data_ptr()
+
+
 def _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps) -> N.FoBlockNormDesc:
-    if y.dim() != 2:
-        raise ValueError("y must be a 2-D tensor with unit column stride")
-    T, D = y.shape
+    T, D = _shape2(y, "y")
     if norm not in NORMS:
         raise ValueError(f"norm must be one of {sorted(NORMS)}")
-    vecs = [(_vec(v, D, name), name) for v, name in ((w_pre, "w_pre"), (w_post, "w_post"), (b_pre, "b_pre"), (b_post, "b_post"))]
     if w_pre is None:
         raise ValueError("w_pre is required")
+    dt = w_pre.dtype
     d = N.FoBlockNormDesc()
-    d.T, d.D, d.dtype, d.norm = T, D, _sixteen_bit(y.dtype, "y"), NORMS[norm]
-    d.vec_dtype = dtype_code(w_pre.dtype)
+    d.T, d.D, d.dtype, d.norm, d.vec_dtype = T, D, _sixteen_bit(y.dtype, "y"), NORMS[norm], dtype_code(dt)
     d.residual_scale, d.eps = residual_scale, eps
-    for v, name in vecs:
-        if v is not None:
-            if v.dtype != w_pre.dtype:
-                raise ValueError("the norms' parameters and the gate must share one dtype")
-            setattr(d, name, v.data_ptr())
+    d.y, d.ldy = y.data_ptr(), _ld(y, T, D, "y")
+    d.w_pre, d.w_post = _param(w_pre, D, dt, "w_pre"), _param(w_post, D, dt, "w_post")
+    d.b_pre, d.b_post = _param(b_pre, D, dt, "b_pre"), _param(b_post, D, dt, "b_post")
     if gate is not None:
-        g2 = gate.unsqueeze(0) if gate.dim() == 1 else gate
-        if gate.dtype != w_pre.dtype:
-            raise ValueError("the norms' parameters and the gate must share one dtype")
-        if g2.dim() != 2 or g2.shape[1] != D or g2.shape[0] == 0 or T % g2.shape[0]:
-            raise ValueError(f"gate must be [{D}] or [G, {D}] with G dividing T = {T}, got {list(gate.shape)}")
-        d.gate, d.gate_rows, d.ldgate = g2.data_ptr(), g2.shape[0], _rows(g2, "gate")
+        if gate.dim() == 1:
+            d.gate, d.gate_rows, d.ldgate = _param(gate, D, dt, "gate"), 1, D
+        else:
+            G = gate.shape[0]
+            if gate.dtype is not dt:
+                raise ValueError("the norms' parameters and the gate must share one dtype")
+            if gate.dim() != 2 or gate.shape[1] != D or G == 0 or T % G:
+                raise ValueError(f"gate must be [{D}] or [G, {D}] with G dividing T = {T}, got {list(gate.shape)}")
+            d.gate, d.gate_rows, d.ldgate = gate.data_ptr(), G, _ld(gate, G, D, "gate")
     return d
 
 
@@ -169,14 +207,14 @@ def block_norm(y: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tensor],
         with torch.cuda.stream(stream):
             return block_norm(y, x, w_post, w_pre, b_post=b_post, b_pre=b_pre, gate=gate, residual_scale=residual_scale,
                               norm=norm, eps=eps)
-    dev = _require_cuda(y, x, w_post, w_pre, b_post, b_pre, gate)
+    dev = _cuda(y, x, w_post, w_pre, b_post, b_pre, gate)
     d = _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps)
-    shape = (d.T, d.D)
-    if x.dtype != y.dtype:
+    if x.dtype is not y.dtype:
         raise ValueError("x and y must share one dtype")
-    d.y, d.ldy, d.x, d.ldx = y.data_ptr(), _rows(y, "y"), x.data_ptr(), _like(x, shape, "x")
-    r, z = (torch.empty(shape, dtype=y.dtype, device=dev) for _ in range(2))
-    d.r, d.z, d.ldr, d.ldz = r.data_ptr(), z.data_ptr(), d.D, d.D
+    T, D = y.shape
+    d.x, d.ldx = x.data_ptr(), _ld(x, T, D, "x")
+    r, z = y.new_empty((T, D)), y.new_empty((T, D))
+    d.r, d.z, d.ldr, d.ldz = r.data_ptr(), z.data_ptr(), D, D
     _run(dev, N.lib().fo_block_norm, ctypes.byref(d))
     return r, z
 
@@ -193,28 +231,29 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: torch.Tensor, y: torch.T
         with torch.cuda.stream(stream):
             return block_norm_backward(dr, dz, y, r, w_post, w_pre, b_post=b_post, b_pre=b_pre, gate=gate,
                                        residual_scale=residual_scale, norm=norm, eps=eps)
-    dev = _require_cuda(y, dr, dz, r, w_post, w_pre, b_post, b_pre, gate)
+    dev = _cuda(y, dr, dz, r, w_post, w_pre, b_post, b_pre, gate)
     d = _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps)
-    shape = (d.T, d.D)
+    T, D = y.shape
     for t, name in ((dr, "dr"), (dz, "dz"), (r, "r")):
-        if t is not None:
-            if t.dtype != y.dtype:
-                raise ValueError(f"{name} and y must share one dtype")
-            setattr(d, name, t.data_ptr())
-            setattr(d, "ld" + name, _like(t, shape, name))
-    d.y, d.ldy = y.data_ptr(), _rows(y, "y")
-    out = {k: torch.empty(shape, dtype=y.dtype, device=dev) for k in ("dy", "dx")}
-    d.lddy = d.lddx = d.D
+        if t is not None and t.dtype is not y.dtype:
+            raise ValueError(f"{name} and y must share one dtype")
+    if dr is not None:
+        d.dr, d.lddr = dr.data_ptr(), _ld(dr, T, D, "dr")
+    d.dz, d.lddz = dz.data_ptr(), _ld(dz, T, D, "dz")
+    d.r, d.ldr = r.data_ptr(), _ld(r, T, D, "r")
+    out = {"dy": y.new_empty((T, D)), "dx": y.new_empty((T, D))}
+    d.lddy = d.lddx = D
     for p, name in ((w_pre, "dw_pre"), (w_post, "dw_post"), (b_pre, "db_pre"), (b_post, "db_post"), (gate, "dgate")):
         if p is not None:
-            out[name] = torch.empty(p.shape, dtype=p.dtype, device=dev)
+            out[name] = p.new_empty(p.shape)
     for name, t in out.items():
         setattr(d, name, t.data_ptr())
     lib = N.lib()
-    need = lib.fo_block_norm_backward_workspace_size(ctypes.byref(d))
+    ref = ctypes.byref(d)
+    need = lib.fo_block_norm_backward_workspace_size(ref)
     ws = torch.empty(max(16, need), dtype=torch.uint8, device=dev)
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    _run(dev, lib.fo_block_norm_backward, ctypes.byref(d))
+    _run(dev, lib.fo_block_norm_backward, ref)
     return out
 
 
@@ -254,36 +293,41 @@ def quantize_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True) -> W4
 
 def _w4(w: W4, K: int, dtype: torch.dtype, name: str) -> Tuple[N.FoW4, int]:
     """The C form of a weight and its number of rows."""
-    if w.q.dim() != 2 or w.q.dtype != torch.uint8 or 2 * w.q.shape[1] != K:
-        raise ValueError(f"{name}.q must be uint8 [N, {K // 2}], got {w.q.dtype} {list(w.q.shape)}")
-    if w.group <= 0:
-        raise ValueError(f"{name}.group must be a positive multiple of 32, got {w.group}")
-    n, G = w.q.shape[0], -(-K // w.group)
-    if w.scales.dtype != dtype:
+    q, scales, zeros, group = w
+    if q.dim() != 2 or q.dtype is not torch.uint8 or 2 * q.shape[1] != K:
+        raise ValueError(f"{name}.q must be uint8 [N, {K // 2}], got {q.dtype} {list(q.shape)}")
+    if group <= 0:
+        raise ValueError(f"{name}.group must be a positive multiple of 32, got {group}")
+    n, G = q.shape[0], -(-K // group)
+    if scales.dtype is not dtype:
         raise ValueError(f"{name}.scales must be {dtype}, the activations' dtype")
-    if w.zeros is not None and w.zeros.dtype != torch.uint8:
+    if zeros is None:
+        return N.FoW4(q.data_ptr(), scales.data_ptr(), None, _ld(q, n, K // 2, name + ".q"),
+                      _ld(scales, n, G, name + ".scales"), 0, group), n
+    if zeros.dtype is not torch.uint8:
         raise ValueError(f"{name}.zeros must be uint8")
-    return N.FoW4(w.q.data_ptr(), w.scales.data_ptr(), None if w.zeros is None else w.zeros.data_ptr(),
-                  _rows(w.q, name + ".q"), _like(w.scales, (n, G), name + ".scales"),
-                  0 if w.zeros is None else _like(w.zeros, (n, G), name + ".zeros"), w.group), n
+    return N.FoW4(q.data_ptr(), scales.data_ptr(), zeros.data_ptr(), _ld(q, n, K // 2, name + ".q"),
+                  _ld(scales, n, G, name + ".scales"), _ld(zeros, n, G, name + ".zeros"), group), n
 
 
 def _matvec_w4(x, w, w_up, bias, act):
-    dev = _require_cuda(x, w.q, w.scales, w.zeros, bias, *(w_up[:3] if w_up is not None else ()))
+    dev = _cuda(x, w.q, w.scales, w.zeros, bias, *(w_up[:3] if w_up is not None else ()))
+    T, K = _shape2(x, "x")
+    dt = x.dtype
     d = N.FoMatvecW4Desc()
-    d.dtype, d.ldx = _sixteen_bit(x.dtype, "x"), _rows(x, "x")
-    d.T, d.K = x.shape
-    d.w, d.N = _w4(w, d.K, x.dtype, "w")
+    d.dtype, d.ldx = _sixteen_bit(dt, "x"), _ld(x, T, K, "x")
+    d.w, n = _w4(w, K, dt, "w")
+    d.T, d.K, d.N = T, K, n
     if w_up is not None:
-        d.w_up, n = _w4(w_up, d.K, x.dtype, "w_up")
-        if n != d.N:
-            raise ValueError(f"w_gate has {d.N} rows, w_up {n}")
+        d.w_up, m = _w4(w_up, K, dt, "w_up")
+        if m != n:
+            raise ValueError(f"w_gate has {n} rows, w_up {m}")
     if bias is not None:
-        if bias.dtype != x.dtype:
+        if bias.dtype is not dt:
             raise ValueError("bias must have the activations' dtype")
-        d.bias = _vec(bias, d.N, "bias").data_ptr()
-    out = torch.empty((d.T, d.N), dtype=x.dtype, device=dev)
-    d.x, d.out, d.ldo, d.act = x.data_ptr(), out.data_ptr(), d.N, act
+        d.bias = _vec(bias, n, "bias").data_ptr()
+    out = _matrix(T, n, x)
+    d.x, d.out, d.ldo, d.act = x.data_ptr(), out.data_ptr(), out.stride(0), act
     _run(dev, N.lib().fo_matvec_w4, ctypes.byref(d))
     return out
 

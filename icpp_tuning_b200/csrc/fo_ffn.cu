@@ -171,6 +171,28 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mat h{d->workspace, d->T, d->F, pad8(d->F)};
 
+  if (d->T <= 16 && d->D % 8 == 0 && d->F % 8 == 0 && d->N % 8 == 0) {
+    const int fmt = kn ? W_KN : W_NK, dt = d->dtype == FO_DT_BF16 ? DT_BF16 : DT_F16;
+    SkinnyParams s = {};
+    s.x = d->x, s.ldx = d->ldx;
+    s.T = static_cast<int>(d->T), s.N = static_cast<int>(d->F), s.K = static_cast<int>(d->D);
+    s.w[0] = d->w_gate, s.w[1] = d->w_up, s.ldw[0] = d->ldwg, s.ldw[1] = d->ldwu;
+    s.act = gate_act_of(d->act);
+    s.out = d->workspace, s.ldo = h.ld;
+    s.g = d->g, s.u = d->u, s.ldg = d->ldg, s.ldu = d->ldu;
+    cudaError_t e = launch_skinny(fmt, true, dt, s, hd.sms, st);
+    if (e != cudaSuccess) return fail_launch(e);
+    SkinnyParams o = {};
+    o.x = d->workspace, o.ldx = h.ld;
+    o.T = s.T, o.N = static_cast<int>(d->N), o.K = static_cast<int>(d->F);
+    o.w[0] = d->w_down, o.ldw[0] = d->ldwd;
+    o.out = d->y, o.ldo = d->ldy;
+    e = launch_skinny(fmt, false, dt, o, hd.sms, st);
+    if (e != cudaSuccess) return fail_launch(e);
+    host_count_launches(2);
+    return host_ok();
+  }
+
   Build b(d->dtype, hd);
   FfnProblem& q = b.add(d->T, d->F, d->D, kFfnTile / 2, 1);
   q.b_mn = kn;

@@ -39,17 +39,21 @@ inline bool host_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(
 
 // Launches `kern` as a programmatic dependent of the previous kernel on the stream (the
 // kernel calls griddep_wait before its first global access), as clusters of `cluster` CTAs
-// along x when cluster > 1.  `smem` above 48 KB is opted in once per device and kernel.
+// along x when cluster > 1.  More than the default 48 KB of shared memory (static and
+// dynamic) is opted in once per device and kernel.
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kern)(Params...), std::atomic<uint64_t>& opted, dim3 grid, dim3 block, int smem, int cluster,
                        cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024) {
+  if (smem > 32 * 1024) {
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if ((opted.load(std::memory_order_acquire) & bit) == 0) {
       RelaxedCapture relaxed;
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+      cudaFuncAttributes fa;  // the block's 227 KB hold its static shared memory too
+      cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - static_cast<int>(fa.sharedSizeBytes));
       if (e != cudaSuccess) return e;
       opted.fetch_or(bit, std::memory_order_acq_rel);
     }

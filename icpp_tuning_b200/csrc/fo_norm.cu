@@ -10,12 +10,21 @@
 //   dw_pre = sum dz rhat, dw_post = sum dn yhat, db_* = sum dz, sum dn, dgate = sum t n
 // ([.] in the LayerNorm form only; sums over rows).
 //
-// W warps own a row and hold all of it in registers (thread i the columns
-// (v * 32 W + i) * VEC ..), so each input value crosses HBM once and each output once: both
-// kernels are bound by HBM.  Statistics are fp32 and two-pass over the registers (mean,
-// then centred squares).
+// W warps own a row, 16 columns a thread (8 where a thread carries four sums a column).
+// Rows arrive by bulk copies in a ring of shared memory, several rows ahead, so the copies
+// never wait for a row's reductions.  A row that does not start or end on a 16-byte boundary
+// is copied as the 16-byte blocks around it, as far as they lie inside its tensor; what is
+// left of the tensor's first and last block is read directly.  Each value crosses HBM once:
+// both kernels are bound by HBM.
+// Statistics are fp32, of centred values in the LayerNorm form.  The backward pass needs one
+// round of sums a row (two in the LayerNorm form): mean(e yhat) is linear in t, so its three
+// parts sum(A y dr), sum(A y c), sum(A y r), A = gate w_post, join the round that gives rho
+// and mean(c rhat).  Of the parameter gradients only sum(dz rhat), q = sum(t yhat) (and
+// sum(dz), sum(t) with biases) are carried: dw_post = gate q, dgate = w_post q + b_post
+// sum(t), db_post = gate sum(t) are formed once a gate row, in the kernel that joins the
+// CTAs' sums in a fixed order.
 #include "fo_host.cuh"
-#include "fo_kernel.cuh"
+#include "fo_skinny.cuh"
 #include "../../include/b200fo.h"
 
 namespace fo {
@@ -30,61 +39,115 @@ struct NormParams {
   int rows_per_gate;  // rows sharing one gate row (T for a gate vector)
   int vec_dtype, layer;
   float scale, eps;
-  // backward: units of chunk_rows rows inside one gate group; partial sums of worker w in
-  // part_w[k][w][ldp] (k: w_pre, w_post, b_pre, b_post), of unit u in part_g[u][ldp]
-  int groups, chunks, chunk_rows, workers;
+  // work units: chunks of chunk_rows rows inside one gate group; backward, the sums of unit
+  // u go to part[u][k][ldp] (k: dz rhat, t yhat, dz, t)
+  int groups, chunks, chunk_rows;
   int ldp;
-  float *part_w, *part_g;
+  float* part;
+  int* status;
+  unsigned long long timeout_ns;
 };
 
-template <int DT, int VEC>
-struct RowVec {  // VEC values of a row as stored (16-bit)
-  uint32_t u[VEC == 8 ? 4 : 1];
-  __device__ __forceinline__ void load(const void* row, int c, int D) {
-    if constexpr (VEC == 8) {
-      uint4 q = make_uint4(0u, 0u, 0u, 0u);
-      if (c < D) q = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + c));
-      u[0] = q.x, u[1] = q.y, u[2] = q.z, u[3] = q.w;
-    } else {
-      u[0] = c < D ? __ldg(static_cast<const unsigned short*>(row) + c) : 0u;
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[VEC]) const {
-    if constexpr (VEC == 8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = unpack2<DT>(u[i]);
-        f[2 * i] = v.x;
-        f[2 * i + 1] = v.y;
-      }
-    } else {
-      f[0] = unpack2<DT>(u[0]).x;
-    }
-  }
+// Two fp32 values in one 64-bit register: sm_100 adds and multiplies both in one
+// instruction, which halves these kernels' arithmetic (they issue about 25 instructions a
+// value, and at twice that would be bound by issue, not by HBM).
+struct Two {
+  uint64_t v;
 };
-
-template <int DT, int VEC>
-__device__ __forceinline__ void store_vec(void* row, int c, int D, const float (&f)[VEC]) {
-  if (c >= D) return;
-  unsigned short* p = static_cast<unsigned short*>(row) + c;
-  if constexpr (VEC == 8) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]), pack2<DT>(f[4], f[5]), pack2<DT>(f[6], f[7]));
-  } else {
-    *p = static_cast<unsigned short>(pack2<DT>(f[0], 0.f) & 0xFFFFu);
-  }
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ Two two(float a) { return two(a, a); }
+__device__ __forceinline__ float2 both(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ float sum(Two a) {
+  const float2 f = both(a);
+  return f.x + f.y;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
-// VEC values of a parameter vector (`fill` where the vector is absent or c is past D).
-template <int VEC>
-__device__ __forceinline__ void load_param(const void* ptr, int dt, int c, int D, float fill, float (&f)[VEC]) {
-  if (ptr == nullptr || c >= D) {
+// Where a thread's NP pairs of columns lie.  VEC 8: pair e is columns 2 (e % 4) of the
+// 16-byte block (e / 4) * 32 W + tid; VEC 1: the single columns 2 e * 32 W + tid and
+// (2 e + 1) * 32 W + tid.
+template <int W, int VEC>
+struct Cols {
+  int tid, D;
+  __device__ __forceinline__ int first(int e) const { return VEC == 8 ? ((e >> 2) * 32 * W + tid) * 8 + 2 * (e & 3) : 2 * e * 32 * W + tid; }
+  __device__ __forceinline__ int second(int e) const { return VEC == 8 ? first(e) + 1 : first(e) + 32 * W; }
+  __device__ __forceinline__ bool in(int e) const { return first(e) < D; }        // VEC 8: both columns
+  __device__ __forceinline__ bool in2(int e) const { return VEC == 8 ? in(e) : second(e) < D; }
+  // VEC 1: a thread's i-th column (of 2 NP) can lie past the row: layouts take more than half
+  // of their columns, but for the smallest.
+  __device__ __forceinline__ static constexpr bool maybe_out(int i, int np) { return i >= np || (W == 1 && np == 4); }
+};
+
+// A parameter vector's pairs; `fill` where it is absent, 0 past D.  Every load is in bounds
+// and unconditional, so that they are all under way at once.
+template <int W, int VEC, int NP>
+__device__ __forceinline__ void load_param(const void* ptr, int dt, const Cols<W, VEC>& c, float fill, Two (&f)[NP]) {
+  float v[2 * NP];
+  if (ptr == nullptr) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = fill;
+    for (int i = 0; i < 2 * NP; ++i) v[i] = fill;
   } else if constexpr (VEC == 8) {
-    load_vec8(ptr, dt, c, f);
+#pragma unroll
+    for (int e = 0; e < NP; e += 4) {
+      float t[8];
+      load_vec8(ptr, dt, min(c.first(e), c.D - 8), t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[2 * e + i] = t[i];
+    }
+  } else if (dt == DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) v[i] = __ldg(static_cast<const float*>(ptr) + min(c.tid + i * 32 * W, c.D - 1));
   } else {
-    f[0] = load_vec(ptr, dt, c);
+    unsigned short raw[2 * NP];
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) raw[i] = __ldg(static_cast<const unsigned short*>(ptr) + min(c.tid + i * 32 * W, c.D - 1));
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) v[i] = dt == DT_BF16 ? __bfloat162float(__ushort_as_bfloat16(raw[i])) : __half2float(__ushort_as_half(raw[i]));
+  }
+#pragma unroll
+  for (int e = 0; e < NP; ++e) f[e] = two(c.in(e) ? v[2 * e] : 0.f, c.in2(e) ? v[2 * e + 1] : 0.f);
+}
+
+// Pairs e0 .. e0 + 3.
+template <int DT, int W, int VEC>
+__device__ __forceinline__ void store_row(void* row, const Cols<W, VEC>& c, int e0, const Two (&f)[4]) {
+  unsigned short* p = static_cast<unsigned short*>(row);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = both(f[i]);
+    w[i] = pack2<DT>(v.x, v.y);
+  }
+  if constexpr (VEC == 8) {
+    if (c.in(e0)) *reinterpret_cast<uint4*>(p + c.first(e0)) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c.in(e0 + i)) p[c.first(e0 + i)] = static_cast<unsigned short>(w[i] & 0xFFFFu);
+      if (c.in2(e0 + i)) p[c.second(e0 + i)] = static_cast<unsigned short>(w[i] >> 16);
+    }
   }
 }
 
@@ -92,293 +155,614 @@ __device__ __forceinline__ const void* vec_at(const void* ptr, int dt, long long
   return ptr == nullptr ? nullptr : static_cast<const char*>(ptr) + i * (dt == DT_F32 ? 4 : 2);
 }
 
-// Sums of N values over the W warps of a row.  Rounds alternate between two halves of the
-// scratch: a warp enters round k + 2 only after every warp has read round k (the barrier of
-// round k + 1 lies between), so one barrier a round is enough.
-template <int W, int N>
+// Sums of N <= 8 values over a warp: each butterfly step halves the values a lane carries
+// (value i ends in the lanes with those bits), so 8 values take 9 shuffles instead of 40.
+template <int N>
+__device__ __forceinline__ float warp_sums(const float (&v)[N], int lane) {
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = i < N ? v[i] : 0.f;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      if (i >= N) continue;  // both halves empty
+      const float keep = up ? a[i + o] : a[i], give = up ? a[i] : a[i + o];
+      a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  a[0] += __shfl_xor_sync(0xffffffffu, a[0], 8);
+  a[0] += __shfl_xor_sync(0xffffffffu, a[0], 16);
+  return a[0];  // lane l: the warp's sum of value l & 7
+}
+
+// Sums over the W warps of a row.  Rounds alternate between two halves of the scratch: a
+// warp enters round k + 2 only after every warp has read round k (the barrier of round
+// k + 1 lies between), so one barrier a round is enough.
+template <int W>
 struct RowSum {
-  float* red;  // [2][N][W] of this row group
+  float* red;  // [2][W][8] of this row group
   int round, bar;
+  template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N]) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (N == 1) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+      for (int o = 16; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      if constexpr (W > 1) {
+        float* s = red + round * 8 * W;
+        if (lane == 0) s[threadIdx.x >> 5] = v[0];
+        named_bar_sync(bar, 32 * W);
+        v[0] = s[lane & (W - 1)];
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if constexpr (W > 1) {
-      float* s = red + round * N * W;
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i * W + (threadIdx.x >> 5)] = v[i];
-      named_bar_sync(bar, 32 * W);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float t = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) t += s[i * W + w];
-        v[i] = t;
+        for (int o = W / 2; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        round ^= 1;
       }
+      return;
+    }
+    float mine = warp_sums(v, lane);  // lane l: value l & 7
+    if constexpr (W > 1) {
+      float* s = red + round * 8 * W;
+      if (lane < 8) s[(threadIdx.x >> 5) * 8 + lane] = mine;
+      named_bar_sync(bar, 32 * W);
+      mine = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w += 4)
+        if (W >= 4 || (lane >> 3) < W) mine += s[w * 8 + lane];  // warps w .. w + 3: eight lanes each
+      mine += __shfl_xor_sync(0xffffffffu, mine, 8);
+      mine += __shfl_xor_sync(0xffffffffu, mine, 16);
       round ^= 1;
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, mine, i);
   }
 };
 
-constexpr int rows_per_cta(int W) { return W >= 4 ? 1 : 4 / W; }
+constexpr int kCtaWarps = 8;
+constexpr int row_groups(int W) { return W >= kCtaWarps ? 1 : kCtaWarps / W; }
+constexpr int kBwdStages = 3;
 
-// hat[] = the normalised values of v[] (v itself on return is v - mean in the LayerNorm
-// form); returns rho.  Columns past D hold 0 and stay 0.
-template <int VEC, int NV, int W, class Sum>
-__device__ __forceinline__ float normalise(float (&v)[NV][VEC], const NormParams& p, Sum& sum, int tid) {
-  const float inv = 1.0f / static_cast<float>(p.D);
-  if (p.layer) {
-    float s[1] = {0.f};
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s[0] += v[j][i];
-    sum(s);
-    const float mean = s[0] * inv;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const bool in = (j * 32 * W + tid) * VEC < p.D;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = in ? v[j][i] - mean : 0.f;
-    }
-  }
-  float q[1] = {0.f};
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) q[0] = fmaf(v[j][i], v[j][i], q[0]);
-  sum(q);
-  return rsqrtf(fmaf(q[0], inv, p.eps));
+// Bytes of one row in the ring: every column a row group's threads hold (those past the row
+// stay zero), and with VEC 1 up to a 16-byte block more on either side.
+template <int W, int NP, int VEC>
+constexpr int ring_row() {
+  return NP * 2 * 32 * W * 2 + (VEC == 8 ? 0 : 32);
 }
 
-template <int DT, int W, int NV, int VEC>
-__global__ void __launch_bounds__(32 * W * rows_per_cta(W)) fo_norm_fwd_kernel(const NormParams p) {
-  __shared__ float red[rows_per_cta(W) * 2 * W];
-  const int tid = threadIdx.x;
-  RowSum<W, 1> sum{red + threadIdx.y * 2 * W, 0, 1 + static_cast<int>(threadIdx.y)};
-  griddep_launch_dependents();
-  griddep_wait();
-  for (int row = blockIdx.x * rows_per_cta(W) + threadIdx.y; row < p.T; row += gridDim.x * rows_per_cta(W)) {
-    const unsigned short* yr = static_cast<const unsigned short*>(p.y) + row * p.ldy;
-    const unsigned short* xr = static_cast<const unsigned short*>(p.x) + row * p.ldx;
-    RowVec<DT, VEC> yv[NV], xv[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) yv[j].load(yr, (j * 32 * W + tid) * VEC, p.D);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) xv[j].load(xr, (j * 32 * W + tid) * VEC, p.D);
-    float v[NV][VEC];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) yv[j].get(v[j]);
-    float rho = 1.f;
-    if (p.w_post != nullptr) rho = normalise<VEC, NV, W>(v, p, sum, tid);
-    const void* gate = p.gate == nullptr ? nullptr : vec_at(p.gate, p.vec_dtype, row / p.rows_per_gate * p.ldgate);
-    unsigned short* rr = static_cast<unsigned short*>(p.r) + row * p.ldr;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * W + tid) * VEC;
-      float w[VEC], b[VEC], g[VEC], x[VEC];
-      load_param(p.w_post, p.vec_dtype, c, p.D, 1.f, w);
-      load_param(p.b_post, p.vec_dtype, c, p.D, 0.f, b);
-      load_param(gate, p.vec_dtype, c, p.D, 1.f, g);
-      xv[j].get(x);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = fmaf(p.scale, x[i], g[i] * fmaf(v[j][i] * rho, w[i], b[i]));
-      store_vec<DT, VEC>(rr, c, p.D, v[j]);
+// One row group's ring and its columns: NT rows (one of each tensor) a stage.
+template <int DT, int NT, int NP, int VEC, int W, int S>
+struct Rows {
+  static constexpr int kRow = ring_row<W, NP, VEC>();
+  const NormParams& p;
+  Cols<W, VEC> c;
+  uint32_t ring, bars;  // shared addresses: stages, S mbarriers
+  int slot = 0;
+  uint32_t ph = 0;
+  bool ok = true;
+  // VEC 1: the current row's span of each tensor, and whether the ring holds all of them
+  int shift[VEC == 8 ? 1 : NT];
+  bool whole = true;
+
+  // Tensor k: forward y, x; backward r, dz, y, dr (null: not there, read as zero).  Addresses
+  // stay in the kernel's parameters, not in registers.
+  __device__ __forceinline__ const unsigned short* base(int k) const {
+    const void* const t = NT == 2 ? (k == 0 ? p.y : p.x) : (k == 0 ? p.r : k == 1 ? p.dz : k == 2 ? p.y : p.dr);
+    return static_cast<const unsigned short*>(t);
+  }
+  __device__ __forceinline__ long long ld(int k) const {
+    return NT == 2 ? (k == 0 ? p.ldy : p.ldx) : (k == 0 ? p.ldr : k == 1 ? p.lddz : k == 2 ? p.ldy : p.lddr);
+  }
+
+  // Where row `row` of tensor k lies: the blocks copied [from, to) and the offset of column 0
+  // in them (columns).
+  struct Span {
+    uintptr_t from;
+    uint32_t bytes;
+    int shift;
+  };
+  __device__ __forceinline__ Span span(int k, int row) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(base(k) + row * ld(k));
+    if constexpr (VEC == 8) return {a, static_cast<uint32_t>(c.D) * 2, 0};
+    const uintptr_t e = a + static_cast<uintptr_t>(c.D) * 2;
+    uintptr_t from = a & ~static_cast<uintptr_t>(15), to = (e + 15) & ~static_cast<uintptr_t>(15);
+    if (from < reinterpret_cast<uintptr_t>(base(k))) from += 16;
+    if (to > reinterpret_cast<uintptr_t>(base(k) + (p.T - 1) * ld(k) + c.D)) to -= 16;
+    const int shift = static_cast<int>(static_cast<intptr_t>(a - from)) / 2;
+    return {from, to > from ? static_cast<uint32_t>(to - from) : 0u, shift};
+  }
+  // The ring starts as zeros: what no copy fills (columns past the row, absent tensors) stays so.
+  __device__ __forceinline__ void init(uint8_t* smem, uint64_t* mbars) {
+    ring = smem_u32(smem), bars = smem_u32(mbars);
+    if (VEC == 8 && NP * 2 * 32 * W != c.D) {
+      for (int i = c.tid * 16; i < S * NT * kRow; i += 32 * W * 16) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
+    } else if (VEC == 8 && base(NT - 1) == nullptr) {
+      for (int i = c.tid * 16; i < S * NT * kRow; i += 32 * W * 16)
+        if (i / kRow % NT == NT - 1) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
     }
-    rho = normalise<VEC, NV, W>(v, p, sum, tid);
-    unsigned short* zr = static_cast<unsigned short*>(p.z) + row * p.ldz;
+    if (c.tid == 0) {
+      for (int i = 0; i < S; ++i) mbar_init(bars + 8 * i, 1);
+      fence_mbar_init();
+    }
+    fence_proxy_async_smem();  // the zeros come before the copies
+    __syncthreads();
+  }
+  // Asks for a row ahead of its use (row group's first thread).
+  __device__ __forceinline__ void ask(int ahead, int row) {
+    if (c.tid == 0 && ok) {
+      const int at = slot + ahead >= S ? slot + ahead - S : slot + ahead;
+      Span sp[NT];
+      uint32_t bytes = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * 32 * W + tid) * VEC;
-      float w[VEC], b[VEC];
-      load_param(p.w_pre, p.vec_dtype, c, p.D, 1.f, w);
-      load_param(p.b_pre, p.vec_dtype, c, p.D, 0.f, b);
+      for (int k = 0; k < NT; ++k)
+        if (base(k) != nullptr) sp[k] = span(k, row), bytes += sp[k].bytes;
+      mbar_arrive_expect_tx(bars + 8 * at, bytes);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = fmaf(v[j][i] * rho, w[i], b[i]);
-      store_vec<DT, VEC>(zr, c, p.D, v[j]);
+      for (int k = 0; k < NT; ++k)
+        if (base(k) != nullptr && (VEC == 8 || sp[k].bytes > 0))
+          bulk_load_g2s(ring + (at * NT + k) * kRow, reinterpret_cast<const void*>(sp[k].from), sp[k].bytes, bars + 8 * at);
     }
   }
-}
+  // Waits for the current stage's rows (bounded; once it ran out, no further wait).
+  __device__ __forceinline__ void take(int row) {
+    if constexpr (VEC == 1) {
+      whole = true;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        shift[k] = 0;
+        if (base(k) == nullptr) continue;
+        const Span sp = span(k, row);
+        shift[k] = sp.shift;
+        whole = whole && sp.shift >= 0 && static_cast<int>(sp.bytes / 2) - sp.shift >= c.D;
+      }
+    }
+    if (ok && !mbar_wait(bars + 8 * slot, ph, p.timeout_ns, nullptr)) {
+      ok = false;
+      if (atomicCAS(p.status, 0, kStatusTimeout) == 0) {
+        p.status[1] = 0x50;
+        p.status[2] = static_cast<int>(blockIdx.x);
+      }
+      for (int i = 0; i < S; ++i)  // let the copies in flight land before the CTA can end
+        mbar_wait(bars + 8 * ((slot + i) % S), ph ^ (slot + i >= S ? 1u : 0u), kDrainTimeoutNs, nullptr);
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if (++slot == S) slot = 0, ph ^= 1;
+  }
+  // Pairs e0 .. e0 + 3 of tensor k's row.
+  __device__ __forceinline__ void get(int k, int row, int e0, Two (&f)[4]) const {
+    const uint32_t at = ring + (slot * NT + k) * kRow;
+    if constexpr (VEC == 8) {
+      const uint4 q = lds128(at + c.first(e0) * 2);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2<DT>(w[i]);
+        f[i] = two(v.x, v.y);
+      }
+    } else {
+      if (base(k) == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = two(0.f);
+        return;
+      }
+      unsigned short raw[8];
+      const uint32_t src = at + 2 * (c.tid + shift[k]);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // in the ring's bounds for any column a thread holds
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[i]) : "r"(src + (2 * e0 + i) * 64 * W) : "memory");
+      } else {  // the tensor's first or last row: its first or last block is read directly
+        const int hi = static_cast<int>(span(k, row).bytes / 2) - shift[k];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int col = c.tid + (2 * e0 + i) * 32 * W;
+          raw[i] = 0;
+          if (col < c.D) {
+            if (col + shift[k] >= 0 && col < hi)
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[i]) : "r"(src + (2 * e0 + i) * 64 * W) : "memory");
+            else
+              raw[i] = __ldg(base(k) + row * ld(k) + col);
+          }
+        }
+      }
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = DT == DT_BF16 ? __bfloat162float(__ushort_as_bfloat16(raw[i])) : __half2float(__ushort_as_half(raw[i]));
+        if (c.maybe_out(2 * e0 + i, NP)) v[i] = c.tid + (2 * e0 + i) * 32 * W < c.D ? v[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = two(v[2 * i], v[2 * i + 1]);
+    }
+  }
+};
 
-// BIAS: the bias gradients are accumulated too.
-template <int DT, int W, int NV, int VEC, bool BIAS>
-__global__ void __launch_bounds__(32 * W * rows_per_cta(W)) fo_norm_bwd_kernel(const NormParams p) {
-  __shared__ float red[rows_per_cta(W) * 2 * 3 * W];
-  const int tid = threadIdx.x;
-  RowSum<W, 3> sum3{red + threadIdx.y * 2 * 3 * W, 0, 1 + static_cast<int>(threadIdx.y)};
-  const int worker = blockIdx.x * rows_per_cta(W) + threadIdx.y;
-  const float inv = 1.0f / static_cast<float>(p.D);
-  float a_wpre[NV][VEC] = {}, a_wpost[NV][VEC] = {}, a_gate[NV][VEC] = {};
-  float a_bpre[BIAS ? NV : 1][VEC] = {}, a_bpost[BIAS ? NV : 1][VEC] = {};
-  griddep_launch_dependents();
-  griddep_wait();
-  for (int u = worker; u < p.groups * p.chunks; u += p.workers) {
+// Walks this CTA's units; a unit's rows go to its row groups in turn.  fn.unit(grp) at a
+// unit's start, fn.row(row, ask) for each row, fn.done(u) at its end (the whole CTA calls it).
+// A row's `ask` refills the slot of the row before: it is called after the row's first round
+// of sums, when every warp is done with that one.
+template <int W, int S, class R, class Fn>
+__device__ __forceinline__ void walk(const NormParams& p, R& rows, Fn&& fn) {
+  constexpr int RG = row_groups(W);
+  for (int u = blockIdx.x; u < p.groups * p.chunks; u += gridDim.x) {
     const int grp = u / p.chunks, chunk = u - grp * p.chunks;
-    const int lo = grp * p.rows_per_gate + chunk * p.chunk_rows;
-    const int hi = min((grp + 1) * p.rows_per_gate, lo + p.chunk_rows);
-    const void* gate = p.gate == nullptr ? nullptr : vec_at(p.gate, p.vec_dtype, grp * p.ldgate);
-    for (int row = lo; row < hi; ++row) {
-      const unsigned short* rp[4] = {static_cast<const unsigned short*>(p.r) + row * p.ldr,
-                                     static_cast<const unsigned short*>(p.dz) + row * p.lddz,
-                                     static_cast<const unsigned short*>(p.y) + row * p.ldy,
-                                     static_cast<const unsigned short*>(p.dr) + row * p.lddr};
-      RowVec<DT, VEC> in[4][NV];
+    const int lo = grp * p.rows_per_gate + chunk * p.chunk_rows + static_cast<int>(threadIdx.y);
+    const int hi = min((grp + 1) * p.rows_per_gate, grp * p.rows_per_gate + (chunk + 1) * p.chunk_rows);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < NV; ++j) in[k][j].load(rp[k], (j * 32 * W + tid) * VEC, k == 3 && p.dr == nullptr ? 0 : p.D);
-      float mean_r = 0.f, mean_y = 0.f, mean_c = 0.f;
-      if (p.layer) {
-        float s[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          float r[VEC], z[VEC], y[VEC], w[VEC];
-          in[0][j].get(r), in[1][j].get(z), in[2][j].get(y);
-          load_param(p.w_pre, p.vec_dtype, (j * 32 * W + tid) * VEC, p.D, 1.f, w);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) s[0] += r[i], s[1] += y[i], s[2] = fmaf(z[i], w[i], s[2]);
-        }
-        sum3(s);
-        mean_r = s[0] * inv, mean_y = p.w_post != nullptr ? s[1] * inv : 0.f, mean_c = s[2] * inv;
-      }
-      float q[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float r[VEC], z[VEC], y[VEC], w[VEC];
-        in[0][j].get(r), in[1][j].get(z), in[2][j].get(y);
-        const int c = (j * 32 * W + tid) * VEC;
-        load_param(p.w_pre, p.vec_dtype, c, p.D, 1.f, w);
-        if (c < p.D)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float rc = r[i] - mean_r, yc = y[i] - mean_y;
-            q[0] = fmaf(rc, rc, q[0]);
-            q[1] = fmaf(yc, yc, q[1]);
-            q[2] = fmaf(z[i] * w[i], rc, q[2]);
-          }
-      }
-      sum3(q);
-      const float rho_r = rsqrtf(fmaf(q[0], inv, p.eps));
-      const float rho_y = p.w_post != nullptr ? rsqrtf(fmaf(q[1], inv, p.eps)) : 1.f;
-      const float m_c = q[2] * inv * rho_r;  // mean(c rhat)
-      float t[NV][VEC];
-      float s[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = (j * 32 * W + tid) * VEC;
-        float r[VEC], z[VEC], y[VEC], d[VEC], w[VEC], wp[VEC], bp[VEC], g[VEC], dx[VEC];
-        in[0][j].get(r), in[1][j].get(z), in[2][j].get(y), in[3][j].get(d);
-        load_param(p.w_pre, p.vec_dtype, c, p.D, 1.f, w);
-        load_param(p.w_post, p.vec_dtype, c, p.D, 1.f, wp);
-        load_param(p.b_post, p.vec_dtype, c, p.D, 0.f, bp);
-        load_param(gate, p.vec_dtype, c, p.D, 1.f, g);
-        const bool inb = c < p.D;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float rh = inb ? (r[i] - mean_r) * rho_r : 0.f;
-          const float yh = inb ? (y[i] - mean_y) * rho_y : 0.f;
-          const float tt = inb ? d[i] + rho_r * (fmaf(z[i], w[i], -mean_c) - rh * m_c) : 0.f;
-          dx[i] = p.scale * tt;
-          a_wpre[j][i] = fmaf(z[i], rh, a_wpre[j][i]);
-          const float dn = g[i] * tt;
-          a_wpost[j][i] = fmaf(dn, yh, a_wpost[j][i]);
-          a_gate[j][i] = fmaf(tt, fmaf(yh, wp[i], bp[i]), a_gate[j][i]);
-          if constexpr (BIAS) {
-            a_bpre[j][i] += z[i];
-            a_bpost[j][i] += dn;
-          }
-          t[j][i] = dn * wp[i];  // e
-          s[0] = fmaf(t[j][i], yh, s[0]);
-          s[1] += t[j][i];
-        }
-        store_vec<DT, VEC>(static_cast<unsigned short*>(p.dx) + row * p.lddx, c, p.D, dx);
-      }
-      float m_e = 0.f, mean_e = 0.f;
-      if (p.w_post != nullptr) {
-        sum3(s);
-        m_e = s[0] * inv;
-        mean_e = p.layer ? s[1] * inv : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float y[VEC];
-        in[2][j].get(y);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (p.w_post != nullptr) t[j][i] = rho_y * (t[j][i] - mean_e - (y[i] - mean_y) * rho_y * m_e);
-        store_vec<DT, VEC>(static_cast<unsigned short*>(p.dy) + row * p.lddy, (j * 32 * W + tid) * VEC, p.D, t[j]);
-      }
+    for (int i = 0; i < S - 1; ++i)
+      if (lo + i * RG < hi) rows.ask(i, lo + i * RG);
+    fn.unit(grp);
+    for (int row = lo; row < hi; row += RG) {
+      rows.take(row);
+      fn.row(row, [&] {
+        if (row + (S - 1) * RG < hi) rows.ask(S - 1, row + (S - 1) * RG);
+      });
+      rows.next();
     }
-    if (p.gate != nullptr) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int c = (j * 32 * W + tid) * VEC + i;
-          if (c < p.D) p.part_g[static_cast<long long>(u) * p.ldp + c] = a_gate[j][i];
-          a_gate[j][i] = 0.f;
-        }
-    }
-  }
-  if (worker < p.workers) {
-    const long long stride = static_cast<long long>(p.workers) * p.ldp;
-    float* base = p.part_w + static_cast<long long>(worker) * p.ldp;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = (j * 32 * W + tid) * VEC + i;
-        if (c >= p.D) continue;
-        base[c] = a_wpre[j][i];
-        if (p.w_post != nullptr) base[stride + c] = a_wpost[j][i];
-        if constexpr (BIAS) {
-          base[2 * stride + c] = a_bpre[j][i];
-          base[3 * stride + c] = a_bpost[j][i];
-        }
-      }
+    fn.done(u);
   }
 }
 
-// Joins the partial sums in a fixed order: block (output row, 64 columns).  Output rows
-// 0..3 are the parameter vectors (all workers), 4 + g the gate rows (their own chunks).
-struct JoinParams {
-  const float *part_w, *part_g;
-  void* out[5];  // dw_pre, dw_post, db_pre, db_post, dgate; null: not wanted
-  int workers, chunks, ldp, D, vec_dtype;
+// v - mean in the columns of the row, 0 past them.
+template <int W, int VEC, int NP>
+__device__ __forceinline__ void centre(Two (&v)[NP], float mean, const Cols<W, VEC>& c, int e0 = 0) {
+  const Two m = two(-mean);
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+    const float2 f = both(add2(v[e], m));
+    v[e] = two(c.in(e0 + e) ? f.x : 0.f, c.in2(e0 + e) ? f.y : 0.f);
+  }
+}
+
+template <int DT, int W, int NP, int VEC, bool LAYER, int S>
+struct FwdRow {
+  const NormParams& p;
+  Rows<DT, 2, NP, VEC, W, S>& in;  // y, x
+  RowSum<W> sums;
+  Two a[NP], w[NP];                                  // gate * w_post, w_pre
+  Two b[LAYER ? NP : 1], bw[LAYER ? NP : 1];         // gate * b_post, b_pre
+
+  __device__ __forceinline__ void unit(int grp) {
+    const void* gate = p.gate == nullptr ? nullptr : vec_at(p.gate, p.vec_dtype, grp * p.ldgate);
+    Two g[NP];
+    load_param(gate, p.vec_dtype, in.c, 1.f, g);
+    load_param(p.w_post, p.vec_dtype, in.c, 1.f, a);
+    load_param(p.w_pre, p.vec_dtype, in.c, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < NP; ++e) a[e] = mul2(a[e], g[e]);
+    if constexpr (LAYER) {
+      load_param(p.b_post, p.vec_dtype, in.c, 0.f, b);
+      load_param(p.b_pre, p.vec_dtype, in.c, 0.f, bw);
+#pragma unroll
+      for (int e = 0; e < NP; ++e) b[e] = mul2(b[e], g[e]);
+    }
+  }
+  __device__ __forceinline__ float rho(Two (&v)[NP], float inv) {  // v becomes v - mean in the LayerNorm form
+    if constexpr (LAYER) {
+      Two t = two(0.f);
+#pragma unroll
+      for (int e = 0; e < NP; ++e) t = add2(t, v[e]);
+      float s[1] = {sum(t)};
+      sums(s);
+      centre(v, s[0] * inv, in.c);
+    }
+    Two t = two(0.f);
+#pragma unroll
+    for (int e = 0; e < NP; ++e) t = fma2(v[e], v[e], t);
+    float q[1] = {sum(t)};
+    sums(q);
+    return rsqrtf(fmaf(q[0], inv, p.eps));
+  }
+  template <class Ask>
+  __device__ __forceinline__ void row(int r, Ask&& ask) {
+    const float inv = 1.0f / static_cast<float>(in.c.D);
+    Two v[NP];
+#pragma unroll
+    for (int e0 = 0; e0 < NP; e0 += 4) {
+      Two y[4];
+      in.get(0, r, e0, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e0 + i] = y[i];
+    }
+    float k = 1.f;
+    if (p.w_post != nullptr) {
+      k = rho(v, inv);
+      ask();
+    }
+    const Two k2 = two(k), sc = two(p.scale);
+    unsigned short* rr = static_cast<unsigned short*>(p.r) + r * p.ldr;
+#pragma unroll
+    for (int e0 = 0; e0 < NP; e0 += 4) {
+      Two x[4];
+      in.get(1, r, e0, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i;
+        if constexpr (LAYER) x[i] = fma2(sc, x[i], b[e]);
+        else x[i] = mul2(sc, x[i]);
+        v[e] = x[i] = fma2(mul2(v[e], k2), a[e], x[i]);
+      }
+      store_row<DT>(rr, in.c, e0, x);
+    }
+    k = rho(v, inv);
+    if (p.w_post == nullptr) ask();
+    const Two k3 = two(k);
+    unsigned short* zr = static_cast<unsigned short*>(p.z) + r * p.ldz;
+#pragma unroll
+    for (int e0 = 0; e0 < NP; e0 += 4) {
+      Two z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i;
+        if constexpr (LAYER) z[i] = fma2(mul2(v[e], k3), w[e], bw[e]);
+        else z[i] = mul2(mul2(v[e], k3), w[e]);
+      }
+      store_row<DT>(zr, in.c, e0, z);
+    }
+  }
+  __device__ __forceinline__ void done(int) {}
 };
 
-constexpr int kJoinSplit = 16;
+template <int DT, int W, int NP, int VEC, bool LAYER, int S>
+__global__ void __launch_bounds__(32 * W * row_groups(W)) fo_norm_fwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr int RG = row_groups(W);
+  extern __shared__ __align__(128) uint8_t smem_norm[];
+  __shared__ float red[RG * 2 * 8 * W];
+  __shared__ __align__(8) uint64_t bars[RG * S];
+  Rows<DT, 2, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
+  in.init(smem_norm + threadIdx.y * S * 2 * in.kRow, bars + threadIdx.y * S);
+  FwdRow<DT, W, NP, VEC, LAYER, S> f{p, in, {red + threadIdx.y * 2 * 8 * W, 0, 1 + static_cast<int>(threadIdx.y)}, {}, {}, {}, {}};
+  griddep_wait();
+  griddep_launch_dependents();
+  walk<W, S>(p, in, f);
+}
+
+template <int DT, int W, int NP, int VEC, bool LAYER>
+struct BwdRow {
+  static constexpr int kSums = LAYER ? 4 : 2;  // dz rhat, t yhat; and dz, t for the biases
+  const NormParams& p;
+  Rows<DT, 4, NP, VEC, W, kBwdStages>& in;  // r, dz, y, dr
+  RowSum<W> sums;
+  float* joint;  // [kSums][ldp] where the row groups of a CTA meet
+  Two w[NP], a[NP];  // w_pre, gate * w_post
+  Two acc[kSums][NP];
+
+  __device__ __forceinline__ void unit(int grp) {
+    const void* gate = p.gate == nullptr ? nullptr : vec_at(p.gate, p.vec_dtype, grp * p.ldgate);
+    Two g[NP];
+    load_param(gate, p.vec_dtype, in.c, 1.f, g);
+    load_param(p.w_post, p.vec_dtype, in.c, 1.f, a);
+    load_param(p.w_pre, p.vec_dtype, in.c, 0.f, w);
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
+      a[e] = mul2(a[e], g[e]);
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) acc[k][e] = two(0.f);
+    }
+  }
+  template <class Ask>
+  __device__ __forceinline__ void row(int rw, Ask&& ask) {
+    const float inv = 1.0f / static_cast<float>(in.c.D);
+    const bool post = p.w_post != nullptr;
+    float mr = 0.f, my = 0.f, mc = 0.f;
+    // With 4 pairs a thread the row stays in registers; with 8 each pass reads the ring again.
+    constexpr bool kHold = NP == 4;
+    Two hr[4], hz[4], hy[4], hd[4];
+    auto fetch = [&](int e0, Two (&r)[4], Two (&z)[4], Two (&y)[4], Two (&d)[4]) {
+      if constexpr (kHold) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = hr[i], z[i] = hz[i], y[i] = hy[i], d[i] = hd[i];
+      } else {
+        in.get(0, rw, e0, r), in.get(1, rw, e0, z), in.get(2, rw, e0, y), in.get(3, rw, e0, d);
+        if constexpr (LAYER) centre(r, mr, in.c, e0), centre(y, my, in.c, e0);
+      }
+    };
+    if constexpr (kHold) in.get(0, rw, 0, hr), in.get(1, rw, 0, hz), in.get(2, rw, 0, hy), in.get(3, rw, 0, hd);
+    if constexpr (LAYER) {
+      Two s0 = two(0.f), s1 = s0, s2 = s0;
+#pragma unroll
+      for (int e0 = 0; e0 < NP; e0 += 4) {
+        Two r[4], z[4], y[4];
+        if constexpr (kHold) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = hr[i], z[i] = hz[i], y[i] = hy[i];
+        } else {
+          in.get(0, rw, e0, r), in.get(1, rw, e0, z), in.get(2, rw, e0, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s0 = add2(s0, r[i]), s1 = add2(s1, y[i]), s2 = fma2(z[i], w[e0 + i], s2);
+      }
+      float s[3] = {sum(s0), sum(s1), sum(s2)};
+      sums(s);
+      mr = s[0] * inv, my = post ? s[1] * inv : 0.f, mc = s[2] * inv;
+      if constexpr (kHold) centre(hr, mr, in.c), centre(hy, my, in.c);
+    }
+    const Two mc2 = two(-mc);
+    float kr, ky, m, me, me0 = 0.f;
+    {
+      // r^2, y^2, c r, A y dr, A y c, A y r, and in the LayerNorm form A dr, A c, A r
+      Two t[6], l[3];
+#pragma unroll
+      for (int i = 0; i < 6; ++i) t[i] = two(0.f);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) l[i] = two(0.f);
+#pragma unroll
+      for (int e0 = 0; e0 < NP; e0 += 4) {
+        Two r[4], z[4], y[4], d[4];
+        fetch(e0, r, z, y, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = e0 + i;
+          const Two ay = mul2(a[e], y[i]), c = LAYER ? fma2(z[i], w[e], mc2) : mul2(z[i], w[e]);
+          t[0] = fma2(r[i], r[i], t[0]);
+          t[1] = fma2(y[i], y[i], t[1]);
+          t[2] = fma2(c, r[i], t[2]);
+          t[3] = fma2(ay, d[i], t[3]);
+          t[4] = fma2(ay, c, t[4]);
+          t[5] = fma2(ay, r[i], t[5]);
+          if constexpr (LAYER) {
+            l[0] = fma2(a[e], d[i], l[0]);
+            l[1] = fma2(a[e], c, l[1]);
+            l[2] = fma2(a[e], r[i], l[2]);
+          }
+        }
+      }
+      float q[6];
+#pragma unroll
+      for (int i = 0; i < 6; ++i) q[i] = sum(t[i]);
+      sums(q);
+      ask();
+      kr = rsqrtf(fmaf(q[0], inv, p.eps)), ky = post ? rsqrtf(fmaf(q[1], inv, p.eps)) : 1.f;
+      m = q[2] * inv * kr;  // mean(c rhat)
+      // mean(e yhat) of e = A t, t = dr + kr c - kr kr m r
+      me = post ? ky * inv * fmaf(kr, fmaf(-kr * m, q[5], q[4]), q[3]) : 0.f;
+      if constexpr (LAYER) {
+        float s[3] = {sum(l[0]), sum(l[1]), sum(l[2])};
+        sums(s);
+        me0 = post ? inv * fmaf(kr, fmaf(-kr * m, s[2], s[1]), s[0]) : 0.f;
+      }
+    }
+    const Two kr2 = two(kr), ky2 = two(ky), nm = two(-m), nme = two(-me), sc = two(p.scale);
+    const Two nme0 = two(-me0);
+    unsigned short* dxr = static_cast<unsigned short*>(p.dx) + rw * p.lddx;
+    unsigned short* dyr = static_cast<unsigned short*>(p.dy) + rw * p.lddy;
+#pragma unroll
+    for (int e0 = 0; e0 < NP; e0 += 4) {
+      Two r[4], z[4], y[4], d[4], o[4];
+      fetch(e0, r, z, y, d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i;
+        const Two rh = mul2(r[i], kr2), yh = mul2(y[i], ky2);
+        const Two c = LAYER ? fma2(z[i], w[e], mc2) : mul2(z[i], w[e]);
+        const Two t = fma2(kr2, fma2(rh, nm, c), d[i]);
+        acc[0][e] = fma2(z[i], rh, acc[0][e]);
+        acc[1][e] = fma2(t, yh, acc[1][e]);
+        if constexpr (LAYER) acc[2][e] = add2(acc[2][e], z[i]), acc[3][e] = add2(acc[3][e], t);
+        d[i] = mul2(sc, t);
+        Two q = fma2(yh, nme, mul2(a[e], t));
+        if constexpr (LAYER) q = add2(q, nme0);
+        o[i] = mul2(ky2, q);
+      }
+      store_row<DT>(dxr, in.c, e0, d);
+      store_row<DT>(dyr, in.c, e0, o);
+    }
+  }
+  __device__ __forceinline__ void done(int u) {
+    constexpr int RG = row_groups(W);
+    float* out = p.part + static_cast<long long>(u) * 4 * p.ldp;
+#pragma unroll 1
+    for (int g = 0; g < RG; ++g) {  // the row groups add up in turn, the last one writes
+      if (g == static_cast<int>(threadIdx.y)) {
+#pragma unroll
+        for (int k = 0; k < kSums; ++k)
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            const float2 v = both(acc[k][e]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int at = k * p.ldp + (h ? in.c.second(e) : in.c.first(e));
+              if (!(h ? in.c.in2(e) : in.c.in(e))) continue;
+              const float t = (h ? v.y : v.x) + (g == 0 ? 0.f : joint[at]);
+              if (g == RG - 1) out[at] = t;
+              else joint[at] = t;
+            }
+          }
+      }
+      if (RG > 1) __syncthreads();
+    }
+  }
+};
+
+template <int DT, int W, int NP, int VEC, bool LAYER>
+__global__ void __launch_bounds__(32 * W * row_groups(W), W == 16 ? 1 : 2) fo_norm_bwd_kernel(const __grid_constant__ NormParams p) {
+  constexpr int RG = row_groups(W), S = kBwdStages;
+  extern __shared__ __align__(128) uint8_t smem_norm[];
+  __shared__ float red[RG * 2 * 8 * W];
+  __shared__ __align__(8) uint64_t bars[RG * S];
+  Rows<DT, 4, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
+  in.init(smem_norm + threadIdx.y * S * 4 * in.kRow, bars + threadIdx.y * S);
+  float* joint = reinterpret_cast<float*>(smem_norm + RG * S * 4 * in.kRow);
+  BwdRow<DT, W, NP, VEC, LAYER> f{p, in, {red + threadIdx.y * 2 * 8 * W, 0, 1 + static_cast<int>(threadIdx.y)}, joint, {}, {}, {}};
+  griddep_wait();
+  griddep_launch_dependents();
+  walk<W, S>(p, in, f);
+}
+
+// Joins the units' sums in a fixed order and forms the parameter gradients: block (output
+// row, 64 columns).  Output rows 0..3 are dw_pre, dw_post, db_pre, db_post (all units), 4 + g
+// the gate rows (their own chunks).
+struct JoinParams {
+  const float* part;
+  void* out[5];  // dw_pre, dw_post, db_pre, db_post, dgate; null: not wanted
+  const void *w_post, *b_post, *gate;
+  long long ldgate;
+  int units, chunks, ldp, D, vec_dtype;
+};
+
+constexpr int kJoinSplit = 32;
 
 __global__ void __launch_bounds__(16 * kJoinSplit) fo_norm_join_kernel(const JoinParams p) {
-  __shared__ float4 red[kJoinSplit][16];
+  __shared__ float4 red[2][kJoinSplit][16];
   griddep_launch_dependents();
   griddep_wait();
   const int k = min(static_cast<int>(blockIdx.x), 4);
   if (p.out[k] == nullptr) return;
   const int g = static_cast<int>(blockIdx.x) - 4;
-  const int n = k < 4 ? p.workers : p.chunks;
-  const float* src = k < 4 ? p.part_w + static_cast<long long>(k) * p.workers * p.ldp
-                           : p.part_g + static_cast<long long>(g) * p.chunks * p.ldp;
+  const int lo = k < 4 ? 0 : g * p.chunks, hi = k < 4 ? p.units : lo + p.chunks;
   const int lane = threadIdx.x & 15, split = threadIdx.x >> 4;
   const int c = blockIdx.y * 64 + lane * 4;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool gated = (k == 1 || k == 3) && p.gate != nullptr;  // sums weighted by each unit's gate row
+  // dw_pre: dz rhat; dw_post, dgate: t yhat; db_pre: dz; db_post (and dgate's bias part): t
+  const int slot = k == 0 ? 0 : k == 2 ? 2 : k == 3 ? 3 : 1;
+  float a[2][4] = {};
   if (c < p.ldp) {
-#pragma unroll 4
-    for (int i = split; i < n; i += kJoinSplit) {
-      const float4 q = __ldcg(reinterpret_cast<const float4*>(src + static_cast<long long>(i) * p.ldp + c));
-      a.x += q.x, a.y += q.y, a.z += q.z, a.w += q.w;
+    const float* src = p.part + static_cast<long long>(slot) * p.ldp + c;
+    int grp = -1;
+    float gv[4] = {1.f, 1.f, 1.f, 1.f};
+    for (int u0 = lo + split; u0 < hi; u0 += 4 * kJoinSplit) {  // four loads under way at once
+      float4 q[4], t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int u = u0 + i * kJoinSplit;
+        q[i] = t[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (u < hi) {
+          q[i] = __ldcg(reinterpret_cast<const float4*>(src + static_cast<long long>(u) * 4 * p.ldp));
+          if (k == 4 && p.b_post != nullptr) t[i] = __ldcg(reinterpret_cast<const float4*>(src + (static_cast<long long>(u) * 4 + 2) * p.ldp));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int u = u0 + i * kJoinSplit;
+        if (gated && u < hi && u / p.chunks != grp) {
+          grp = u / p.chunks;
+          const void* row = vec_at(p.gate, p.vec_dtype, grp * p.ldgate);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) gv[j] = c + j < p.D ? load_vec(row, p.vec_dtype, c + j) : 0.f;
+        }
+        a[0][0] = fmaf(q[i].x, gv[0], a[0][0]), a[0][1] = fmaf(q[i].y, gv[1], a[0][1]);
+        a[0][2] = fmaf(q[i].z, gv[2], a[0][2]), a[0][3] = fmaf(q[i].w, gv[3], a[0][3]);
+        a[1][0] += t[i].x, a[1][1] += t[i].y, a[1][2] += t[i].z, a[1][3] += t[i].w;
+      }
     }
   }
-  red[split][lane] = a;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) red[h][split][lane] = make_float4(a[h][0], a[h][1], a[h][2], a[h][3]);
   __syncthreads();
   if (threadIdx.x < 64) {
     const int cc = blockIdx.y * 64 + threadIdx.x;
-    float t = 0.f;
+    float t = 0.f, t1 = 0.f;
 #pragma unroll
-    for (int s = 0; s < kJoinSplit; ++s) t += reinterpret_cast<const float*>(red[s])[threadIdx.x];
+    for (int s = 0; s < kJoinSplit; ++s) {
+      t += reinterpret_cast<const float*>(red[0][s])[threadIdx.x];
+      t1 += reinterpret_cast<const float*>(red[1][s])[threadIdx.x];
+    }
     if (cc < p.D) {
+      if (k == 4) {
+        if (p.w_post != nullptr) t *= load_vec(p.w_post, p.vec_dtype, cc);
+        if (p.b_post != nullptr) t = fmaf(load_vec(p.b_post, p.vec_dtype, cc), t1, t);
+      }
       const long long at = (k < 4 ? 0 : static_cast<long long>(g) * p.D) + cc;
       if (p.vec_dtype == DT_F32) static_cast<float*>(p.out[k])[at] = t;
       if (p.vec_dtype == DT_BF16) static_cast<__nv_bfloat16*>(p.out[k])[at] = __float2bfloat16_rn(t);
@@ -392,44 +776,62 @@ using NormKernel = void (*)(const NormParams);
 
 struct Shape {
   NormKernel kern;
-  int warps;
-  std::atomic<int>* per_sm;  // resident CTAs of a SM, queried once
+  int warps, smem;
+  std::atomic<uint64_t>* opted;
 };
 
-template <int DT, int W, int NV, int VEC>
-Shape fwd_entry() {
-  static std::atomic<int> n{0};
-  return {fo_norm_fwd_kernel<DT, W, NV, VEC>, W, &n};
+template <int DT, int W, int NP, int VEC, bool LAYER, int S = 4>
+Shape fwd_entry(int) {
+  static std::atomic<uint64_t> opted{0};
+  return {fo_norm_fwd_kernel<DT, W, NP, VEC, LAYER, S>, W, row_groups(W) * S * 2 * ring_row<W, NP, VEC>(), &opted};
 }
 
-template <int DT, int W, int NV, int VEC, bool BIAS>
-Shape bwd_entry() {
-  return {fo_norm_bwd_kernel<DT, W, NV, VEC, BIAS>, W, nullptr};
+template <int DT, int W, int NP, int VEC, bool LAYER>
+Shape bwd_entry(int D) {
+  static std::atomic<uint64_t> opted{0};
+  const int joint = row_groups(W) > 1 ? (LAYER ? 4 : 2) * ((D + 3) / 4 * 4) * 4 : 0;
+  return {fo_norm_bwd_kernel<DT, W, NP, VEC, LAYER>, W, row_groups(W) * kBwdStages * 4 * ring_row<W, NP, VEC>() + joint, &opted};
 }
 
-// The row layout for D columns: the fewest warps whose threads hold at most NV vectors of
-// 8 (32 columns a thread forward, 16 backward, where each column also carries its sums).
-template <int DT, int VEC>
+// The row layout for D columns: the fewest warps whose threads hold at most 8 pairs; 4 pairs
+// where a thread carries four sums a column (with 8 the LayerNorm form's backward pass spills).
+#define FO_NORM_SHAPES(entry, pairs4, vec)                 \
+  if constexpr (!(pairs4)) {                               \
+    if (D <= 256) return entry<DT, 1, 4, vec, LAYER>(D);   \
+    if (D <= 512) return entry<DT, 1, 8, vec, LAYER>(D);   \
+    if (D <= 1024) return entry<DT, 2, 8, vec, LAYER>(D);  \
+    if (D <= 2048) return entry<DT, 4, 8, vec, LAYER>(D);  \
+    if (D <= 4096) return entry<DT, 8, 8, vec, LAYER>(D);  \
+  } else {                                                 \
+    if (D <= 256) return entry<DT, 1, 4, vec, LAYER>(D);   \
+    if (D <= 512) return entry<DT, 2, 4, vec, LAYER>(D);   \
+    if (D <= 1024) return entry<DT, 4, 4, vec, LAYER>(D);  \
+    if (D <= 2048) return entry<DT, 8, 4, vec, LAYER>(D);  \
+    if (D <= 4096) return entry<DT, 16, 4, vec, LAYER>(D); \
+  }
+
+template <int DT, int VEC, bool LAYER>
 Shape fwd_shape(int D) {
-  constexpr int M = VEC == 8 ? 1 : 8;
-  if (D <= 256) return fwd_entry<DT, 1, 1 * M, VEC>();
-  if (D <= 512) return fwd_entry<DT, 1, 2 * M, VEC>();
-  if (D <= 1024) return fwd_entry<DT, 2, 2 * M, VEC>();
-  if (D <= 2048) return fwd_entry<DT, 4, 2 * M, VEC>();
-  if (D <= 4096) return fwd_entry<DT, 8, 2 * M, VEC>();
-  if (D <= 8192) return fwd_entry<DT, 16, 2 * M, VEC>();
-  return fwd_entry<DT, 16, 4 * M, VEC>();
+  FO_NORM_SHAPES(fwd_entry, false, VEC)
+  if (D <= 8192) return fwd_entry<DT, 16, 8, VEC, LAYER>(D);
+  return fwd_entry<DT, 16, 16, VEC, LAYER, 3>(D);
 }
 
-template <int DT, int VEC, bool BIAS>
+template <int DT, int VEC, bool LAYER>
 Shape bwd_shape(int D) {
-  constexpr int M = VEC == 8 ? 1 : 8;
-  if (D <= 256) return bwd_entry<DT, 1, 1 * M, VEC, BIAS>();
-  if (D <= 512) return bwd_entry<DT, 1, 2 * M, VEC, BIAS>();
-  if (D <= 1024) return bwd_entry<DT, 2, 2 * M, VEC, BIAS>();
-  if (D <= 2048) return bwd_entry<DT, 4, 2 * M, VEC, BIAS>();
-  if (D <= 4096) return bwd_entry<DT, 8, 2 * M, VEC, BIAS>();
-  return bwd_entry<DT, 16, 2 * M, VEC, BIAS>();
+  FO_NORM_SHAPES(bwd_entry, LAYER || VEC == 1, VEC)
+  return bwd_entry<DT, 16, 8, VEC, LAYER>(D);
+}
+
+template <bool BWD, bool LAYER>
+Shape shape_of(bool bf, bool v8, int D) {
+  if constexpr (BWD) {
+    if (bf) return v8 ? bwd_shape<DT_BF16, 8, LAYER>(D) : bwd_shape<DT_BF16, 1, LAYER>(D);
+    return v8 ? bwd_shape<DT_F16, 8, LAYER>(D) : bwd_shape<DT_F16, 1, LAYER>(D);
+  } else {
+    if (bf) return v8 ? fwd_shape<DT_BF16, 8, LAYER>(D) : fwd_shape<DT_BF16, 1, LAYER>(D);
+    return v8 ? fwd_shape<DT_F16, 8, LAYER>(D) : fwd_shape<DT_F16, 1, LAYER>(D);
+  }
 }
 
 constexpr int kMaxFwd = 16384, kMaxBwd = 8192;
@@ -480,50 +882,45 @@ void fill(NormParams* p, const FoBlockNormDesc* d) {
   p->scale = d->residual_scale, p->eps = d->eps;
 }
 
-// CTAs of one wave a kernel is launched with (the rows are walked with that stride).
-int resident(const Shape& k, int threads, int sms) {
-  int n = k.per_sm->load(std::memory_order_relaxed);
-  if (n == 0) {
-    RelaxedCapture relaxed;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k.kern, threads, 0) != cudaSuccess || n < 1) n = 1;
-    k.per_sm->store(n, std::memory_order_relaxed);
-  }
-  return sms * n;
-}
-
-std::atomic<uint64_t> g_no_opt{0};  // these kernels use no dynamic shared memory
-
-// Work split of the backward kernel: one wave of workers, each walking chunks of rows that
-// share a gate row.  It goes by 148 SMs whatever the device, so that the workspace's size
-// needs no device.
-
-int bwd_warps(int64_t D) {
-  return D <= 512 ? 1 : D <= 1024 ? 2 : D <= 2048 ? 4 : D <= 4096 ? 8 : 16;
-}
-
-struct BwdPlan {
-  int workers, groups, chunks, chunk_rows, ldp;
+// Work split: units of rows inside one gate group, about one a resident CTA (three a SM
+// forward, two backward, where a unit also costs its partial sums), whatever the device, so
+// that the workspace's size needs no device.  16 row-group turns or more a CTA keep its ring
+// and its sums worth while; shorter batches give each row group one row at least.
+struct Plan {
+  int groups, chunks, chunk_rows, units, ldp;
   size_t bytes;
 };
 
-BwdPlan bwd_plan(const FoBlockNormDesc* d) {
-  BwdPlan b{};
-  const int W = bwd_warps(d->D);
-  // 16 warps a SM carry rows at once (one row a CTA of 8 warps: two CTAs)
-  const int cap = 148 * (W >= 16 ? 1 : 16 / W);
+Plan plan(const FoBlockNormDesc* d, int per_sm, int row_groups) {
+  Plan b{};
+  const int cap = 148 * per_sm;
   b.groups = d->gate_rows > 0 ? static_cast<int>(d->gate_rows) : 1;
   const int rpg = static_cast<int>(d->T / b.groups);
   int chunks = b.groups >= cap ? 1 : cap / b.groups;
-  if (chunks > rpg) chunks = rpg;
+  const int turns = (rpg + row_groups - 1) / row_groups;
+  if (chunks > turns) chunks = turns;
   if (chunks < 1) chunks = 1;
   b.chunk_rows = (rpg + chunks - 1) / chunks;
-  b.chunks = b.chunk_rows > 0 ? (rpg + b.chunk_rows - 1) / b.chunk_rows : 1;
-  const long long units = static_cast<long long>(b.groups) * b.chunks;
-  b.workers = static_cast<int>(units < cap ? units : cap);
+  b.chunks = (rpg + b.chunk_rows - 1) / b.chunk_rows;
+  b.units = b.groups * b.chunks;
   b.ldp = (static_cast<int>(d->D) + 3) / 4 * 4;
-  b.bytes = (4 * static_cast<size_t>(b.workers) + (d->gate_rows > 0 ? static_cast<size_t>(units) : 0)) * b.ldp * sizeof(float);
+  b.bytes = 4 * static_cast<size_t>(b.units) * b.ldp * sizeof(float);
   return b;
 }
+
+void set_plan(NormParams* p, const Plan& b) {
+  p->groups = b.groups, p->chunks = b.chunks, p->chunk_rows = b.chunk_rows, p->ldp = b.ldp;
+}
+
+// The backward plan without a device or a dtype: the row groups of the 16-byte layout.
+Plan bwd_plan(const FoBlockNormDesc* d) {
+  const int W = d->D <= 512 ? 1 : d->D <= 1024 ? 2 : d->D <= 2048 ? 4 : 8;
+  return plan(d, d->D > 4096 ? 1 : 2, kCtaWarps / W);
+}
+
+int min_grid(const Plan& b, int most) { return b.units < most ? b.units : most; }
+
+std::atomic<uint64_t> g_no_opt{0};
 
 }  // namespace
 }  // namespace fo
@@ -539,14 +936,13 @@ extern "C" int fo_block_norm(const FoBlockNormDesc* d, void* stream) {
   NormParams p;
   fill(&p, d);
   const bool v8 = vectors(d, false), bf = d->dtype == FO_DT_BF16;
-  const int D = p.D;
-  const Shape s = bf ? (v8 ? fwd_shape<DT_BF16, 8>(D) : fwd_shape<DT_BF16, 1>(D))
-                     : (v8 ? fwd_shape<DT_F16, 8>(D) : fwd_shape<DT_F16, 1>(D));
-  const int R = rows_per_cta(s.warps);
-  const long long want = (d->T + R - 1) / R;
-  const int most = resident(s, 32 * s.warps * R, hd.sms);
-  const cudaError_t e = launch_pdl(s.kern, g_no_opt, dim3(static_cast<unsigned>(want < most ? want : most)),
-                                   dim3(32 * s.warps, R), 0, 1, static_cast<cudaStream_t>(stream), p);
+  const Shape s = p.layer ? shape_of<false, true>(bf, v8, p.D) : shape_of<false, false>(bf, v8, p.D);
+  const int per_sm = s.warps == 16 ? 1 : 3;
+  const Plan b = plan(d, per_sm, row_groups(s.warps));
+  set_plan(&p, b);
+  p.status = hd.status, p.timeout_ns = hd.timeout_ns;
+  const cudaError_t e = launch_pdl(s.kern, *s.opted, dim3(min_grid(b, hd.sms * per_sm)), dim3(32 * s.warps, row_groups(s.warps)), s.smem, 1,
+                                   static_cast<cudaStream_t>(stream), p);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   host_count_launches(1);
   return host_ok();
@@ -576,30 +972,27 @@ extern "C" int fo_block_norm_backward(const FoBlockNormDesc* d, void* stream) {
     return host_fail(FO_EINVAL, "y, r, dz, w_pre, dy, dx and dw_pre must be device pointers");
   if ((d->w_post != nullptr && d->dw_post == nullptr) || (d->gate != nullptr && d->dgate == nullptr))
     return host_fail(FO_EINVAL, "w_post needs dw_post, a gate needs dgate");
-  const BwdPlan b = bwd_plan(d);
+  const Plan b = bwd_plan(d);
   if (d->workspace == nullptr || d->workspace_bytes < b.bytes || !host_aligned16(d->workspace))
     return host_fail(FO_EINVAL, "the backward pass needs a 16-byte aligned workspace of %zu bytes", b.bytes);
   HostDevice hd;
   if (int rc = host_device(&hd)) return rc;
   NormParams p;
   fill(&p, d);
-  p.groups = b.groups, p.chunks = b.chunks, p.chunk_rows = b.chunk_rows, p.workers = b.workers, p.ldp = b.ldp;
-  p.part_w = static_cast<float*>(d->workspace);
-  p.part_g = p.part_w + 4 * static_cast<size_t>(b.workers) * b.ldp;
-  const bool v8 = vectors(d, true), bf = d->dtype == FO_DT_BF16, bias = d->db_post != nullptr || d->db_pre != nullptr;
+  set_plan(&p, b);
+  p.part = static_cast<float*>(d->workspace);
+  p.status = hd.status, p.timeout_ns = hd.timeout_ns;
+  const bool v8 = vectors(d, true), bf = d->dtype == FO_DT_BF16;
   const int D = p.D;
-  const Shape s = bf ? (v8 ? (bias ? bwd_shape<DT_BF16, 8, true>(D) : bwd_shape<DT_BF16, 8, false>(D))
-                           : (bias ? bwd_shape<DT_BF16, 1, true>(D) : bwd_shape<DT_BF16, 1, false>(D)))
-                     : (v8 ? (bias ? bwd_shape<DT_F16, 8, true>(D) : bwd_shape<DT_F16, 8, false>(D))
-                           : (bias ? bwd_shape<DT_F16, 1, true>(D) : bwd_shape<DT_F16, 1, false>(D)));
-  const int R = rows_per_cta(s.warps);
-  cudaError_t e = launch_pdl(s.kern, g_no_opt, dim3((b.workers + R - 1) / R), dim3(32 * s.warps, R), 0, 1, st, p);
+  const Shape s = p.layer ? shape_of<true, true>(bf, v8, D) : shape_of<true, false>(bf, v8, D);
+  cudaError_t e = launch_pdl(s.kern, *s.opted, dim3(min_grid(b, hd.sms * 2)), dim3(32 * s.warps, row_groups(s.warps)), s.smem, 1, st, p);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   JoinParams j{};
-  j.part_w = p.part_w, j.part_g = p.part_g;
+  j.part = p.part;
   j.out[0] = d->dw_pre, j.out[1] = d->w_post != nullptr ? d->dw_post : nullptr, j.out[2] = d->db_pre, j.out[3] = d->db_post;
   j.out[4] = d->gate != nullptr ? d->dgate : nullptr;
-  j.workers = b.workers, j.chunks = b.chunks, j.ldp = b.ldp, j.D = D, j.vec_dtype = d->vec_dtype;
+  j.w_post = d->w_post, j.b_post = d->b_post, j.gate = d->gate, j.ldgate = d->ldgate;
+  j.units = b.units, j.chunks = b.chunks, j.ldp = b.ldp, j.D = D, j.vec_dtype = d->vec_dtype;
   const unsigned outs = 4u + (d->gate != nullptr ? static_cast<unsigned>(b.groups) : 0u);
   e = launch_pdl(fo_norm_join_kernel, g_no_opt, dim3(outs, (D + 63) / 64), dim3(16 * kJoinSplit), 0, 1, st, j);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));

@@ -121,6 +121,11 @@ extern "C" int fo_matvec_w4(const FoMatvecW4Desc* d, void* stream) {
   set_weight(&p, 0, &d->w);
   if (gated) set_weight(&p, 1, &d->w_up);
   p.group = d->w.group, p.groups = static_cast<int>((d->K + d->w.group - 1) / d->w.group);
+  p.scale_vec = p.groups % 8 == 0, p.zero_vec = p.groups % 16 == 0;
+  for (int m = 0; m < (gated ? 2 : 1); ++m) {
+    p.scale_vec = p.scale_vec && host_aligned16(p.scale[m]) && p.lds[m] % 8 == 0;
+    p.zero_vec = p.zero_vec && host_aligned16(p.zero[m]) && p.ldz[m] % 16 == 0;
+  }
   p.bias = d->bias, p.out = d->out, p.ldo = d->ldo;
   p.act = gate_act_of(d->act);
   const cudaError_t e = launch_skinny(W_Q4, gated, d->dtype == FO_DT_BF16 ? DT_BF16 : DT_F16, p, hd.sms, static_cast<cudaStream_t>(stream));

@@ -34,6 +34,7 @@ struct SkinnyParams {
   const unsigned char* zero[2];  // null: 8
   long long lds[2], ldz[2];
   int group, groups;
+  int scale_vec, zero_vec;  // their rows are read by 16 bytes
   const void* bias;
   int act;
   void *out, *g, *u;  // g, u: the products before the activation (or null)
@@ -188,22 +189,36 @@ __global__ void __launch_bounds__(256) fo_skinny_kernel(const SkinnyParams p) {
   griddep_wait();
   griddep_launch_dependents();
   if constexpr (FMT == W_Q4) {
-    for (int i = threadIdx.x; i < S::kRows * p.groups; i += 256) {
-      const int row = i / p.groups, gi = i - row * p.groups;
+    // The rows' scales and zeros, whole: a warp takes rows warp, warp + 8, .. by 16-byte
+    // copies where the rows allow them (they land with the ring's first steps), else by
+    // single loads.
+    for (int row = warp; row < S::kRows; row += S::kWarps) {
       const int m = row / S::kFeatures, n = n0 + row % S::kFeatures;
-      unsigned short sc = 0;
-      unsigned char z = 0;
-      if (n < p.N) {
-        sc = __ldg(static_cast<const unsigned short*>(p.scale[m]) + n * p.lds[m] + gi);
-        if (p.zero[0] != nullptr) z = __ldg(p.zero[m] + n * p.ldz[m] + gi);
+      const bool in = n < p.N;
+      const unsigned short* sc = static_cast<const unsigned short*>(p.scale[m]) + (in ? n : 0) * p.lds[m];
+      unsigned short* sd = reinterpret_cast<unsigned short*>(scales + row * sstride);
+      if (p.scale_vec) {
+        for (int i = lane * 8; i < p.groups; i += 256) cp_async_16(smem_u32(sd + i), sc + i, in ? 16u : 0u);
+      } else {
+        for (int i = lane; i < p.groups; i += 32) sd[i] = in ? __ldg(sc + i) : 0;
       }
-      *reinterpret_cast<unsigned short*>(scales + row * sstride + gi * 2) = sc;
-      if (p.zero[0] != nullptr) zeros[row * zstride + gi] = z;
+      if (p.zero[0] != nullptr) {
+        const unsigned char* zc = p.zero[m] + (in ? n : 0) * p.ldz[m];
+        unsigned char* zd = zeros + row * zstride;
+        if (p.zero_vec) {
+          for (int i = lane * 16; i < p.groups; i += 512) cp_async_16(smem_u32(zd + i), zc + i, in ? 16u : 0u);
+        } else {
+          for (int i = lane; i < p.groups; i += 32) zd[i] = in ? __ldg(zc + i) : 0;
+        }
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) issue(i);
-  if constexpr (FMT == W_Q4) __syncthreads();
+  if constexpr (FMT == W_Q4) {
+    cp_async_wait<S::kStages - 2>();  // the scales are older than every step but the first, and land with it
+    __syncthreads();
+  }
 
   float acc[S::kTiles][NT][4] = {};
   for (int i = 0; i < mine; ++i) {
