@@ -243,11 +243,18 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: torch.Tensor, y: torch.T
     d.r, d.ldr = r.data_ptr(), _ld(r, T, D, "r")
     out = {"dy": y.new_empty((T, D)), "dx": y.new_empty((T, D))}
     d.lddy = d.lddx = D
-    for p, name in ((w_pre, "dw_pre"), (w_post, "dw_post"), (b_pre, "db_pre"), (b_post, "db_post"), (gate, "dgate")):
-        if p is not None:
-            out[name] = p.new_empty(p.shape)
-    for name, t in out.items():
-        setattr(d, name, t.data_ptr())
+    # the parameters' gradients share one allocation, gate rows last
+    names = [n for n, p in (("dw_pre", w_pre), ("dw_post", w_post), ("db_pre", b_pre), ("db_post", b_post)) if p is not None]
+    rows = len(names)
+    flat = w_pre.new_empty((rows + d.gate_rows, D))
+    at, step = flat.data_ptr(), D * flat.element_size()
+    out.update(zip(names, flat.unbind(0)))
+    for i, name in enumerate(names):
+        setattr(d, name, at + i * step)
+    if gate is not None:
+        out["dgate"] = out_gate = flat[rows] if gate.dim() == 1 else flat[rows:]
+        d.dgate = out_gate.data_ptr()
+    d.dy, d.dx = out["dy"].data_ptr(), out["dx"].data_ptr()
     lib = N.lib()
     ref = ctypes.byref(d)
     need = lib.fo_block_norm_backward_workspace_size(ref)

@@ -30,6 +30,7 @@ SOURCES = [
     ("fo_family_direct.cu", "fo_family_direct", []),
     ("fo_noalloc.cu", "fo_noalloc", []),
     ("fo_ffn.cu", "fo_ffn", []),
+    ("fo_few.cu", "fo_few", []),
     ("fo_norm.cu", "fo_norm", []),
     ("fo_skinny.cu", "fo_skinny", []),
 ]

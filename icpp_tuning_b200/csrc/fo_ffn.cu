@@ -1,7 +1,8 @@
 // fo_ffn.cu -- launches and C entries of the gated feed-forward block.
+#include <cstdlib>
 #include <cstring>
 
-#include "fo_ffn.cuh"
+#include "fo_few.cuh"
 #include "fo_host.cuh"
 #include "../../include/b200fo.h"
 
@@ -144,6 +145,62 @@ int fail_launch(cudaError_t e) { return host_fail(FO_ECUDA, "kernel launch faile
 }  // namespace
 }  // namespace fo
 
+namespace fo {
+namespace {
+
+
+int few_most() {
+  static const int v = getenv("FO_FEW") ? atoi(getenv("FO_FEW")) : 256;
+  return v;
+}
+
+constexpr int kSms = 148;
+
+int64_t kblocks(int64_t k) { return (k + kBK - 1) / kBK; }
+
+// The short-token products of a call.
+struct Few {
+  bool on;
+  FewPlan first, second;  // forward: gated, down; backward: dgate, dx
+};
+
+Few few_of(const FoGatedFfnDesc* d, bool backward) {
+  Few f{};
+  f.on = d->T <= few_most();
+  if (f.on) {
+    f.first = backward ? few_plan(FEW_DGATE, d->F, d->T, static_cast<int>(kblocks(d->N)), kSms)
+                       : few_plan(FEW_GATED, d->F, d->T, static_cast<int>(kblocks(d->D)), kSms);
+    f.second = backward ? few_plan(FEW_PLAIN, d->D, d->T, static_cast<int>(2 * kblocks(d->F)), kSms)
+                        : few_plan(FEW_PLAIN, d->N, d->T, static_cast<int>(kblocks(d->F)), kSms);
+  }
+  return f;
+}
+
+struct FewBuild {
+  FewMaps m;
+  FewParams p;
+  int dt, rc = FO_OK;
+
+  FewBuild(const FoGatedFfnDesc* d, const HostDevice& hd, int64_t features, int64_t k, int segments) : dt(d->dtype) {
+    memset(&m, 0, sizeof(m));
+    memset(&p, 0, sizeof(p));
+    p.F = static_cast<int>(features), p.T = static_cast<int>(d->T);
+    p.kb0 = static_cast<int>(kblocks(k)), p.kb = segments * p.kb0;
+    p.bf16 = d->dtype == FO_DT_BF16;
+    p.status = hd.status, p.timeout_ns = hd.timeout_ns;
+  }
+  void weight(int i, const Mat& w, bool transposed, const char* what) {
+    p.a_mn = transposed;
+    if (rc == FO_OK) rc = host_tmap(&m.a[i], dt, w.p, w.cols, w.rows, static_cast<uint64_t>(w.ld) * 2, 64, transposed ? 64 : 128, what);
+  }
+  void token(int i, const Mat& t, int nt, const char* what) {
+    if (rc == FO_OK) rc = host_tmap(&m.b[i], dt, t.p, t.cols, t.rows, static_cast<uint64_t>(t.ld) * 2, 64, nt, what);
+  }
+};
+
+}  // namespace
+}  // namespace fo
+
 extern "C" size_t fo_gated_ffn_workspace_size(const FoGatedFfnDesc* d, int32_t backward) {
   if (d == nullptr || d->T <= 0 || d->F <= 0) return 0;
   return static_cast<size_t>(d->T) * fo::pad8(d->F) * 2 * (backward ? 3 : 1);
@@ -163,6 +220,7 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
     if (int rc = check_mat(d->g, d->ldg, d->F, "g")) return rc;
     if (int rc = check_mat(d->u, d->ldu, d->F, "u")) return rc;
   }
+  const Few few = few_of(d, false);
   const size_t need = fo_gated_ffn_workspace_size(d, 0);
   if (d->workspace == nullptr || d->workspace_bytes < need || !host_aligned16(d->workspace))
     return host_fail(FO_EINVAL, "the block needs a 16-byte aligned workspace of %zu bytes", need);
@@ -171,23 +229,22 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Mat h{d->workspace, d->T, d->F, pad8(d->F)};
 
-  if (d->T <= 16 && d->D % 8 == 0 && d->F % 8 == 0 && d->N % 8 == 0) {
-    const int fmt = kn ? W_KN : W_NK, dt = d->dtype == FO_DT_BF16 ? DT_BF16 : DT_F16;
-    SkinnyParams s = {};
-    s.x = d->x, s.ldx = d->ldx;
-    s.T = static_cast<int>(d->T), s.N = static_cast<int>(d->F), s.K = static_cast<int>(d->D);
-    s.w[0] = d->w_gate, s.w[1] = d->w_up, s.ldw[0] = d->ldwg, s.ldw[1] = d->ldwu;
-    s.act = gate_act_of(d->act);
-    s.out = d->workspace, s.ldo = h.ld;
-    s.g = d->g, s.u = d->u, s.ldg = d->ldg, s.ldu = d->ldu;
-    cudaError_t e = launch_skinny(fmt, true, dt, s, hd.sms, st);
-    if (e != cudaSuccess) return fail_launch(e);
-    SkinnyParams o = {};
-    o.x = d->workspace, o.ldx = h.ld;
-    o.T = s.T, o.N = static_cast<int>(d->N), o.K = static_cast<int>(d->F);
-    o.w[0] = d->w_down, o.ldw[0] = d->ldwd;
-    o.out = d->y, o.ldo = d->ldy;
-    e = launch_skinny(fmt, false, dt, o, hd.sms, st);
+  const Mat x{d->x, d->T, d->D, d->ldx};
+  const Mat wg{d->w_gate, kn ? d->D : d->F, kn ? d->F : d->D, d->ldwg}, wu{d->w_up, wg.rows, wg.cols, d->ldwu};
+  const Mat wd{d->w_down, kn ? d->F : d->N, kn ? d->N : d->F, d->ldwd};
+  if (few.on) {
+    FewBuild a(d, hd, d->F, d->D, 1), o(d, hd, d->N, d->F, 1);
+    a.weight(0, wg, kn, "w_gate"), a.weight(1, wu, kn, "w_up");
+    a.token(0, x, few.first.nt, "x");
+    a.p.out = d->workspace, a.p.ldo = h.ld;
+    a.p.g = d->g, a.p.u = d->u, a.p.ldg = d->ldg, a.p.ldu = d->ldu;
+    o.weight(0, wd, kn, "w_down");
+    o.token(0, h, few.second.nt, "h");
+    o.p.out = d->y, o.p.ldo = d->ldy;
+    o.p.early = 1;
+    if (a.rc || o.rc) return a.rc ? a.rc : o.rc;
+    cudaError_t e = launch_few(FEW_GATED, d->act, a.m, a.p, few.first, st);
+    if (e == cudaSuccess) e = launch_few(FEW_PLAIN, 0, o.m, o.p, few.second, st);
     if (e != cudaSuccess) return fail_launch(e);
     host_count_launches(2);
     return host_ok();
@@ -196,8 +253,6 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
   Build b(d->dtype, hd);
   FfnProblem& q = b.add(d->T, d->F, d->D, kFfnTile / 2, 1);
   q.b_mn = kn;
-  const Mat x{d->x, d->T, d->D, d->ldx};
-  const Mat wg{d->w_gate, kn ? d->D : d->F, kn ? d->F : d->D, d->ldwg}, wu{d->w_up, wg.rows, wg.cols, d->ldwu};
   b.operand(&b.maps.a[0][0], x, false, "x");
   b.operand(&b.maps.b[0][0], wg, kn, "w_gate");
   b.operand(&b.maps.b[0][1], wu, kn, "w_up");
@@ -212,7 +267,7 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
   if (e != cudaSuccess) return fail_launch(e);
 
   Build y(d->dtype, hd);
-  y.product(d->T, d->N, d->F, h, false, {d->w_down, kn ? d->F : d->N, kn ? d->N : d->F, d->ldwd}, kn, {d->y, d->T, d->N, d->ldy});
+  y.product(d->T, d->N, d->F, h, false, wd, kn, {d->y, d->T, d->N, d->ldy});
   if (y.rc) return y.rc;
   e = launch(FFN_GRADS, 0, y.maps, y.p, hd.sms / 2, st);
   if (e != cudaSuccess) return fail_launch(e);
@@ -245,6 +300,7 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   if (int rc = check_mat(d->g, d->ldg, d->F, "g")) return rc;
   if (int rc = check_mat(d->u, d->ldu, d->F, "u")) return rc;
   if (int rc = check_mat(d->dx, d->lddx, d->D, "dx")) return rc;
+  const Few few = few_of(d, true);
   const size_t need = fo_gated_ffn_workspace_size(d, 1);
   if (d->workspace == nullptr || d->workspace_bytes < need || !host_aligned16(d->workspace))
     return host_fail(FO_EINVAL, "the backward pass needs a 16-byte aligned workspace of %zu bytes", need);
@@ -256,18 +312,36 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   const Mat wg{d->w_gate, up_rows, up_cols, d->ldwg}, wu{d->w_up, up_rows, up_cols, d->ldwu};
   const Mat wd{d->w_down, down_rows, down_cols, d->ldwd};
 
-  Build b(d->dtype, hd);
-  FfnProblem& q = b.add(d->T, d->F, d->N, kFfnTile, 1);
-  q.b_mn = !kn;
-  b.operand(&b.maps.a[0][0], dy, false, "dy");
-  b.operand(&b.maps.b[0][0], wd, !kn, "w_down");
-  b.map(&b.maps.c[0], dg, 32, "dg");
-  b.map(&b.maps.c[1], du, 32, "du");
-  b.map(&b.maps.c[2], h, 32, "h");
-  b.p.g = d->g, b.p.u = d->u, b.p.ldg = d->ldg, b.p.ldu = d->ldu;
-  if (b.rc) return b.rc;
-  cudaError_t e = launch(FFN_DGATE, d->act, b.maps, b.p, hd.sms / 2, st);
-  if (e != cudaSuccess) return fail_launch(e);
+  cudaError_t e;
+  if (few.on) {
+    FewBuild a(d, hd, d->F, d->N, 1), o(d, hd, d->D, d->F, 2);
+    a.weight(0, wd, !kn, "w_down");
+    a.token(0, dy, few.first.nt, "dy");
+    a.p.out = const_cast<void*>(dg.p), a.p.g = const_cast<void*>(du.p), a.p.u = const_cast<void*>(h.p);
+    a.p.ldo = a.p.ldg = a.p.ldu = ldf;
+    a.p.sg = d->g, a.p.su = d->u, a.p.ldsg = d->ldg, a.p.ldsu = d->ldu;
+    o.weight(0, wg, !kn, "w_gate"), o.weight(1, wu, !kn, "w_up");
+    o.token(0, dg, few.second.nt, "dg"), o.token(1, du, few.second.nt, "du");
+    o.p.out = d->dx, o.p.ldo = d->lddx;
+    o.p.early = 1;
+    if (a.rc || o.rc) return a.rc ? a.rc : o.rc;
+    e = launch_few(FEW_DGATE, d->act, a.m, a.p, few.first, st);
+    if (e == cudaSuccess) e = launch_few(FEW_PLAIN, 0, o.m, o.p, few.second, st);
+    if (e != cudaSuccess) return fail_launch(e);
+  } else {
+    Build b(d->dtype, hd);
+    FfnProblem& q = b.add(d->T, d->F, d->N, kFfnTile, 1);
+    q.b_mn = !kn;
+    b.operand(&b.maps.a[0][0], dy, false, "dy");
+    b.operand(&b.maps.b[0][0], wd, !kn, "w_down");
+    b.map(&b.maps.c[0], dg, 32, "dg");
+    b.map(&b.maps.c[1], du, 32, "du");
+    b.map(&b.maps.c[2], h, 32, "h");
+    b.p.g = d->g, b.p.u = d->u, b.p.ldg = d->ldg, b.p.ldu = d->ldu;
+    if (b.rc) return b.rc;
+    e = launch(FFN_DGATE, d->act, b.maps, b.p, hd.sms / 2, st);
+    if (e != cudaSuccess) return fail_launch(e);
+  }
 
   Build w(d->dtype, hd);
   auto add_dx = [&] { w.product(d->T, d->D, d->F, dg, false, wg, !kn, {d->dx, d->T, d->D, d->lddx}, &du, &wu); };
@@ -284,7 +358,9 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
       w.product(d->N, d->F, d->T, dy, true, h, true, owd);
     }
   };
-  if (2 * d->F >= d->T) {  // longest tiles first
+  if (few.on) {
+    add_weights();
+  } else if (2 * d->F >= d->T) {  // longest tiles first
     add_dx();
     add_weights();
   } else {
@@ -295,6 +371,6 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   w.schedule(hd.sms / 2);
   e = launch(FFN_GRADS, 0, w.maps, w.p, hd.sms / 2, st);
   if (e != cudaSuccess) return fail_launch(e);
-  host_count_launches(2);
+  host_count_launches(few.on ? 3 : 2);
   return host_ok();
 }

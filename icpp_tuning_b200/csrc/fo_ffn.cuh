@@ -148,6 +148,11 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
     tmem_alloc_pair(smem_u32(tmem_slot), 512);
     tmem_relinquish_pair();
   }
+  if (threadIdx.x == 64) {
+    tma_prefetch_desc(&maps.a[0][0]);
+    tma_prefetch_desc(&maps.b[0][0]);
+    tma_prefetch_desc(&maps.c[0]);
+  }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -168,33 +173,45 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
         const FfnProblem& q = p.prob[un.pr];
         const int arow = un.tm * kFfnTile + static_cast<int>(rank) * 128;
         const int bcol = EPI == FFN_GATED ? un.tn * 128 : un.tn * kFfnTile + static_cast<int>(rank) * 128;
-        for (int k0 = 0; k0 < q.kb; k0 += kFfnKps) {
-          const int nk = min(kFfnKps, q.kb - k0);
+        // everything of the problem in registers: a constant read costs this one thread as
+        // much as issuing a copy
+        const int kb = q.kb, a_mn = q.a_mn, b_mn = q.b_mn;
+        int left = q.kb0, k = 0;  // K blocks left in the segment, the next one's first column
+        const CUtensorMap* ma = &maps.a[un.pr][0];
+        const CUtensorMap* mB = EPI == FFN_GATED ? &maps.b[0][rank] : &maps.b[un.pr][0];
+        for (int k0 = 0; k0 < kb; k0 += kFfnKps) {
           if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, tmo, abort_flag)) {
             ok = false;
             break;
           }
+          const int nk = min(kFfnKps, kb - k0);
           const uint32_t fb = bar_full + 8 * s;
           const uint32_t fbl = mapa_shared(fb, 0);  // both CTAs' bytes complete on the leader's barrier
           if (rank == 0) mbar_arrive_expect_tx(fb, 2 * nk * (kFfnStageA + kFfnStageB) / kFfnKps);
-          for (int i = 0; i < nk; ++i) {
-            const int seg = k0 + i >= q.kb0;
-            const int k = (k0 + i - (seg ? q.kb0 : 0)) * kBK;
-            const CUtensorMap* ma = &maps.a[un.pr][seg];
-            const CUtensorMap* mB = EPI == FFN_GATED ? &maps.b[0][rank] : &maps.b[un.pr][seg];
-            const uint32_t sa = sA + (s * kFfnKps + i) * kAStageBytes, sb = sB + (s * kFfnKps + i) * kAStageBytes;
-            if (q.a_mn) {
+          uint32_t sa = sA + s * kFfnStageA, sb = sB + s * kFfnStageB;
+#pragma unroll
+          for (int i = 0; i < kFfnKps; ++i) {
+            if (i >= nk) break;
+            if (EPI == FFN_GRADS && left == 0) {  // the second segment
+              ++ma, ++mB;
+              k = 0;
+              left = kb;
+            }
+            if (a_mn) {
               tma_load_2d_pair(sa, ma, fbl, arow, k);
               tma_load_2d_pair(sa + 64 * 128, ma, fbl, arow + 64, k);
             } else {
               tma_load_2d_pair(sa, ma, fbl, k, arow);
             }
-            if (q.b_mn) {
+            if (b_mn) {
               tma_load_2d_pair(sb, mB, fbl, bcol, k);
               tma_load_2d_pair(sb + 64 * 128, mB, fbl, bcol + 64, k);
             } else {
               tma_load_2d_pair(sb, mB, fbl, k, bcol);
             }
+            sa += kAStageBytes, sb += kAStageBytes;
+            k += kBK;
+            --left;
           }
           ++issued;
           if (++s == kFfnStages) {
@@ -212,15 +229,20 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
+      // One thread issues every MMA and commit: the descriptors are stepped per stage, and
+      // nothing of a problem is read again inside its K loop.
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
+      uint64_t off = 0;  // of stage s, in descriptor units (A and B stages are alike)
       bool ok = true;
       for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
-        const FfnProblem& q = p.prob[ffn_unit(p, u).pr];
-        const uint32_t idesc = idesc_f16(p.bf16, q.b_mn, 256, 256) | (static_cast<uint32_t>(q.a_mn) << 15);
-        const uint64_t a0 = q.a_mn ? sdesc_sw128(sA, 64 * 128, 1024) : sdesc_sw128(sA, 16, 1024);
-        const uint64_t b0 = q.b_mn ? sdesc_sw128(sB, 64 * 128, 1024) : sdesc_sw128(sB, 16, 1024);
-        const uint32_t as = q.a_mn ? (2048 >> 4) : (32 >> 4), bs = q.b_mn ? (2048 >> 4) : (32 >> 4);
+        const FfnProblem& q = p.prob[EPI == FFN_GRADS ? ffn_unit(p, u).pr : 0];
+        const int kb = q.kb, a_mn = q.a_mn, b_mn = q.b_mn;
+        const uint32_t idesc = idesc_f16(p.bf16, b_mn, 256, 256) | (static_cast<uint32_t>(a_mn) << 15);
+        const uint64_t a0 = a_mn ? sdesc_sw128(sA, 64 * 128, 1024) : sdesc_sw128(sA, 16, 1024);
+        const uint64_t b0 = b_mn ? sdesc_sw128(sB, 64 * 128, 1024) : sdesc_sw128(sB, 16, 1024);
+        const uint32_t as = a_mn ? (2048 >> 4) : (32 >> 4), bs = b_mn ? (2048 >> 4) : (32 >> 4);
+        uint64_t ad = a0 + off, bd = b0 + off;
         if (!mbar_wait_cluster(bar_tempty + 8 * acc, acc_ph ^ 1, tmo, abort_flag)) {
           ok = false;
           break;
@@ -228,18 +250,17 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
         tc_fence_after();
         const uint32_t d = tmem_base + acc * 256;
         uint32_t accum = 0;
-        const int kb = q.kb;
         for (int k0 = 0; k0 < kb; k0 += kFfnKps) {
+          const int nk = min(kFfnKps, kb - k0);
           if (!mbar_wait(bar_full + 8 * s, ph, tmo, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int nk = min(kFfnKps, kb - k0);
 #pragma unroll 2
           for (int i = 0; i < nk; ++i) {
-            const uint64_t a = a0 + static_cast<uint64_t>((s * kFfnKps + i) * (kAStageBytes >> 4));
-            const uint64_t b = b0 + static_cast<uint64_t>((s * kFfnKps + i) * (kAStageBytes >> 4));
+            const uint64_t a = ad + static_cast<uint64_t>(i * (kAStageBytes >> 4));
+            const uint64_t b = bd + static_cast<uint64_t>(i * (kAStageBytes >> 4));
             tc_mma_f16_pair(d, a, b, idesc, accum);
             tc_mma_f16_pair(d, a + as, b + bs, idesc, 1u);
             tc_mma_f16_pair(d, a + 2 * as, b + 2 * bs, idesc, 1u);
@@ -250,6 +271,13 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
           if (++s == kFfnStages) {
             s = 0;
             ph ^= 1;
+            off = 0;
+            ad = a0;
+            bd = b0;
+          } else {
+            off += kFfnStageA >> 4;
+            ad += kFfnStageA >> 4;
+            bd += kFfnStageB >> 4;
           }
         }
         if (!ok) break;

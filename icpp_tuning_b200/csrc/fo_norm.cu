@@ -155,15 +155,16 @@ __device__ __forceinline__ const void* vec_at(const void* ptr, int dt, long long
   return ptr == nullptr ? nullptr : static_cast<const char*>(ptr) + i * (dt == DT_F32 ? 4 : 2);
 }
 
-// Sums of N <= 8 values over a warp: each butterfly step halves the values a lane carries
+// Sums of N <= 16 values over a warp: each butterfly step halves the values a lane carries
 // (value i ends in the lanes with those bits), so 8 values take 9 shuffles instead of 40.
 template <int N>
 __device__ __forceinline__ float warp_sums(const float (&v)[N], int lane) {
-  float a[8];
+  constexpr int M = N <= 8 ? 8 : 16;
+  float a[M];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = i < N ? v[i] : 0.f;
+  for (int i = 0; i < M; ++i) a[i] = i < N ? v[i] : 0.f;
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
+  for (int o = M / 2; o > 0; o >>= 1) {
     const bool up = (lane & o) != 0;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
@@ -172,9 +173,9 @@ __device__ __forceinline__ float warp_sums(const float (&v)[N], int lane) {
       a[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
     }
   }
-  a[0] += __shfl_xor_sync(0xffffffffu, a[0], 8);
-  a[0] += __shfl_xor_sync(0xffffffffu, a[0], 16);
-  return a[0];  // lane l: the warp's sum of value l & 7
+#pragma unroll
+  for (int o = M; o < 32; o <<= 1) a[0] += __shfl_xor_sync(0xffffffffu, a[0], o);
+  return a[0];  // lane l: the warp's sum of value l & (M - 1)
 }
 
 // Sums over the W warps of a row.  Rounds alternate between two halves of the scratch: a
@@ -182,7 +183,7 @@ __device__ __forceinline__ float warp_sums(const float (&v)[N], int lane) {
 // k + 1 lies between), so one barrier a round is enough.
 template <int W>
 struct RowSum {
-  float* red;  // [2][W][8] of this row group
+  float* red;  // [2][W][16] of this row group
   int round, bar;
   template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N]) {
@@ -191,7 +192,7 @@ struct RowSum {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
       if constexpr (W > 1) {
-        float* s = red + round * 8 * W;
+        float* s = red + round * 16 * W;
         if (lane == 0) s[threadIdx.x >> 5] = v[0];
         named_bar_sync(bar, 32 * W);
         v[0] = s[lane & (W - 1)];
@@ -201,17 +202,18 @@ struct RowSum {
       }
       return;
     }
-    float mine = warp_sums(v, lane);  // lane l: value l & 7
+    constexpr int M = N <= 8 ? 8 : 16, kPer = 32 / M;  // warps whose sums the lanes read at once
+    float mine = warp_sums(v, lane);                   // lane l: value l & (M - 1)
     if constexpr (W > 1) {
-      float* s = red + round * 8 * W;
-      if (lane < 8) s[(threadIdx.x >> 5) * 8 + lane] = mine;
+      float* s = red + round * 16 * W;
+      if (lane < M) s[(threadIdx.x >> 5) * M + lane] = mine;
       named_bar_sync(bar, 32 * W);
       mine = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; w += 4)
-        if (W >= 4 || (lane >> 3) < W) mine += s[w * 8 + lane];  // warps w .. w + 3: eight lanes each
-      mine += __shfl_xor_sync(0xffffffffu, mine, 8);
-      mine += __shfl_xor_sync(0xffffffffu, mine, 16);
+      for (int w = 0; w < W; w += kPer)
+        if (W >= kPer || lane / M < W) mine += s[w * M + lane];
+#pragma unroll
+      for (int o = M; o < 32; o <<= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
       round ^= 1;
     }
 #pragma unroll
@@ -508,11 +510,11 @@ template <int DT, int W, int NP, int VEC, bool LAYER, int S>
 __global__ void __launch_bounds__(32 * W * row_groups(W)) fo_norm_fwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int RG = row_groups(W);
   extern __shared__ __align__(128) uint8_t smem_norm[];
-  __shared__ float red[RG * 2 * 8 * W];
+  __shared__ float red[RG * 2 * 16 * W];
   __shared__ __align__(8) uint64_t bars[RG * S];
   Rows<DT, 2, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
   in.init(smem_norm + threadIdx.y * S * 2 * in.kRow, bars + threadIdx.y * S);
-  FwdRow<DT, W, NP, VEC, LAYER, S> f{p, in, {red + threadIdx.y * 2 * 8 * W, 0, 1 + static_cast<int>(threadIdx.y)}, {}, {}, {}, {}};
+  FwdRow<DT, W, NP, VEC, LAYER, S> f{p, in, {red + threadIdx.y * 2 * 16 * W, 0, 1 + static_cast<int>(threadIdx.y)}, {}, {}, {}, {}};
   griddep_wait();
   griddep_launch_dependents();
   walk<W, S>(p, in, f);
@@ -608,20 +610,17 @@ struct BwdRow {
           }
         }
       }
-      float q[6];
+      float q[LAYER ? 9 : 6];
 #pragma unroll
       for (int i = 0; i < 6; ++i) q[i] = sum(t[i]);
+      if constexpr (LAYER) q[6] = sum(l[0]), q[7] = sum(l[1]), q[8] = sum(l[2]);
       sums(q);
       ask();
       kr = rsqrtf(fmaf(q[0], inv, p.eps)), ky = post ? rsqrtf(fmaf(q[1], inv, p.eps)) : 1.f;
       m = q[2] * inv * kr;  // mean(c rhat)
-      // mean(e yhat) of e = A t, t = dr + kr c - kr kr m r
+      // mean(e yhat) and mean(e) of e = A t, t = dr + kr c - kr kr m r
       me = post ? ky * inv * fmaf(kr, fmaf(-kr * m, q[5], q[4]), q[3]) : 0.f;
-      if constexpr (LAYER) {
-        float s[3] = {sum(l[0]), sum(l[1]), sum(l[2])};
-        sums(s);
-        me0 = post ? inv * fmaf(kr, fmaf(-kr * m, s[2], s[1]), s[0]) : 0.f;
-      }
+      if constexpr (LAYER) me0 = post ? inv * fmaf(kr, fmaf(-kr * m, q[8], q[7]), q[6]) : 0.f;
     }
     const Two kr2 = two(kr), ky2 = two(ky), nm = two(-m), nme = two(-me), sc = two(p.scale);
     const Two nme0 = two(-me0);
@@ -679,19 +678,19 @@ template <int DT, int W, int NP, int VEC, bool LAYER>
 __global__ void __launch_bounds__(32 * W * row_groups(W), W == 16 ? 1 : 2) fo_norm_bwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int RG = row_groups(W), S = kBwdStages;
   extern __shared__ __align__(128) uint8_t smem_norm[];
-  __shared__ float red[RG * 2 * 8 * W];
+  __shared__ float red[RG * 2 * 16 * W];
   __shared__ __align__(8) uint64_t bars[RG * S];
   Rows<DT, 4, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
   in.init(smem_norm + threadIdx.y * S * 4 * in.kRow, bars + threadIdx.y * S);
   float* joint = reinterpret_cast<float*>(smem_norm + RG * S * 4 * in.kRow);
-  BwdRow<DT, W, NP, VEC, LAYER> f{p, in, {red + threadIdx.y * 2 * 8 * W, 0, 1 + static_cast<int>(threadIdx.y)}, joint, {}, {}, {}};
+  BwdRow<DT, W, NP, VEC, LAYER> f{p, in, {red + threadIdx.y * 2 * 16 * W, 0, 1 + static_cast<int>(threadIdx.y)}, joint, {}, {}, {}};
   griddep_wait();
   griddep_launch_dependents();
   walk<W, S>(p, in, f);
 }
 
 // Joins the units' sums in a fixed order and forms the parameter gradients: block (output
-// row, 64 columns).  Output rows 0..3 are dw_pre, dw_post, db_pre, db_post (all units), 4 + g
+// row, 32 columns).  Output rows 0..3 are dw_pre, dw_post, db_pre, db_post (all units), 4 + g
 // the gate rows (their own chunks).
 struct JoinParams {
   const float* part;
@@ -703,16 +702,16 @@ struct JoinParams {
 
 constexpr int kJoinSplit = 32;
 
-__global__ void __launch_bounds__(16 * kJoinSplit) fo_norm_join_kernel(const JoinParams p) {
-  __shared__ float4 red[2][kJoinSplit][16];
+__global__ void __launch_bounds__(8 * kJoinSplit) fo_norm_join_kernel(const JoinParams p) {
+  __shared__ float4 red[2][kJoinSplit][8];
   griddep_launch_dependents();
   griddep_wait();
   const int k = min(static_cast<int>(blockIdx.x), 4);
   if (p.out[k] == nullptr) return;
   const int g = static_cast<int>(blockIdx.x) - 4;
   const int lo = k < 4 ? 0 : g * p.chunks, hi = k < 4 ? p.units : lo + p.chunks;
-  const int lane = threadIdx.x & 15, split = threadIdx.x >> 4;
-  const int c = blockIdx.y * 64 + lane * 4;
+  const int lane = threadIdx.x & 7, split = threadIdx.x >> 3;
+  const int c = blockIdx.y * 32 + lane * 4;
   const bool gated = (k == 1 || k == 3) && p.gate != nullptr;  // sums weighted by each unit's gate row
   // dw_pre: dz rhat; dw_post, dgate: t yhat; db_pre: dz; db_post (and dgate's bias part): t
   const int slot = k == 0 ? 0 : k == 2 ? 2 : k == 3 ? 3 : 1;
@@ -750,8 +749,8 @@ __global__ void __launch_bounds__(16 * kJoinSplit) fo_norm_join_kernel(const Joi
 #pragma unroll
   for (int h = 0; h < 2; ++h) red[h][split][lane] = make_float4(a[h][0], a[h][1], a[h][2], a[h][3]);
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int cc = blockIdx.y * 64 + threadIdx.x;
+  if (threadIdx.x < 32) {
+    const int cc = blockIdx.y * 32 + threadIdx.x;
     float t = 0.f, t1 = 0.f;
 #pragma unroll
     for (int s = 0; s < kJoinSplit; ++s) {
@@ -994,7 +993,7 @@ extern "C" int fo_block_norm_backward(const FoBlockNormDesc* d, void* stream) {
   j.w_post = d->w_post, j.b_post = d->b_post, j.gate = d->gate, j.ldgate = d->ldgate;
   j.units = b.units, j.chunks = b.chunks, j.ldp = b.ldp, j.D = D, j.vec_dtype = d->vec_dtype;
   const unsigned outs = 4u + (d->gate != nullptr ? static_cast<unsigned>(b.groups) : 0u);
-  e = launch_pdl(fo_norm_join_kernel, g_no_opt, dim3(outs, (D + 63) / 64), dim3(16 * kJoinSplit), 0, 1, st, j);
+  e = launch_pdl(fo_norm_join_kernel, g_no_opt, dim3(outs, (D + 31) / 32), dim3(8 * kJoinSplit), 0, 1, st, j);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   host_count_launches(2);
   return host_ok();
