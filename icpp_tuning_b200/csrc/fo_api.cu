@@ -1066,6 +1066,19 @@ int host_tmap(CUtensorMap* m, int dt, const void* base, uint64_t inner, uint64_t
   return make_tmap(m, dt, base, inner, outer, row_bytes, box_inner, box_outer, what);
 }
 
+int host_tmap_planes(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t row_bytes,
+                     const char* what) {
+  auto encode = encode_fn();
+  if (encode == nullptr) return fail(FO_ECUDA, "cuTensorMapEncodeTiled is unavailable in the driver");
+  const cuuint64_t dims[3] = {inner, outer, planes}, strides[2] = {row_bytes, row_bytes * outer};
+  const cuuint32_t box[3] = {32, 32, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FO_EINVAL, "tensor map for %s rejected by the driver (CUresult %d)", what, static_cast<int>(r));
+  return FO_OK;
+}
+
 void host_count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n)); }
 
 }  // namespace fo

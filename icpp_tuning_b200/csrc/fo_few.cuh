@@ -225,15 +225,15 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
         static_cast<unsigned short*>(p.g)[t * p.ldg + f] = to16(v, p.bf16);
         static_cast<unsigned short*>(p.u)[t * p.ldu + f] = to16(w, p.bf16);
       }
-      *out = to16(gate_act<ACT>(v) * w, p.bf16);
+      *out = to16(both(gate_act<ACT>(two(v))).x * w, p.bf16);
     } else if constexpr (MODE == FEW_DGATE) {
       const float sg = from16(__ldg(static_cast<const unsigned short*>(p.sg) + t * p.ldsg + f), p.bf16);
       const float su = from16(__ldg(static_cast<const unsigned short*>(p.su) + t * p.ldsu + f), p.bf16);
-      float dg, du, h;
-      gate_grad<ACT>(v, sg, su, dg, du, h);
-      *out = to16(dg, p.bf16);
-      static_cast<unsigned short*>(p.g)[t * p.ldg + f] = to16(du, p.bf16);
-      static_cast<unsigned short*>(p.u)[t * p.ldu + f] = to16(h, p.bf16);
+      Two dg, du, h;
+      gate_grad<ACT>(two(v), two(sg), two(su), dg, du, h);
+      *out = to16(both(dg).x, p.bf16);
+      static_cast<unsigned short*>(p.g)[t * p.ldg + f] = to16(both(du).x, p.bf16);
+      static_cast<unsigned short*>(p.u)[t * p.ldu + f] = to16(both(h).x, p.bf16);
     } else {
       *out = to16(v, p.bf16);
     }

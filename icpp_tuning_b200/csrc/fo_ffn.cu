@@ -33,6 +33,26 @@ cudaError_t launch(int epi, int act, const FfnMaps& m, const FfnParams& p, int p
   return p.bf16 ? by_act<FFN_DGATE, DT_BF16>(act, m, p, pairs, s) : by_act<FFN_DGATE, DT_F16>(act, m, p, pairs, s);
 }
 
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t kblocks(int64_t k) { return (k + kBK - 1) / kBK; }
+
+// Parts to cut a product's K into: its tiles of kb K blocks beside `others` K blocks of other
+// units on `pairs` CTA pairs.  A cut costs a pass over the parts (about 10 K blocks' time),
+// so it has to shorten the longest chain by more.
+int cut(int64_t M, int64_t N, int64_t kb, int64_t others, int pairs) {
+  const int64_t tiles = (M + kFfnTile - 1) / kFfnTile * ((N + kFfnTile - 1) / kFfnTile);
+  int best = 1;
+  int64_t best_cost = 0;
+  for (int s = 1; s <= kFfnMaxParts && s <= kb; ++s) {
+    const int64_t unit = (kb + s - 1) / s + 8, units = tiles * s;
+    const int64_t mean = (units * unit + others + pairs - 1) / pairs;
+    const int64_t rounds = others > 0 ? (units + pairs - 1) / pairs * unit : (units + pairs - 1) / pairs * unit;
+    const int64_t cost = (mean > rounds ? mean : rounds) + (s > 1 ? 10 + s : 0);
+    if (best_cost == 0 || cost < best_cost) best = s, best_cost = cost;
+  }
+  return best;
+}
+
 // A stored matrix [rows, cols], row-major.
 struct Mat {
   const void* p;
@@ -43,6 +63,7 @@ struct Mat {
 struct Build {
   FfnMaps maps;
   FfnParams p;
+  JoinPartsParams join = {};
   int dt;
   int rc = FO_OK;
 
@@ -69,14 +90,16 @@ struct Build {
     q.tiles_n = (q.N + tile_n - 1) / tile_n;
     q.kb0 = static_cast<int>((K + kBK - 1) / kBK);
     q.kb = segments * q.kb0;
+    q.parts = 1;
     q.unit0 = p.units;
     p.units += q.tiles_m * q.tiles_n;
     return q;
   }
 
-  // C [M, N] = op(A) op(B) over K (a second pair of operands: a second K segment).
+  // C [M, N] = op(A) op(B) over K (a second pair of operands: a second K segment); parts > 1:
+  // fp32 parts in `part`, to be joined into C by join().
   void product(int64_t M, int64_t N, int64_t K, const Mat& a, bool a_t, const Mat& b, bool b_t, const Mat& c,
-               const Mat* a1 = nullptr, const Mat* b1 = nullptr) {
+               const Mat* a1 = nullptr, const Mat* b1 = nullptr, int parts = 1, void* part = nullptr) {
     FfnProblem& q = add(M, N, K, kFfnTile, a1 != nullptr ? 2 : 1);
     const int i = p.nprob - 1;
     q.a_mn = a_t, q.b_mn = b_t;
@@ -86,7 +109,25 @@ struct Build {
       operand(&maps.a[i][1], *a1, a_t, "a product's first operand");
       operand(&maps.b[i][1], *b1, b_t, "a product's second operand");
     }
-    map(&maps.c[i], c, 32, "a product's output");
+    if (parts > 1) {
+      q.parts = parts;
+      p.units += (parts - 1) * q.tiles_m * q.tiles_n;
+      join = {static_cast<const float*>(part), const_cast<void*>(c.p), q.M, q.N, parts, pad8(N), c.ld};
+      if (rc == FO_OK) rc = host_tmap_planes(&maps.c[i], part, N, M, parts, static_cast<uint64_t>(pad8(N)) * 4, "a product's parts");
+    } else {
+      map(&maps.c[i], c, 32, "a product's output");
+    }
+  }
+
+  // Launches the products (and the join of the one that was cut).
+  cudaError_t run(const HostDevice& hd, cudaStream_t st) {
+    cudaError_t e = launch(FFN_GRADS, 0, maps, p, hd.sms / 2, st);
+    if (e != cudaSuccess || join.parts < 2) return e;
+    static std::atomic<uint64_t> none{0};
+    const long long n = static_cast<long long>(join.M) * (join.ldp / 8);
+    const long long blocks = (n + 255) / 256, most = 8ll * hd.sms;
+    return launch_pdl(p.bf16 ? fo_ffn_join_kernel<DT_BF16> : fo_ffn_join_kernel<DT_F16>, none, dim3(static_cast<unsigned>(blocks < most ? blocks : most)),
+                      dim3(256), 0, 1, st, join);
   }
 
   // Names each unit's pair when the problems' K differ: longest first, to the pair with the
@@ -101,18 +142,16 @@ struct Build {
     p.owned = 1;
     for (int i = 0; i < p.nprob; ++i) {
       const FfnProblem& q = p.prob[i];
-      for (int t = 0; t < q.tiles_m * q.tiles_n; ++t) {
+      for (int t = 0; t < q.tiles_m * q.tiles_n * q.parts; ++t) {
         int best = 0;
         for (int c = 1; c < pairs; ++c)
           if (load[c] < load[best]) best = c;
         p.owner[q.unit0 + t] = static_cast<unsigned char>(best);
-        load[best] += q.kb + 8;  // the tile's K blocks and about its epilogue
+        load[best] += q.kb / q.parts + 8;  // the unit's K blocks and about its epilogue
       }
     }
   }
 };
-
-int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
 int check_mat(const void* p, int64_t ld, int64_t cols, const char* name) {
   if (p == nullptr || !host_aligned16(p)) return host_fail(FO_EINVAL, "%s must be a 16-byte aligned device pointer", name);
@@ -150,29 +189,42 @@ namespace {
 
 
 int few_most() {
-  static const int v = getenv("FO_FEW") ? atoi(getenv("FO_FEW")) : 256;
+  static const int v = getenv("FO_FEW") ? atoi(getenv("FO_FEW")) : 32;
   return v;
 }
 
 constexpr int kSms = 148;
 
-int64_t kblocks(int64_t k) { return (k + kBK - 1) / kBK; }
-
-// The short-token products of a call.
+// How a call runs: on the short-token kernels, or on CTA pairs with the product that has few
+// tiles (forward: down, backward: dx) cut into parts.
 struct Few {
   bool on;
   FewPlan first, second;  // forward: gated, down; backward: dgate, dx
+  int parts;
+  size_t matrices, bytes;  // the workspace: h, or dg, du, h; then the parts
 };
 
 Few few_of(const FoGatedFfnDesc* d, bool backward) {
   Few f{};
-  f.on = d->T <= few_most();
+  f.matrices = (static_cast<size_t>(d->T) * pad8(d->F) * 2 * (backward ? 3 : 1) + 255) / 256 * 256;
+  f.bytes = f.matrices;
+  f.parts = 1;
+  f.on = d->T <= (backward ? few_most() * 2 : few_most());
   if (f.on) {
     f.first = backward ? few_plan(FEW_DGATE, d->F, d->T, static_cast<int>(kblocks(d->N)), kSms)
                        : few_plan(FEW_GATED, d->F, d->T, static_cast<int>(kblocks(d->D)), kSms);
     f.second = backward ? few_plan(FEW_PLAIN, d->D, d->T, static_cast<int>(2 * kblocks(d->F)), kSms)
                         : few_plan(FEW_PLAIN, d->N, d->T, static_cast<int>(kblocks(d->F)), kSms);
+    return f;
   }
+  if (backward) {
+    auto tiles = [](int64_t a, int64_t b) { return (a + kFfnTile - 1) / kFfnTile * ((b + kFfnTile - 1) / kFfnTile); };
+    const int64_t others = (2 * tiles(d->D, d->F) + tiles(d->F, d->N)) * (kblocks(d->T) + 8);
+    f.parts = cut(d->T, d->D, 2 * kblocks(d->F), others, kSms / 2);
+  } else {
+    f.parts = cut(d->T, d->N, kblocks(d->F), 0, kSms / 2);
+  }
+  if (f.parts > 1) f.bytes += static_cast<size_t>(f.parts) * d->T * pad8(backward ? d->D : d->N) * 4;
   return f;
 }
 
@@ -203,7 +255,7 @@ struct FewBuild {
 
 extern "C" size_t fo_gated_ffn_workspace_size(const FoGatedFfnDesc* d, int32_t backward) {
   if (d == nullptr || d->T <= 0 || d->F <= 0) return 0;
-  return static_cast<size_t>(d->T) * fo::pad8(d->F) * 2 * (backward ? 3 : 1);
+  return fo::few_of(d, backward != 0).bytes;
 }
 
 extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
@@ -267,11 +319,12 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
   if (e != cudaSuccess) return fail_launch(e);
 
   Build y(d->dtype, hd);
-  y.product(d->T, d->N, d->F, h, false, wd, kn, {d->y, d->T, d->N, d->ldy});
+  y.product(d->T, d->N, d->F, h, false, wd, kn, {d->y, d->T, d->N, d->ldy}, nullptr, nullptr, few.parts,
+            static_cast<char*>(d->workspace) + few.matrices);
   if (y.rc) return y.rc;
-  e = launch(FFN_GRADS, 0, y.maps, y.p, hd.sms / 2, st);
+  e = y.run(hd, st);
   if (e != cudaSuccess) return fail_launch(e);
-  host_count_launches(2);
+  host_count_launches(few.parts > 1 ? 3 : 2);
   return host_ok();
 }
 
@@ -334,9 +387,7 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
     q.b_mn = !kn;
     b.operand(&b.maps.a[0][0], dy, false, "dy");
     b.operand(&b.maps.b[0][0], wd, !kn, "w_down");
-    b.map(&b.maps.c[0], dg, 32, "dg");
-    b.map(&b.maps.c[1], du, 32, "du");
-    b.map(&b.maps.c[2], h, 32, "h");
+    b.p.dg = const_cast<void*>(dg.p), b.p.du = const_cast<void*>(du.p), b.p.h = const_cast<void*>(h.p), b.p.ldo = ldf;
     b.p.g = d->g, b.p.u = d->u, b.p.ldg = d->ldg, b.p.ldu = d->ldu;
     if (b.rc) return b.rc;
     e = launch(FFN_DGATE, d->act, b.maps, b.p, hd.sms / 2, st);
@@ -344,7 +395,9 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   }
 
   Build w(d->dtype, hd);
-  auto add_dx = [&] { w.product(d->T, d->D, d->F, dg, false, wg, !kn, {d->dx, d->T, d->D, d->lddx}, &du, &wu); };
+  auto add_dx = [&] {
+    w.product(d->T, d->D, d->F, dg, false, wg, !kn, {d->dx, d->T, d->D, d->lddx}, &du, &wu, few.parts, ws + few.matrices);
+  };
   auto add_weights = [&] {
     const Mat owg{d->dw_gate, up_rows, up_cols, d->lddwg}, owu{d->dw_up, up_rows, up_cols, d->lddwu};
     const Mat owd{d->dw_down, down_rows, down_cols, d->lddwd};
@@ -360,7 +413,7 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   };
   if (few.on) {
     add_weights();
-  } else if (2 * d->F >= d->T) {  // longest tiles first
+  } else if (2 * d->F / few.parts >= d->T) {  // longest units first
     add_dx();
     add_weights();
   } else {
@@ -369,8 +422,8 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   }
   if (w.rc) return w.rc;
   w.schedule(hd.sms / 2);
-  e = launch(FFN_GRADS, 0, w.maps, w.p, hd.sms / 2, st);
+  e = w.run(hd, st);
   if (e != cudaSuccess) return fail_launch(e);
-  host_count_launches(few.on ? 3 : 2);
+  host_count_launches(few.on || few.parts > 1 ? 3 : 2);
   return host_ok();
 }

@@ -11,7 +11,8 @@
 //   FFN_DGATE  acc = dh = dy Wd^T; reads g, u and writes dg = dh u act'(g), du = dh act(g),
 //              h = act(g) u: the block's whole elementwise backward, dh never in memory
 //   FFN_GRADS  plain products, up to four of them in one launch, each over one or two K
-//              segments with their own operands (dx = dg Wg^T + du Wu^T)
+//              segments with their own operands (dx = dg Wg^T + du Wu^T); a product of few
+//              tiles and long K is cut along K into fp32 parts, which the next launch joins
 // Operands are K-major or MN-major (read transposed) per problem, so every product of the
 // block and its gradients runs on tensors as they are, without a transposition pass.
 #pragma once
@@ -20,6 +21,7 @@
 namespace fo {
 
 enum : int { FFN_GATED = 0, FFN_DGATE = 1, FFN_GRADS = 2 };
+constexpr int kFfnMaxParts = 8;
 
 constexpr int kFfnStages = 3;  // of two 64-wide k-blocks: 64 KB a stage and CTA
 constexpr int kFfnKps = 2;
@@ -35,6 +37,8 @@ struct FfnProblem {
   int unit0;           // first unit of this problem
   int kb0, kb;         // k-blocks of the first segment, of all
   int a_mn, b_mn;      // operands read transposed
+  int parts;           // > 1: units are (tile, part), K blocks [kb part / parts, kb (part + 1) / parts);
+                       // part q goes to plane q of an fp32 output
 };
 
 struct FfnMaps {
@@ -45,39 +49,20 @@ struct FfnParams {
   FfnProblem prob[kFfnMaxProblems];
   int nprob, units, group_m;
   int bf16, save;
-  const void *g, *u;  // FFN_DGATE
+  const void *g, *u;  // FFN_DGATE: saved; dg, du and h are written, rows ldo (a multiple of 8) apart
   long long ldg, ldu;
+  void *dg, *du, *h;
+  long long ldo;
   int* status;
   unsigned long long timeout_ns;
   int owned;  // owner[u] names the pair that runs unit u (else pair u % pairs)
   unsigned char owner[kFfnOwners];
 };
 
-// dg and du of one value from dh; h too.
-template <int ACT>
-__device__ __forceinline__ void gate_grad(float dh, float g, float u, float& dg, float& du, float& h) {
-  float s, ds;
-  if constexpr (ACT == ACT_SILU) {
-    const float p = sigmoid_fast(g);
-    s = g * p;
-    ds = fmaf(s, 1.0f - p, p);
-  } else if constexpr (ACT == ACT_GELU_TANH) {
-    // gelu_tanh(g) = g p, p = sigmoid(2 w), w = c (g + 0.044715 g^3): derivative p + g p (1 - p) 2 w'
-    const float g2 = g * g;
-    const float p = sigmoid_fast(1.5957691216057308f * fmaf(0.044715f * g, g2, g));
-    s = g * p;
-    ds = fmaf(s * (1.0f - p), 1.5957691216057308f * fmaf(0.134145f, g2, 1.0f), p);
-  } else if constexpr (ACT == ACT_GELU_ERF) {
-    const float c = 0.5f * (1.0f + erf_as7128(g * 0.7071067811865476f));
-    s = g * c;
-    ds = fmaf(g * 0.3989422804014327f, __expf(-0.5f * g * g), c);
-  } else {
-    s = g < 0.f ? 0.f : g;
-    ds = g > 0.f ? 1.f : 0.f;
-  }
-  dg = dh * u * ds;
-  du = dh * s;
-  h = s * u;
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(m), "r"(src), "r"(x),
+               "r"(y), "r"(z)
+               : "memory");
 }
 
 __device__ __forceinline__ void ffn_error(const FfnParams& p, int where) {
@@ -88,7 +73,7 @@ __device__ __forceinline__ void ffn_error(const FfnParams& p, int where) {
 }
 
 struct FfnUnit {
-  int pr, tm, tn;
+  int pr, tm, tn, part;
 };
 
 __device__ __forceinline__ FfnUnit ffn_unit(const FfnParams& p, int u) {
@@ -96,7 +81,13 @@ __device__ __forceinline__ FfnUnit ffn_unit(const FfnParams& p, int u) {
   r.pr = 0;
   while (r.pr + 1 < p.nprob && u >= p.prob[r.pr + 1].unit0) ++r.pr;
   const FfnProblem& q = p.prob[r.pr];
-  const int t = u - q.unit0;
+  int t = u - q.unit0;
+  r.part = 0;
+  if (q.parts > 1) {
+    const int tiles = q.tiles_m * q.tiles_n;
+    r.part = t / tiles;
+    t -= r.part * tiles;
+  }
   const int per = p.group_m * q.tiles_n;  // rasters of group_m row blocks, for reuse in L2
   const int gr = t / per, in = t - gr * per;
   const int gm = min(p.group_m, q.tiles_m - gr * p.group_m);
@@ -151,7 +142,7 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
   if (threadIdx.x == 64) {
     tma_prefetch_desc(&maps.a[0][0]);
     tma_prefetch_desc(&maps.b[0][0]);
-    tma_prefetch_desc(&maps.c[0]);
+    if (EPI != FFN_DGATE) tma_prefetch_desc(&maps.c[0]);
   }
   __syncwarp();
   tc_fence_before();
@@ -175,11 +166,14 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
         const int bcol = EPI == FFN_GATED ? un.tn * 128 : un.tn * kFfnTile + static_cast<int>(rank) * 128;
         // everything of the problem in registers: a constant read costs this one thread as
         // much as issuing a copy
-        const int kb = q.kb, a_mn = q.a_mn, b_mn = q.b_mn;
-        int left = q.kb0, k = 0;  // K blocks left in the segment, the next one's first column
-        const CUtensorMap* ma = &maps.a[un.pr][0];
-        const CUtensorMap* mB = EPI == FFN_GATED ? &maps.b[0][rank] : &maps.b[un.pr][0];
-        for (int k0 = 0; k0 < kb; k0 += kFfnKps) {
+        const int a_mn = q.a_mn, b_mn = q.b_mn;
+        const int kbeg = q.kb * un.part / q.parts, kb = q.kb * (un.part + 1) / q.parts;
+        const int seg = EPI == FFN_GRADS && kbeg >= q.kb0;
+        // K blocks left in the segment, the next one's first column
+        int left = seg ? q.kb : q.kb0 - kbeg, k = (kbeg - (seg ? q.kb0 : 0)) * kBK;
+        const CUtensorMap* ma = &maps.a[un.pr][seg];
+        const CUtensorMap* mB = EPI == FFN_GATED ? &maps.b[0][rank] : &maps.b[un.pr][seg];
+        for (int k0 = kbeg; k0 < kb; k0 += kFfnKps) {
           if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, tmo, abort_flag)) {
             ok = false;
             break;
@@ -236,8 +230,10 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
       uint64_t off = 0;  // of stage s, in descriptor units (A and B stages are alike)
       bool ok = true;
       for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
-        const FfnProblem& q = p.prob[EPI == FFN_GRADS ? ffn_unit(p, u).pr : 0];
-        const int kb = q.kb, a_mn = q.a_mn, b_mn = q.b_mn;
+        const FfnUnit un = ffn_unit(p, u);
+        const FfnProblem& q = p.prob[un.pr];
+        const int a_mn = q.a_mn, b_mn = q.b_mn;
+        const int kbeg = q.kb * un.part / q.parts, kb = q.kb * (un.part + 1) / q.parts;
         const uint32_t idesc = idesc_f16(p.bf16, b_mn, 256, 256) | (static_cast<uint32_t>(a_mn) << 15);
         const uint64_t a0 = a_mn ? sdesc_sw128(sA, 64 * 128, 1024) : sdesc_sw128(sA, 16, 1024);
         const uint64_t b0 = b_mn ? sdesc_sw128(sB, 64 * 128, 1024) : sdesc_sw128(sB, 16, 1024);
@@ -250,7 +246,7 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
         tc_fence_after();
         const uint32_t d = tmem_base + acc * 256;
         uint32_t accum = 0;
-        for (int k0 = 0; k0 < kb; k0 += kFfnKps) {
+        for (int k0 = kbeg; k0 < kb; k0 += kFfnKps) {
           const int nk = min(kFfnKps, kb - k0);
           if (!mbar_wait(bar_full + 8 * s, ph, tmo, abort_flag)) {
             ok = false;
@@ -328,6 +324,49 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_shared(bar_tempty + 8 * acc, 0));
     };
+    // FFN_DGATE: the two staging blocks in turn: a lane may write one while others still read
+    // the other, and meets them at the barrier between.
+    int turn = 0;
+    auto block = [&]() {
+      turn ^= 1;
+      return buf + (turn ? 2048u : 0u);
+    };
+    auto st_block = [&](uint32_t blk, int r, int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(blk + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)), "r"(a), "r"(b),
+                   "r"(c), "r"(d)
+                   : "memory");
+    };
+    // 32 rows x 32 columns of g and u: four lanes a row, eight rows a load.
+    uint4 pg[EPI == FFN_DGATE ? 4 : 1], pu[EPI == FFN_DGATE ? 4 : 1];
+    auto ask_gu = [&](int u, int ch) {
+      if constexpr (EPI == FFN_DGATE) {
+        const FfnUnit un = ffn_unit(p, u);
+        const FfnProblem& q = p.prob[0];
+        const int col = un.tn * kFfnTile + half * 128 + ch * 32 + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = un.tm * kFfnTile + static_cast<int>(rank) * 128 + quarter * 32 + i * 8 + (lane >> 2);
+          pg[i] = pu[i] = make_uint4(0u, 0u, 0u, 0u);
+          const unsigned short* gp = static_cast<const unsigned short*>(p.g) + row * p.ldg + col;
+          const unsigned short* up = static_cast<const unsigned short*>(p.u) + row * p.ldu + col;
+          if (row < q.M && col + 8 <= q.N) {
+            pg[i] = __ldg(reinterpret_cast<const uint4*>(gp));
+            pu[i] = __ldg(reinterpret_cast<const uint4*>(up));
+          } else if (row < q.M && col < q.N) {  // the last, partial eight columns
+            uint32_t x[8] = {}, y[8] = {};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (col + k < q.N) x[k] = gp[k], y[k] = up[k];
+            pg[i] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+            pu[i] = make_uint4(y[0] | y[1] << 16, y[2] | y[3] << 16, y[4] | y[5] << 16, y[6] | y[7] << 16);
+          }
+        }
+      }
+    };
+    if (EPI == FFN_DGATE) {
+      const int u = ffn_next(p, first, cid, ncl);
+      if (u < p.units) ask_gu(u, 0);
+    }
     for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
       const FfnUnit un = ffn_unit(p, u);
       const FfnProblem& q = p.prob[un.pr];
@@ -371,67 +410,89 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            w[i] = pack2<DT>(gate_act<ACT>(__uint_as_float(g[2 * i])) * __uint_as_float(v[2 * i]),
-                             gate_act<ACT>(__uint_as_float(g[2 * i + 1])) * __uint_as_float(v[2 * i + 1]));
+            w[i] = pack2<DT>(mul2(gate_act<ACT>(two(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]))),
+                                  two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]))));
 #pragma unroll
           for (int j = 0; j < 4; ++j) put(sub * 4 + j, w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         }
         end(&maps.c[0], col, row0, q);
       } else if constexpr (EPI == FFN_DGATE) {
-        const int row = row0 + lane;
+        // 32 columns at a time.  g and u are asked for one step ahead; they and the results
+        // cross HBM as 64 contiguous bytes a row and change hands in shared memory, between
+        // that layout and a lane's own row, in two 32 x 64 B blocks a warp.  (TMA stores had
+        // to wait for each other's reads of the staging memory: 10 us a tile.)
 #pragma unroll 1
-        for (int ch = 0; ch < 2; ++ch) {
-          const int col = un.tn * kFfnTile + half * 128 + ch * 64;
-          uint32_t gq[32], uq[32];
-          const unsigned short* gp = static_cast<const unsigned short*>(p.g) + row * p.ldg + col;
-          const unsigned short* up = static_cast<const unsigned short*>(p.u) + row * p.ldu + col;
+        for (int ch = 0; ch < 4; ++ch) {
+          const int col = un.tn * kFfnTile + half * 128 + ch * 32;
+          uint32_t gq[16], uq[16];
+          auto own_row = [&](const uint4 (&src)[4], uint32_t (&dst)[16]) {
+            const uint32_t blk = block();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-            if (row < q.M && col + 8 * j + 8 <= q.N) {
-              a = __ldg(reinterpret_cast<const uint4*>(gp) + j);
-              b = __ldg(reinterpret_cast<const uint4*>(up) + j);
-            } else if (row < q.M && col + 8 * j < q.N) {  // the last, partial eight columns
-              uint32_t x[8] = {}, y[8] = {};
+            for (int i = 0; i < 4; ++i) st_block(blk, i * 8 + (lane >> 2), lane & 3, src[i].x, src[i].y, src[i].z, src[i].w);
+            __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (col + 8 * j + i < q.N) x[i] = gp[8 * j + i], y[i] = up[8 * j + i];
-              a = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
-              b = make_uint4(y[0] | y[1] << 16, y[2] | y[3] << 16, y[4] | y[5] << 16, y[6] | y[7] << 16);
+            for (int j = 0; j < 4; ++j) {
+              const uint4 v = lds128(blk + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+              dst[4 * j] = v.x, dst[4 * j + 1] = v.y, dst[4 * j + 2] = v.z, dst[4 * j + 3] = v.w;
             }
-            gq[4 * j] = a.x, gq[4 * j + 1] = a.y, gq[4 * j + 2] = a.z, gq[4 * j + 3] = a.w;
-            uq[4 * j] = b.x, uq[4 * j + 1] = b.y, uq[4 * j + 2] = b.z, uq[4 * j + 3] = b.w;
+          };
+          own_row(pg, gq);
+          own_row(pu, uq);
+          {  // the next 32 columns, of this tile or of this pair's next one
+            int un2 = u;
+            if (ch == 3) un2 = ffn_next(p, u + step, cid, ncl);
+            if (un2 < p.units) ask_gu(un2, (ch + 1) & 3);
           }
-          begin();
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tb + half * 128 + ch * 32, r);
+          tc_wait_ld_regs(r);
+          if (ch == 3) release();
+          uint32_t w[16];
 #pragma unroll
-          for (int sub = 0; sub < 2; ++sub) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(tb + half * 128 + ch * 64 + sub * 32, r);
-            tc_wait_ld_regs(r);
-            if (ch == 1 && sub == 1) release();
-            uint32_t w[16];
+          for (int i = 0; i < 16; ++i) {
+            const float2 g2 = unpack2<DT>(gq[i]), u2 = unpack2<DT>(uq[i]);
+            Two dg, du, h;
+            gate_grad<ACT>(two(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), two(g2.x, g2.y), two(u2.x, u2.y), dg, du, h);
+            w[i] = pack2<DT>(dg);
+            gq[i] = pack2<DT>(du);  // g and u give way to du and h
+            uq[i] = pack2<DT>(h);
+          }
+          auto store = [&](void* out, const uint32_t (&v)[16]) {
+            const uint32_t blk = block();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 g2 = unpack2<DT>(gq[sub * 16 + i]), u2 = unpack2<DT>(uq[sub * 16 + i]);
-              float dg0, dg1, du0, du1, h0, h1;
-              gate_grad<ACT>(__uint_as_float(r[2 * i]), g2.x, u2.x, dg0, du0, h0);
-              gate_grad<ACT>(__uint_as_float(r[2 * i + 1]), g2.y, u2.y, dg1, du1, h1);
-              w[i] = pack2<DT>(dg0, dg1);
-              gq[sub * 16 + i] = pack2<DT>(du0, du1);  // g and u give way to du and h
-              uq[sub * 16 + i] = pack2<DT>(h0, h1);
+            for (int j = 0; j < 4; ++j) st_block(blk, lane, j, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            __syncwarp();
+            const int c = col + (lane & 3) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + (lane >> 2);
+              const uint4 t = lds128(blk + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+              unsigned short* dst = static_cast<unsigned short*>(out) + (row0 + rr) * p.ldo + c;
+              if (row0 + rr < q.M && c < q.N) *reinterpret_cast<uint4*>(dst) = t;  // rows are padded to 8 columns
             }
+          };
+          store(p.dg, w);
+          store(p.du, gq);
+          store(p.h, uq);
+        }
+      } else if (q.parts > 1) {
+        // an fp32 part: 32 columns are a 128-byte row
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          const int col = un.tn * kFfnTile + half * 128 + ch * 32;
+          begin();
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tb + half * 128 + ch * 32, r);
+          tc_wait_ld_regs(r);
+          if (ch == 3) release();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) put(sub * 4 + j, w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          for (int j = 0; j < 8; ++j) put(j, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < q.M && col < q.N) tma_store_3d(&maps.c[un.pr], buf, col, row0, un.part);
+            bulk_commit();
           }
-          end(&maps.c[0], col, row0, q);
-          begin();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) put(j, gq[4 * j], gq[4 * j + 1], gq[4 * j + 2], gq[4 * j + 3]);
-          end(&maps.c[1], col, row0, q);
-          begin();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) put(j, uq[4 * j], uq[4 * j + 1], uq[4 * j + 2], uq[4 * j + 3]);
-          end(&maps.c[2], col, row0, q);
         }
       } else {
 #pragma unroll 1
@@ -472,6 +533,43 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// Joins the fp32 parts [parts][M][ldp] of a product in part order and rounds once.
+struct JoinPartsParams {
+  const float* part;
+  void* out;
+  int M, N, parts;
+  long long ldp, ldo;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(256) fo_ffn_join_kernel(const JoinPartsParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int per_row = static_cast<int>(p.ldp / 8);  // ldp: N rounded up to 8
+  const long long n = static_cast<long long>(p.M) * per_row, plane = p.M * p.ldp;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256) {
+    const int row = static_cast<int>(i / per_row), c = static_cast<int>(i - static_cast<long long>(row) * per_row) * 8;
+    const float* src = p.part + row * p.ldp + c;
+    float v[8] = {};
+#pragma unroll
+    for (int q = 0; q < kFfnMaxParts; ++q) {
+      if (q >= p.parts) break;
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(src + q * plane)), b = __ldcg(reinterpret_cast<const float4*>(src + q * plane) + 1);
+      v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    }
+    unsigned short* dst = static_cast<unsigned short*>(p.out) + row * p.ldo + c;
+    const uint4 w = make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
+    if (c + 8 <= p.N) {
+      *reinterpret_cast<uint4*>(dst) = w;
+    } else {
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < p.N) dst[j] = static_cast<unsigned short>(u[j / 2] >> (16 * (j & 1)));
+    }
   }
 }
 

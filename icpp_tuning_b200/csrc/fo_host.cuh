@@ -33,6 +33,9 @@ int host_device(HostDevice* out);
 // 2-D row-major map [outer, inner] with 128-byte swizzled boxes of box_inner x box_outer.
 int host_tmap(CUtensorMap* m, int dt, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
               uint32_t box_inner, uint32_t box_outer, const char* what);
+// fp32 planes [planes, outer, inner], rows `row_bytes` apart, boxes of 32 x 32 x 1.
+int host_tmap_planes(CUtensorMap* m, const void* base, uint64_t inner, uint64_t outer, uint64_t planes, uint64_t row_bytes,
+                     const char* what);
 void host_count_launches(int n);
 
 inline bool host_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -24,6 +24,7 @@
 // sum(t), db_post = gate sum(t) are formed once a gate row, in the kernel that joins the
 // CTAs' sums in a fixed order.
 #include "fo_host.cuh"
+#include "fo_math.cuh"
 #include "fo_skinny.cuh"
 #include "../../include/b200fo.h"
 
@@ -47,43 +48,6 @@ struct NormParams {
   int* status;
   unsigned long long timeout_ns;
 };
-
-// Two fp32 values in one 64-bit register: sm_100 adds and multiplies both in one
-// instruction, which halves these kernels' arithmetic (they issue about 25 instructions a
-// value, and at twice that would be bound by issue, not by HBM).
-struct Two {
-  uint64_t v;
-};
-__device__ __forceinline__ Two two(float a, float b) {
-  Two r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ Two two(float a) { return two(a, a); }
-__device__ __forceinline__ float2 both(Two a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
-  return r;
-}
-__device__ __forceinline__ float sum(Two a) {
-  const float2 f = both(a);
-  return f.x + f.y;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-  Two r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-  Two r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-  Two r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 
 // Where a thread's NP pairs of columns lie.  VEC 8: pair e is columns 2 (e % 4) of the
 // 16-byte block (e / 4) * 32 W + tid; VEC 1: the single columns 2 e * 32 W + tid and

@@ -17,12 +17,11 @@
 // The 8 warps of a CTA and the CTAs of a cluster split K; partial sums meet in shared
 // memory (distributed across the cluster) and are added in a fixed order.
 #pragma once
-#include "fo_kernel.cuh"
+#include "fo_math.cuh"
 
 namespace fo {
 
 enum : int { W_NK = 0, W_KN = 1, W_Q4 = 2 };
-enum : int { ACT_SILU = 4 };  // beside ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF
 
 struct SkinnyParams {
   const void* x;
@@ -41,25 +40,6 @@ struct SkinnyParams {
   long long ldo, ldg, ldu;
   int early_w;  // the weights are final before the previous kernel ends: prefetch them
 };
-
-// Activations of the gated product in the forms whose error stays at fp32's: the sigmoid
-// forms need one exponential and one reciprocal (gelu_tanh(x) = x sigmoid(2 u)).
-__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
-
-template <int ACT>
-__device__ __forceinline__ float gate_act(float x) {
-  if constexpr (ACT == ACT_SILU) return x * sigmoid_fast(x);
-  if constexpr (ACT == ACT_GELU_TANH) return x * sigmoid_fast(1.5957691216057308f * fmaf(0.044715f * x, x * x, x));
-  if constexpr (ACT == ACT_GELU_ERF) return 0.5f * x * (1.0f + erf_as7128(x * 0.7071067811865476f));
-  return x < 0.f ? 0.f : x;
-}
-
-__device__ __forceinline__ float gate_act(int act, float x) {
-  if (act == ACT_SILU) return gate_act<ACT_SILU>(x);
-  if (act == ACT_GELU_TANH) return gate_act<ACT_GELU_TANH>(x);
-  if (act == ACT_GELU_ERF) return gate_act<ACT_GELU_ERF>(x);
-  return gate_act<ACT_RELU>(x);
-}
 
 template <int DT>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -371,7 +351,7 @@ __global__ void __launch_bounds__(256) fo_skinny_kernel(const SkinnyParams p) {
         static_cast<unsigned short*>(p.g)[row * p.ldg + n] = static_cast<unsigned short>(pack2<DT>(v, 0.f));
         static_cast<unsigned short*>(p.u)[row * p.ldu + n] = static_cast<unsigned short>(pack2<DT>(u, 0.f));
       }
-      v = gate_act(p.act, v) * u;
+      v = both(gate_act(p.act, two(v))).x * u;
     } else if (p.bias != nullptr) {
       v += load_vec(p.bias, DT, n);
     }
