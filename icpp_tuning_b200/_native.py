@@ -26,7 +26,7 @@ FO_B_KN, FO_B_NK = 0, 1
  FO_EPI_BIAS_LN, FO_EPI_RELU, FO_EPI_BIAS_RESIDUAL_LN, FO_EPI_BN, FO_EPI_BN_RELU, FO_EPI_BN_ADD_RELU) = range(11)
 FO_NOALLOC_LN_SCRATCH_BYTES = 8 << 20
 FO_NORM_RMS, FO_NORM_LAYER = 0, 1
-FO_GATE_NONE, FO_GATE_SILU, FO_GATE_GELU_TANH, FO_GATE_GELU_ERF, FO_GATE_RELU = range(5)
+FO_GATE_SILU, FO_GATE_GELU_TANH, FO_GATE_GELU_ERF, FO_GATE_RELU = range(1, 5)
 
 # Every symbol include/b200fo.h declares; tests check the library exports all of them.
 EXPORTED = (
@@ -35,7 +35,7 @@ EXPORTED = (
     "fo_selftest_wait_timeout", "fo_last_error", "fo_version", "fo_launch_count",
     "fo_gemm_bias_layernorm_noalloc", "fo_conv2d_workspace_size",
     "fo_block_norm", "fo_block_norm_backward", "fo_block_norm_backward_workspace_size",
-    "fo_matvec_w4", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
+    "fo_matvec_w4", "fo_gated_ffn_w4", "fo_gated_ffn_w4_workspace_size", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
 )
 
 
@@ -99,8 +99,15 @@ class FoW4(ctypes.Structure):
 
 class FoMatvecW4Desc(ctypes.Structure):
     _fields_ = [("T", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("x", ctypes.c_void_p),
-                ("w", FoW4), ("w_up", FoW4), ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
-                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32)]
+                ("w", FoW4), ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class FoGatedFfnW4Desc(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int64), ("D", ctypes.c_int64), ("F", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("x", ctypes.c_void_p), ("w_gate", FoW4), ("w_up", FoW4), ("w_down", FoW4), ("out", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class FoError(RuntimeError):
@@ -135,6 +142,9 @@ def _declare(l: ctypes.CDLL) -> None:
         f.argtypes, f.restype = [P(FoGatedFfnDesc), ctypes.c_void_p], ctypes.c_int
     l.fo_gated_ffn_workspace_size.argtypes = [P(FoGatedFfnDesc), ctypes.c_int32]
     l.fo_gated_ffn_workspace_size.restype = ctypes.c_size_t
+    l.fo_gated_ffn_w4.argtypes, l.fo_gated_ffn_w4.restype = [P(FoGatedFfnW4Desc), ctypes.c_void_p], ctypes.c_int
+    l.fo_gated_ffn_w4_workspace_size.argtypes = [P(FoGatedFfnW4Desc)]
+    l.fo_gated_ffn_w4_workspace_size.restype = ctypes.c_size_t
     l.fo_matvec_w4.argtypes, l.fo_matvec_w4.restype = [P(FoMatvecW4Desc), ctypes.c_void_p], ctypes.c_int
     l.fo_query_config_legal.argtypes = [ctypes.c_int32, ctypes.c_int32, P(FoTileCfg),
                                         ctypes.c_char_p, ctypes.c_size_t]

@@ -317,42 +317,51 @@ def _w4(w: W4, K: int, dtype: torch.dtype, name: str) -> Tuple[N.FoW4, int]:
                   _ld(scales, n, G, name + ".scales"), _ld(zeros, n, G, name + ".zeros"), group), n
 
 
-def _matvec_w4(x, w, w_up, bias, act):
-    dev = _cuda(x, w.q, w.scales, w.zeros, bias, *(w_up[:3] if w_up is not None else ()))
+def matvec_w4(x: torch.Tensor, w: W4, *, bias: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """x [T, K] @ w^T (+ bias) for a few tokens, w in 4 bits: [T, N] of x's dtype."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return matvec_w4(x, w, bias=bias)
+    dev = _cuda(x, w.q, w.scales, w.zeros, bias)
     T, K = _shape2(x, "x")
     dt = x.dtype
     d = N.FoMatvecW4Desc()
     d.dtype, d.ldx = _sixteen_bit(dt, "x"), _ld(x, T, K, "x")
     d.w, n = _w4(w, K, dt, "w")
     d.T, d.K, d.N = T, K, n
-    if w_up is not None:
-        d.w_up, m = _w4(w_up, K, dt, "w_up")
-        if m != n:
-            raise ValueError(f"w_gate has {n} rows, w_up {m}")
     if bias is not None:
         if bias.dtype is not dt:
             raise ValueError("bias must have the activations' dtype")
         d.bias = _vec(bias, n, "bias").data_ptr()
-    out = _matrix(T, n, x)
-    d.x, d.out, d.ldo, d.act = x.data_ptr(), out.data_ptr(), out.stride(0), act
+    out = x.new_empty((T, n))
+    d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
     _run(dev, N.lib().fo_matvec_w4, ctypes.byref(d))
     return out
 
 
-def matvec_w4(x: torch.Tensor, w: W4, *, bias: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-    """x [T, K] @ w^T (+ bias) for a few tokens, w in 4 bits: [T, N] of x's dtype."""
-    if stream is not None:
-        with torch.cuda.stream(stream):
-            return _matvec_w4(x, w, None, bias, N.FO_GATE_NONE)
-    return _matvec_w4(x, w, None, bias, N.FO_GATE_NONE)
-
-
 def gated_ffn_w4(x: torch.Tensor, w_gate: W4, w_up: W4, w_down: W4, *, act: str = "silu", stream=None) -> torch.Tensor:
-    """(act(x w_gate^T) * (x w_up^T)) w_down^T for a few tokens, all weights in 4 bits.  The
-    product is rounded to x's dtype between the two kernels."""
-    if act not in GATE_ACTS:
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T for a few tokens, all weights in 4 bits: [T, N]
+    of x's dtype.  w_gate and w_up share one group size."""
+    code = GATE_ACTS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(GATE_ACTS)}")
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn_w4(x, w_gate, w_up, w_down, act=act)
-    return _matvec_w4(_matvec_w4(x, w_gate, w_up, None, GATE_ACTS[act]), w_down, None, None, N.FO_GATE_NONE)
+    dev = _cuda(x, *w_gate[:3], *w_up[:3], *w_down[:3])
+    T, D = _shape2(x, "x")
+    dt = x.dtype
+    d = N.FoGatedFfnW4Desc()
+    d.dtype, d.act, d.ldx = _sixteen_bit(dt, "x"), code, _ld(x, T, D, "x")
+    d.w_gate, F = _w4(w_gate, D, dt, "w_gate")
+    d.w_up, F_up = _w4(w_up, D, dt, "w_up")
+    if F_up != F:
+        raise ValueError(f"w_gate has {F} rows, w_up {F_up}")
+    d.w_down, n = _w4(w_down, F, dt, "w_down")
+    d.T, d.D, d.F, d.N = T, D, F, n
+    out = x.new_empty((T, n))
+    ws = x.new_empty((2 * T, (F + 7) // 8 * 8))
+    d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
+    d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * 2
+    _run(dev, N.lib().fo_gated_ffn_w4, ctypes.byref(d))
+    return out

@@ -32,7 +32,7 @@ SOURCES = [
     ("fo_ffn.cu", "fo_ffn", []),
     ("fo_few.cu", "fo_few", []),
     ("fo_norm.cu", "fo_norm", []),
-    ("fo_skinny.cu", "fo_skinny", []),
+    ("fo_w4.cu", "fo_w4", []),
 ]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",

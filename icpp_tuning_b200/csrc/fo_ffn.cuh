@@ -16,7 +16,7 @@
 // Operands are K-major or MN-major (read transposed) per problem, so every product of the
 // block and its gradients runs on tensors as they are, without a transposition pass.
 #pragma once
-#include "fo_skinny.cuh"
+#include "fo_math.cuh"
 
 namespace fo {
 

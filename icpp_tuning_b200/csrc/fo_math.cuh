@@ -1,4 +1,4 @@
-// fo_math.cuh -- paired fp32 arithmetic and the gated activations built on it.
+// fo_math.cuh -- paired fp32 arithmetic, and the gated activations built on it.
 #pragma once
 #include "fo_kernel.cuh"
 
@@ -40,6 +40,12 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
   Two r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
 }
 
 template <int DT>

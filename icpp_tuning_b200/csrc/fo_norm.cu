@@ -25,7 +25,6 @@
 // CTAs' sums in a fixed order.
 #include "fo_host.cuh"
 #include "fo_math.cuh"
-#include "fo_skinny.cuh"
 #include "../../include/b200fo.h"
 
 namespace fo {

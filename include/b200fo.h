@@ -225,7 +225,6 @@ size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* desc);
 
 /* ---- the gated feed-forward block ---------------------------------------------------- */
 /* Activations of the gated products, act(x Wg) * (x Wu). */
-#define FO_GATE_NONE 0
 #define FO_GATE_SILU 1      /* g / (1 + e^-g)                                            */
 #define FO_GATE_GELU_TANH 2
 #define FO_GATE_GELU_ERF 3
@@ -278,21 +277,37 @@ typedef struct FoW4 {
   int32_t group;
 } FoW4;
 
-/* act FO_GATE_NONE: out[T, N] = x[T, K] w^T (+ bias).  Otherwise out = act(x w^T) * (x w_up^T).
- * K a multiple of 32 and at most 1024 groups.  Any T; the weights are read once for every
- * 64 tokens, so it pays for few. */
+/* out[T, N] = x[T, K] w^T (+ bias).  K a multiple of 32.  Any T; the weights are read once
+ * for every 32 tokens, so it pays for few. */
 typedef struct FoMatvecW4Desc {
   int64_t T, N, K;
   const void* x;
-  FoW4 w, w_up;
+  FoW4 w;
   const void* bias; /* [N] of dtype or NULL                                                */
   void* out;
   int64_t ldx, ldo;
   int32_t dtype; /* FO_DT_F16 or FO_DT_BF16: x, scales, bias and out                       */
-  int32_t act;   /* FO_GATE_*                                                              */
 } FoMatvecW4Desc;
 
 int fo_matvec_w4(const FoMatvecW4Desc* desc, void* stream);
+
+/* out[T, N] = (act(x w_gate^T) * (x w_up^T)) w_down^T; w_gate, w_up [F, D] with one group
+ * size, w_down [N, F].  D and F multiples of 32.  The product between is kept in two 16-bit
+ * parts (its high and its low bits). */
+typedef struct FoGatedFfnW4Desc {
+  int64_t T, D, F, N;
+  const void* x;
+  FoW4 w_gate, w_up, w_down;
+  void* out;
+  int64_t ldx, ldo;
+  int32_t dtype;
+  int32_t act; /* FO_GATE_SILU .. FO_GATE_RELU                                             */
+  void* workspace; /* fo_gated_ffn_w4_workspace_size bytes, any content                    */
+  size_t workspace_bytes;
+} FoGatedFfnW4Desc;
+
+int fo_gated_ffn_w4(const FoGatedFfnW4Desc* desc, void* stream);
+size_t fo_gated_ffn_w4_workspace_size(const FoGatedFfnW4Desc* desc);
 
 /* Legality of a tile config for an op (0 = gemm family, 1 = conv2d) and output dtype:
  * shared memory <= 227 KB, TMEM columns <= 512, tcgen05 shape rules.  Returns FO_OK or
