@@ -1,5 +1,6 @@
 // fo_few.cuh -- the tcgen05 kernel for products whose token side is short: the weights are
-// the MMA's M side (128 features a tile), the tokens its N side (NT = 16 .. 256 of them).
+// the MMA's M side (128 features a tile), the tokens its N side (NT = 16, 32 or 64 columns,
+// all of them in one tile).
 //
 // With few tokens the time is that of the weights' bytes: an MMA costs by its token columns,
 // so nothing is spent on absent rows, and a SM keeps about 200 KB of weight tiles in flight
@@ -13,6 +14,9 @@
 //   FEW_GATED  two weight tiles a K block: h = act(g) * u (and g, u)
 //   FEW_PLAIN  one weight tile a K block, over one or two K segments
 //   FEW_DGATE  FEW_PLAIN's accumulator is dh: writes dg, du, h from the saved g, u
+// Between the forward pass's two products h travels as two 16-bit parts, high and low, in rows
+// 2 t and 2 t + 1: twice the token columns of an MMA that is not the bound, and h costs no
+// precision.
 #pragma once
 #include "fo_ffn.cuh"
 
@@ -31,12 +35,11 @@ struct FewShape {
   static constexpr int kCols = NT < 32 ? 32 : NT;               // TMEM columns of one product
   static constexpr int kTmem = kTiles * kCols;
   static constexpr int kExchange = kTiles * NT * 128 * 4;       // sums received from the cluster
-  // two CTAs a SM up to 32 tokens (128 for one weight tile), else one with a deep ring
-  static constexpr int kBudget = (MODE == FEW_GATED ? NT <= 32 : NT <= 128) ? 110 * 1024 : 200 * 1024;
+  static constexpr int kBudget = 110 * 1024;                    // two CTAs a SM
   static constexpr int kStages = kBudget / kStage < kFewMaxStages ? kBudget / kStage : kFewMaxStages;
   static constexpr int kRing = kStages * kStage > kExchange ? kStages * kStage : kExchange;
   static constexpr int kSmem = 1024 + kRing + 512;
-  static_assert(kStages >= 3, "a ring");
+  static_assert(kStages >= 2, "a ring");
 };
 
 struct FewMaps {
@@ -44,14 +47,14 @@ struct FewMaps {
 };
 
 struct FewParams {
-  int F, T;             // features, tokens
-  int tok_tiles;        // tile = feature tile * tok_tiles + token tile
+  int F, T;             // features, token columns (two a token where joint)
   int kb0, kb;          // K blocks of the first segment, of all
   int a_mn, bf16;
   void *out, *g, *u;    // FEW_GATED: h, g, u (or null); FEW_PLAIN: out; FEW_DGATE: dg, du, h
   long long ldo, ldg, ldu;
   const void *sg, *su;  // FEW_DGATE: the saved g, u
   long long ldsg, ldsu;
+  int split, joint;     // FEW_GATED: h is written in two parts; FEW_PLAIN: it comes so
   int early;            // the weights are final before the previous kernel ends
   int* status;
   unsigned long long timeout_ns;
@@ -90,8 +93,7 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
   int Q;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(Q));
   const int rank = static_cast<int>(cluster_ctarank());
-  const int tile = static_cast<int>(blockIdx.x) / Q;
-  const int f0 = tile / p.tok_tiles * 128, tok0 = tile % p.tok_tiles * NT;
+  const int f0 = static_cast<int>(blockIdx.x) / Q * 128;
   const int k0 = p.kb * rank / Q, k1 = p.kb * (rank + 1) / Q;  // this CTA's K blocks
 
   if (threadIdx.x == 0) {
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
           weights(kb, s);
         }
         const int seg = MODE != FEW_GATED && kb >= p.kb0;
-        tma_load_2d(ring + s * S::kStage + S::kW, &maps.b[seg], bar_full + 8 * s, (kb - (seg ? p.kb0 : 0)) * kBK, tok0);
+        tma_load_2d(ring + s * S::kStage + S::kW, &maps.b[seg], bar_full + 8 * s, (kb - (seg ? p.kb0 : 0)) * kBK, 0);
         ++issued;
         if (++s == S::kStages) {
           s = 0;
@@ -219,13 +221,16 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
   const int f = f0 + quarter * 32 + lane;
   auto finish = [&](int t, float v, float w) {
     if (f >= p.F || t >= p.T) return;
-    unsigned short* out = static_cast<unsigned short*>(p.out) + t * p.ldo + f;
+    unsigned short* out = static_cast<unsigned short*>(p.out) + (MODE == FEW_GATED && p.split ? 2 * t : MODE == FEW_PLAIN && p.joint ? t / 2 : t) * p.ldo + f;
     if constexpr (MODE == FEW_GATED) {
       if (p.g != nullptr) {
         static_cast<unsigned short*>(p.g)[t * p.ldg + f] = to16(v, p.bf16);
         static_cast<unsigned short*>(p.u)[t * p.ldu + f] = to16(w, p.bf16);
       }
-      *out = to16(both(gate_act<ACT>(two(v))).x * w, p.bf16);
+      const float h = both(gate_act<ACT>(two(v))).x * w;
+      const unsigned short hi = to16(h, p.bf16);
+      *out = hi;
+      if (p.split) out[p.ldo] = to16(h - from16(hi, p.bf16), p.bf16);
     } else if constexpr (MODE == FEW_DGATE) {
       const float sg = from16(__ldg(static_cast<const unsigned short*>(p.sg) + t * p.ldsg + f), p.bf16);
       const float su = from16(__ldg(static_cast<const unsigned short*>(p.su) + t * p.ldsu + f), p.bf16);
@@ -243,14 +248,19 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
     if (warp >= 2) {
       tc_fence_after();
 #pragma unroll 1
-      for (int c0 = 0; c0 < NT && tok0 + c0 < p.T; c0 += kChunk) {
+      for (int c0 = 0; c0 < NT && c0 < p.T; c0 += kChunk) {
         uint32_t r[32], s[32];
         tmem_ld_32x32b_x32(tb + c0, r);
         if constexpr (MODE == FEW_GATED) tmem_ld_32x32b_x32(tb + S::kCols + c0, s);
         tc_wait_ld_regs(r);
         if constexpr (MODE == FEW_GATED) tc_pin_regs(s);
+        if (MODE == FEW_PLAIN && p.joint) {
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) finish(tok0 + c0 + i, __uint_as_float(r[i]), MODE == FEW_GATED ? __uint_as_float(s[i]) : 0.f);
+          for (int i = 0; i < kChunk; i += 2) finish(c0 + i, __uint_as_float(r[i]) + __uint_as_float(r[i + 1]), 0.f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) finish(c0 + i, __uint_as_float(r[i]), MODE == FEW_GATED ? __uint_as_float(s[i]) : 0.f);
+        }
       }
     }
   } else {
@@ -276,16 +286,19 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
     }
     cluster_sync();  // every sum has arrived
     if (warp >= 2) {
-      for (int j = 0; j < own; ++j) {
-        const int t = tok0 + rank * own + j;
+      const int step = MODE == FEW_PLAIN && p.joint ? 2 : 1;  // (own is even: NT >= 16, Q <= 8)
+      for (int j = 0; j < own; j += step) {
+        const int t = rank * own + j;
         if (t >= p.T) break;
         float v = 0.f, w = 0.f;
         for (int q = 0; q < Q; ++q) {
           const float* src = reinterpret_cast<const float*>(smem) + (q * S::kTiles * own + j) * 128 + quarter * 32 + lane;
           v += src[0];
+          if (step == 2) w += src[128];
           if constexpr (MODE == FEW_GATED) w += src[own * 128];
         }
-        finish(t, v, w);
+        if (step == 2) finish(t, v + w, 0.f);
+        else finish(t, v, w);
       }
     }
   }
@@ -299,13 +312,12 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
   }
 }
 
-// The token columns of a tile and the CTAs that split its K blocks.
+// Token columns, feature tiles, and the CTAs that split a tile's K blocks.
 struct FewPlan {
-  int nt, tok_tiles, tiles, q;
+  int nt, tiles, q;
 };
 
-FewPlan few_plan(int mode, int64_t F, int64_t T, int kb, int sms);
-// p: everything but the plan's fields.
-cudaError_t launch_few(int mode, int act, const FewMaps& m, FewParams p, const FewPlan& plan, cudaStream_t stream);
+FewPlan few_plan(int mode, int64_t F, int64_t columns, int kb, int sms);  // columns <= 64
+cudaError_t launch_few(int mode, int act, const FewMaps& m, const FewParams& p, const FewPlan& plan, cudaStream_t stream);
 
 }  // namespace fo

@@ -1,5 +1,4 @@
 // fo_ffn.cu -- launches and C entries of the gated feed-forward block.
-#include <cstdlib>
 #include <cstring>
 
 #include "fo_few.cuh"
@@ -188,10 +187,9 @@ namespace fo {
 namespace {
 
 
-int few_most() {
-  static const int v = getenv("FO_FEW") ? atoi(getenv("FO_FEW")) : 32;
-  return v;
-}
+// Tokens up to which the short-token kernels run.  Forward, T = 32 and 48 at 1024 x 4096: 14 and
+// 23 us there, 25 and 25 us on CTA pairs; backward, T = 64 and 256: 52 and 89 against 85 and 55.
+constexpr int kFewForward = 32, kFewBackward = 64;
 
 constexpr int kSms = 148;
 
@@ -209,12 +207,14 @@ Few few_of(const FoGatedFfnDesc* d, bool backward) {
   f.matrices = (static_cast<size_t>(d->T) * pad8(d->F) * 2 * (backward ? 3 : 1) + 255) / 256 * 256;
   f.bytes = f.matrices;
   f.parts = 1;
-  f.on = d->T <= (backward ? few_most() * 2 : few_most());
+  f.on = d->T <= (backward ? kFewBackward : kFewForward);
   if (f.on) {
     f.first = backward ? few_plan(FEW_DGATE, d->F, d->T, static_cast<int>(kblocks(d->N)), kSms)
                        : few_plan(FEW_GATED, d->F, d->T, static_cast<int>(kblocks(d->D)), kSms);
     f.second = backward ? few_plan(FEW_PLAIN, d->D, d->T, static_cast<int>(2 * kblocks(d->F)), kSms)
-                        : few_plan(FEW_PLAIN, d->N, d->T, static_cast<int>(kblocks(d->F)), kSms);
+                        : few_plan(FEW_PLAIN, d->N, 2 * d->T, static_cast<int>(kblocks(d->F)), kSms);
+    if (!backward) f.matrices *= 2;  // h in two parts
+    f.bytes = f.matrices;
     return f;
   }
   if (backward) {
@@ -288,10 +288,12 @@ extern "C" int fo_gated_ffn(const FoGatedFfnDesc* d, void* stream) {
     FewBuild a(d, hd, d->F, d->D, 1), o(d, hd, d->N, d->F, 1);
     a.weight(0, wg, kn, "w_gate"), a.weight(1, wu, kn, "w_up");
     a.token(0, x, few.first.nt, "x");
-    a.p.out = d->workspace, a.p.ldo = h.ld;
+    const Mat h2{d->workspace, 2 * d->T, d->F, h.ld};
+    a.p.out = d->workspace, a.p.ldo = h.ld, a.p.split = 1;
     a.p.g = d->g, a.p.u = d->u, a.p.ldg = d->ldg, a.p.ldu = d->ldu;
     o.weight(0, wd, kn, "w_down");
-    o.token(0, h, few.second.nt, "h");
+    o.token(0, h2, few.second.nt, "h");
+    o.p.T *= 2, o.p.joint = 1;
     o.p.out = d->y, o.p.ldo = d->ldy;
     o.p.early = 1;
     if (a.rc || o.rc) return a.rc ? a.rc : o.rc;
