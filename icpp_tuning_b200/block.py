@@ -164,7 +164,14 @@ def _param(v: Optional[torch.Tensor], D: int, dt: torch.dtype, name: str) -> Opt
         return None
     if v.dtype is not dt:
         raise ValueError("the norms' parameters and the gate must share one dtype")
-    return _vec(v, D, name).data_ptr()
+    if v.shape != (D,) or not v.is_contiguous():
+        _vec(v, D, name)  # raises
+    return v.data_ptr()
+
+
+def _rows_like(y: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of y's shape."""
+    return torch.empty_like(y) if y.is_contiguous() else y.new_empty(y.shape)
 
 
 def _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps) -> N.FoBlockNormDesc:
@@ -178,8 +185,13 @@ def _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps)
     d.T, d.D, d.dtype, d.norm, d.vec_dtype = T, D, _sixteen_bit(y.dtype, "y"), NORMS[norm], dtype_code(dt)
     d.residual_scale, d.eps = residual_scale, eps
     d.y, d.ldy = y.data_ptr(), _ld(y, T, D, "y")
-    d.w_pre, d.w_post = _param(w_pre, D, dt, "w_pre"), _param(w_post, D, dt, "w_post")
-    d.b_pre, d.b_post = _param(b_pre, D, dt, "b_pre"), _param(b_post, D, dt, "b_post")
+    d.w_pre = _param(w_pre, D, dt, "w_pre")
+    if w_post is not None:
+        d.w_post = _param(w_post, D, dt, "w_post")
+    if b_pre is not None:
+        d.b_pre = _param(b_pre, D, dt, "b_pre")
+    if b_post is not None:
+        d.b_post = _param(b_post, D, dt, "b_post")
     if gate is not None:
         if gate.dim() == 1:
             d.gate, d.gate_rows, d.ldgate = _param(gate, D, dt, "gate"), 1, D
@@ -213,7 +225,7 @@ def block_norm(y: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tensor],
         raise ValueError("x and y must share one dtype")
     T, D = y.shape
     d.x, d.ldx = x.data_ptr(), _ld(x, T, D, "x")
-    r, z = y.new_empty((T, D)), y.new_empty((T, D))
+    r, z = _rows_like(y), _rows_like(y)
     d.r, d.z, d.ldr, d.ldz = r.data_ptr(), z.data_ptr(), D, D
     _run(dev, N.lib().fo_block_norm, ctypes.byref(d))
     return r, z
@@ -241,7 +253,7 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: torch.Tensor, y: torch.T
         d.dr, d.lddr = dr.data_ptr(), _ld(dr, T, D, "dr")
     d.dz, d.lddz = dz.data_ptr(), _ld(dz, T, D, "dz")
     d.r, d.ldr = r.data_ptr(), _ld(r, T, D, "r")
-    out = {"dy": y.new_empty((T, D)), "dx": y.new_empty((T, D))}
+    out = {"dy": _rows_like(y), "dx": _rows_like(y)}
     d.lddy = d.lddx = D
     # the parameters' gradients share one allocation, gate rows last
     names = [n for n, p in (("dw_pre", w_pre), ("dw_post", w_post), ("db_pre", b_pre), ("db_post", b_post)) if p is not None]
@@ -258,7 +270,7 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: torch.Tensor, y: torch.T
     lib = N.lib()
     ref = ctypes.byref(d)
     need = lib.fo_block_norm_backward_workspace_size(ref)
-    ws = torch.empty(max(16, need), dtype=torch.uint8, device=dev)
+    ws = y.new_empty((max(16, need) + 1) // 2)  # y's dtype has two bytes
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
     _run(dev, lib.fo_block_norm_backward, ref)
     return out

@@ -335,7 +335,6 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
   if (int rc = check(d)) return rc;
   if (d->D == 0 || d->F == 0 || d->N == 0) return host_fail(FO_EINVAL, "D, F and N must be positive");
   const bool kn = d->b_layout == FO_B_KN;
-  if (int rc = check_weights(d, kn)) return rc;
   if (int rc = check_mat(d->dw_gate, d->lddwg, kn ? d->F : d->D, "dw_gate")) return rc;
   if (int rc = check_mat(d->dw_up, d->lddwu, kn ? d->F : d->D, "dw_up")) return rc;
   if (int rc = check_mat(d->dw_down, d->lddwd, kn ? d->N : d->F, "dw_down")) return rc;
@@ -351,6 +350,7 @@ extern "C" int fo_gated_ffn_backward(const FoGatedFfnDesc* d, void* stream) {
       return host_fail(FO_ECUDA, "clearing a weight gradient failed");
     return host_ok();
   }
+  if (int rc = check_weights(d, kn)) return rc;
   if (int rc = check_mat(d->dy, d->lddy, d->N, "dy")) return rc;
   if (int rc = check_mat(d->g, d->ldg, d->F, "g")) return rc;
   if (int rc = check_mat(d->u, d->ldu, d->F, "u")) return rc;
