@@ -35,7 +35,7 @@ EXPORTED = (
     "fo_selftest_wait_timeout", "fo_last_error", "fo_version", "fo_launch_count",
     "fo_gemm_bias_layernorm_noalloc", "fo_conv2d_workspace_size",
     "fo_block_norm", "fo_block_norm_backward", "fo_block_norm_backward_workspace_size",
-    "fo_matvec_w4", "fo_gated_ffn_w4", "fo_gated_ffn_w4_workspace_size", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
+    "fo_matvec_w4", "fo_matvec_w4_workspace_size", "fo_gated_ffn_w4", "fo_gated_ffn_w4_workspace_size", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
 )
 
 
@@ -100,7 +100,8 @@ class FoW4(ctypes.Structure):
 class FoMatvecW4Desc(ctypes.Structure):
     _fields_ = [("T", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("x", ctypes.c_void_p),
                 ("w", FoW4), ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
-                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class FoGatedFfnW4Desc(ctypes.Structure):
@@ -142,6 +143,8 @@ def _declare(l: ctypes.CDLL) -> None:
         f.argtypes, f.restype = [P(FoGatedFfnDesc), ctypes.c_void_p], ctypes.c_int
     l.fo_gated_ffn_workspace_size.argtypes = [P(FoGatedFfnDesc), ctypes.c_int32]
     l.fo_gated_ffn_workspace_size.restype = ctypes.c_size_t
+    l.fo_matvec_w4_workspace_size.argtypes = [P(FoMatvecW4Desc)]
+    l.fo_matvec_w4_workspace_size.restype = ctypes.c_size_t
     l.fo_gated_ffn_w4.argtypes, l.fo_gated_ffn_w4.restype = [P(FoGatedFfnW4Desc), ctypes.c_void_p], ctypes.c_int
     l.fo_gated_ffn_w4_workspace_size.argtypes = [P(FoGatedFfnW4Desc)]
     l.fo_gated_ffn_w4_workspace_size.restype = ctypes.c_size_t

@@ -347,7 +347,13 @@ def matvec_w4(x: torch.Tensor, w: W4, *, bias: Optional[torch.Tensor] = None, st
         d.bias = _vec(bias, n, "bias").data_ptr()
     out = x.new_empty((T, n))
     d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
-    _run(dev, N.lib().fo_matvec_w4, ctypes.byref(d))
+    lib = N.lib()
+    ref = ctypes.byref(d)
+    need = lib.fo_matvec_w4_workspace_size(ref)
+    if need:
+        ws = x.new_empty((need + 1) // 2)  # x's dtype has two bytes
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _run(dev, lib.fo_matvec_w4, ref)
     return out
 
 
@@ -372,8 +378,11 @@ def gated_ffn_w4(x: torch.Tensor, w_gate: W4, w_up: W4, w_down: W4, *, act: str 
     d.w_down, n = _w4(w_down, F, dt, "w_down")
     d.T, d.D, d.F, d.N = T, D, F, n
     out = x.new_empty((T, n))
-    ws = x.new_empty((2 * T, (F + 7) // 8 * 8))
     d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
-    d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel() * 2
-    _run(dev, N.lib().fo_gated_ffn_w4, ctypes.byref(d))
+    lib = N.lib()
+    ref = ctypes.byref(d)
+    need = lib.fo_gated_ffn_w4_workspace_size(ref)
+    ws = x.new_empty((need + 1) // 2)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _run(dev, lib.fo_gated_ffn_w4, ref)
     return out

@@ -4,20 +4,36 @@
 // Bound by the weights' bytes, and close behind by issue: a SM has to open about 46 weights
 // a cycle to keep up with HBM.  So
 //   * a warp streams 32 rows (16 and their 16 partners of a gated pair) and its tokens' x in
-//     steps of 128 k, by 16-byte cp.async into a ring it keeps for itself, and asks for a step's scales one
-//     step ahead: no block-wide barrier in the loop, and no load whose latency the loop sees;
+//     steps of 128 k, by 16-byte cp.async into a ring it keeps for itself, and asks for a
+//     step's scales one step ahead: no block-wide barrier in the loop, and no load whose
+//     latency the loop sees;
 //   * one ldmatrix hands every lane the 32-bit words (8 weights each) of a 32-k group: of
-//     weight row lane / 4, word lane % 4 -- the fragment layout of mma.m16n8k16 when the k
+//     weight row lane / 4, word lane % 4 -- the fragment layout of the m16n8 MMAs when the k
 //     order inside a group is that of the words.  The order is free as long as both operands
-//     share it: a word's nibbles pair as (0,4), (1,5), (2,6), (3,7), x to match;
-//   * a pair is opened by a shift and one logic operation: in fp16 the bits of q alone are
-//     the subnormal q 2^-24, exact, and the scale takes 2^24 back; in bf16 the bits of 128 + q
-//     (its subnormals would leave fp32's range).  What stays of an offset, and the zero, leave
-//     by a product with sum(x) of the group, which one more MMA with a row of ones gives;
-//   * 16 weight rows x 8 tokens an MMA: up to 8 tokens cost what one costs.
-// W of a CTA's 8 warps share a tile of rows and split its K (and, for few tiles, the CTAs of
-// a cluster): as many as make about 2000 warps, so that each still walks many steps.  Partial
-// sums meet in shared memory (distributed across the cluster) and are added in a fixed order.
+//     share it.
+// A token or a few times large weights (fo_w4i_kernel): the MMA is m16n8k32 on 8-bit integers: a word opens into two
+// fragment registers by one shift and two masks, where 16-bit operands take three shifts and
+// four masks and half the k an MMA.  x becomes integers first (fo_w4_digits_kernel): each
+// token's 128 k's of a step as fixed point of 23 bits, relative to the power of two below
+// their largest magnitude, in three 8-bit digits, which are three columns of the MMA.  A
+// group's integer sum is exact, and so are 16-bit values within 2^11 of the step's largest; a
+// smaller one is off by 2^-22 of that power at most, no more than a fp32 sum loses.
+// All else (fo_w4_kernel) takes m16n8k16 on 16-bit floats: a word's nibbles pair as (0,4),
+// (1,5), (2,6), (3,7), x to match; in fp16 the bits of q alone are the subnormal q 2^-24,
+// exact, and the scale takes 2^24 back; in bf16 the bits of 128 + q (its subnormals would
+// leave fp32's range).
+// In both an offset of the opened weights, and their zero, leave by a product with sum(x) of
+// the group.  W of a CTA's 8 warps share a tile of rows and split its K (and, for few tiles,
+// the CTAs of a cluster): as many as fill the SMs with warps, so that each still walks many
+// steps.  Partial sums meet in shared memory (distributed across the cluster) and are added in
+// a fixed order.
+//
+// Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (101 MB of
+// weights) 37.5 us with its digits' kernels, 4.9 TB/s in the gated product (16-bit operands:
+// 51.9); 16384 x 4096 product 13.8 us (16.5); 8 tokens, block 51.3 us; 5 tokens, fp16, groups
+// of 32 with zeros, 57.7 us (113 MB).  The 16-bit form keeps the integer and logic pipe busy
+// 61% of the time, which bounds it; short products are bound by the launch and the start and
+// end of their few steps a warp (4096 x 4096, one token: 6.7 us for 8.7 MB).
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"
@@ -35,7 +51,7 @@ struct W4Params {
   long long ldq[2], lds[2], ldz[2];
   int per32;      // 32-k blocks a group
   uint32_t rcp;   // 2^32 / (steps a group), rounded up: GS 4, groups longer than a step
-  int vec;        // four scales (zeros) of a row are read at once
+  int vec;        // a step's scales (zeros) of a row are read at once
   int share;      // W: warps that share a tile
   const void* bias;
   int act;
@@ -45,6 +61,10 @@ struct W4Params {
   // low, in rows 2 t and 2 t + 1: written so (split), or read so and added (joint; T rows of
   // x, T / 2 of out).
   int split, joint;
+  // The digits of x, a record of every step; f32: the output is fp32 (the gated block's inner
+  // product).
+  const uint8_t* digits;
+  int f32;
 };
 
 template <int DT>
@@ -82,13 +102,12 @@ constexpr int kRows = 32;                  // weight rows of a tile: two 16-row 
 constexpr int kStepW = kRows * 64;         // their bytes in a step
 constexpr int kTable = kRows * 40;         // a step's (scale, -scale * offset) pairs, up to 4 a row
 
-// NT: 8-token MMA blocks; XT: tokens the ring has room for.
-template <int NT, int XT>
+// NT: 8-token MMA blocks.
+template <int NT>
 struct W4Shape {
-  static constexpr int kStep = kStepW + 256 * XT;
-  // three CTAs a SM for a token or two, two up to 16 tokens, else one
-  static constexpr int kCtas = XT == 2 ? 3 : NT <= 2 ? 2 : 1;
-  static constexpr int kBudget = (XT == 2 ? 73 : NT <= 2 ? 110 : 200) * 1024 / kWarps - kTable;
+  static constexpr int kStep = kStepW + 2048 * NT;
+  static constexpr int kCtas = NT <= 2 ? 2 : 1;    // a SM
+  static constexpr int kBudget = (NT <= 2 ? 110 : 200) * 1024 / kWarps - kTable;
   static constexpr int kStages = kBudget / kStep < 6 ? kBudget / kStep : 6;
   static constexpr int kRed = kRows * 8 * NT * 4;  // one warp's sums: its idle ring at the end
   static constexpr int kWarp = ((kStages * kStep > kRed ? kStages * kStep : kRed) + kTable + 127) / 128 * 128;  // bytes of a warp
@@ -97,9 +116,9 @@ struct W4Shape {
 };
 
 // GS: 32-k blocks whose sums share a scale in one step (1, 2 or 4; 1 serves any group size).
-template <bool GATED, int NT, int XT, int GS, int DT>
-__global__ void __launch_bounds__(256, (W4Shape<NT, XT>::kCtas)) fo_w4_kernel(const __grid_constant__ W4Params p) {
-  using S = W4Shape<NT, XT>;
+template <bool GATED, int NT, int GS, int DT>
+__global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __grid_constant__ W4Params p) {
+  using S = W4Shape<NT>;
   constexpr int ENT = 4 / GS, kOut = GATED ? 16 : 32;         // outputs of a tile
   constexpr float kLeft = DT == DT_BF16 ? 128.f : 0.f;        // offset that stays in the opened weights
   constexpr float kBack = DT == DT_BF16 ? 1.f : 16777216.f;   // what their scale lacks
@@ -147,7 +166,7 @@ __global__ void __launch_bounds__(256, (W4Shape<NT, XT>::kCtas)) fo_w4_kernel(co
 #pragma unroll
       for (int c = 0; c < 4; ++c) cp_async_16(put + w_at + c * 512, src[c] + wo, wn);
 #pragma unroll
-      for (int c = 0; c < XT / 2; ++c) {  // two tokens a copy, 16 blocks each
+      for (int c = 0; c < 4 * NT; ++c) {  // two tokens a copy, 16 blocks each
         if (c > 0 && 2 * c >= toks) break;
         if (2 * c + (lane >> 4) < toks) cp_async_16(put + x_at + c * 512, xs + 2 * c * p.ldx + xo, xn);
       }
@@ -170,6 +189,12 @@ __global__ void __launch_bounds__(256, (W4Shape<NT, XT>::kCtas)) fo_w4_kernel(co
       sraw[0] = static_cast<unsigned short>(v.x), sraw[1 % ENT] = static_cast<unsigned short>(v.x >> 16);
       sraw[2 % ENT] = static_cast<unsigned short>(v.y), sraw[3 % ENT] = static_cast<unsigned short>(v.y >> 16);
       if (zc != nullptr) zraw = __ldg(reinterpret_cast<const uint32_t*>(zc + s * 4));
+      return;
+    }
+    if (GS == 2 && p.vec && s * 2 + 2 <= groups) {
+      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(sc + s * 2));
+      sraw[0] = static_cast<unsigned short>(v), sraw[1 % ENT] = static_cast<unsigned short>(v >> 16);
+      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const unsigned short*>(zc + s * 2));
       return;
     }
     uint32_t z = 0;
@@ -306,37 +331,397 @@ __global__ void __launch_bounds__(256, (W4Shape<NT, XT>::kCtas)) fo_w4_kernel(co
   if (Q > 1) cluster_sync();  // the others may still read this CTA's sums
 }
 
+// ---------------------------------------------------------------------- up to 8 tokens
+constexpr int kPlanes = 3;
+
+// A step's record: 4 groups x 8 NT columns x 32 digits, then every column's sums over the
+// step's ENT blocks, then its scale.  Column 3 t + p is digit p of token t, the first the
+// highest; a group's digits are ordered like the fragments: for each word the k of its even
+// nibbles, then of its odd ones.  Sums are scaled already.
+template <int NT, int GS>
+struct W4iShape {
+  static constexpr int kEnt = 4 / GS;
+  static constexpr int kRec = 1024 * NT + (kEnt + 1) * 32 * NT;
+  static constexpr int kStep = kStepW + kRec;
+  static constexpr int kBudget = 113 * 1024 / kWarps - kTable;  // two CTAs a SM
+  static constexpr int kStages = kBudget / kStep < 6 ? kBudget / kStep : 6;
+  static constexpr int kRed = kRows * 8 * NT * 4;
+  static constexpr int kWarp = ((kStages * kStep > kRed ? kStages * kStep : kRed) + kTable) / 16 * 16;
+  static constexpr int kSmem = kWarps * kWarp + kRed;
+  static_assert(kStages >= 2 && kStep % 16 == 0, "a ring");
+};
+
+// x (16-bit or fp32) [T, K] into digit records: sixteen lanes a step of a token.  A step with
+// a value that is not finite gets the scale NaN.
+struct DigitParams {
+  const void* x;
+  long long ldx;
+  int T, K, steps, dt;
+  uint8_t* digits;
+};
+
+template <int NT, int GS>
+__global__ void __launch_bounds__(256) fo_w4_digits_kernel(const __grid_constant__ DigitParams p) {
+  using S = W4iShape<NT, GS>;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int unit = blockIdx.x * 16 + (threadIdx.x >> 4), l = threadIdx.x & 15;
+  const int tok = min(unit / p.steps, p.T - 1), step = unit % p.steps, k = step * 128 + l * 8;
+  float f[8] = {};
+  if (k < p.K) {
+    if (p.dt == DT_F32) {
+      const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + tok * p.ldx + k);
+      const float4 a = src[0], b = src[1];
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p.x) + tok * p.ldx + k);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = p.dt == DT_BF16 ? unpack2<DT_BF16>(w[i]) : unpack2<DT_F16>(w[i]);
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+      }
+    }
+  }
+  uint32_t most = 0;  // the largest magnitude's bits: infinities and NaN come out on top
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(fabsf(f[i])));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const bool fine = most < 0x7F800000u;
+  // Units of 2^(e - 21): |v| <= 2^22, which leaves the high digit room for a carry.  A power of
+  // two, so that a 16-bit value within 2^11 of the largest is exact.  (Its inverse by two
+  // factors: one would leave the range for small values.)
+  const int e = max(static_cast<int>(most >> 23), 1) - 127, up = 21 - e, up1 = up / 2, up2 = up - up1;
+  const float s1 = __int_as_float((up1 + 127) << 23), s2 = __int_as_float((up2 + 127) << 23);
+  int d[kPlanes][8], sum[kPlanes] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int v = fine ? __float2int_rn(f[i] * s1 * s2) : 0;
+    d[2][i] = static_cast<int8_t>(v);
+    const int v1 = (v - d[2][i]) >> 8;
+    d[1][i] = static_cast<int8_t>(v1);
+    d[0][i] = (v1 - d[1][i]) >> 8;
+#pragma unroll
+    for (int q = 0; q < kPlanes; ++q) sum[q] += d[q][i];
+  }
+#pragma unroll
+  for (int q = 0; q < kPlanes; ++q)
+#pragma unroll
+    for (int o = 1; o < 4 * GS; o <<= 1) sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], o);  // a block's 4 GS words
+  if (unit >= p.T * p.steps) return;
+  uint8_t* rec = p.digits + static_cast<long long>(step) * S::kRec;
+#pragma unroll
+  for (int q = 0; q < kPlanes; ++q) {
+    uint2 w = make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w.x |= (d[q][2 * i] & 255u) << (8 * i);
+      w.y |= (d[q][2 * i + 1] & 255u) << (8 * i);
+    }
+    const int col = tok * kPlanes + q;
+    *reinterpret_cast<uint2*>(rec + (l >> 2) * (256 * NT) + col * 32 + (l & 3) * 8) = w;
+    float* tail = reinterpret_cast<float*>(rec + 1024 * NT) + col;
+    // the digit's unit; it may be subnormal, and its integers still scale exactly
+    const float unit_q = fine ? ldexpf(1.f, 8 * (kPlanes - 1 - q) - up) : __int_as_float(0x7FC00000);
+    if ((l & (4 * GS - 1)) == 0) tail[l / (4 * GS) * (8 * NT)] = static_cast<float>(sum[q]) * unit_q;
+    if (l == 0) tail[S::kEnt * 8 * NT] = unit_q;
+  }
+}
+
+__device__ __forceinline__ void imma_16832(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int* c) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+template <bool GATED, int NT, int GS, int DT>
+__global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ W4Params p) {
+  using S = W4iShape<NT, GS>;
+  constexpr int ENT = S::kEnt, kOut = GATED ? 16 : 32;
+  extern __shared__ __align__(128) uint8_t smem_w4[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  int rank, Q;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(Q));
+  const int W = p.share, per_cta = kWarps / W;
+  const int tile0 = static_cast<int>(blockIdx.x / Q) * per_cta;
+  const int n0 = (tile0 + warp / W) * kOut;
+  const int cols = kPlanes * p.T;
+  const int steps = (p.K + 127) / 128;
+  const int first = rank * W + warp % W, stride = Q * W;  // this warp's steps
+  const int mine = n0 < p.N && first < steps ? (steps - first + stride - 1) / stride : 0;
+  uint8_t* const own = smem_w4 + warp * S::kWarp;
+  const uint32_t ring = smem_u32(own);
+  uint8_t* const table = own + S::kWarp - kTable;
+
+  const char* src[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int m = GATED ? c >> 1 : 0, n = n0 + r + 8 * (GATED ? c & 1 : c);
+    src[c] = static_cast<const char*>(p.q[m]) + min(n, p.N - 1) * p.ldq[m] + t * 16;
+  }
+  const uint32_t w_at = (r * 4 + (t ^ ((r >> 1) & 3))) * 16;
+  int todo = 0, xtodo = 0;
+  auto weights = [&](int i) {  // step i's weights
+    if (i < mine) {
+      const int s = first + i * stride;
+      const uint32_t put = ring + i % S::kStages * S::kStep, wn = s * 128 + t * 32 < p.K ? 16u : 0u;
+      const int wo = wn ? s * 64 : 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) cp_async_16(put + w_at + c * 512, src[c] + wo, wn);
+    }
+  };
+  auto digits = [&](int i) {  // and its digits (used columns only) and their sums
+    if (i < mine) {
+      const uint32_t put = ring + i % S::kStages * S::kStep + kStepW;
+      const uint8_t* rec = p.digits + static_cast<long long>(first + i * stride) * S::kRec;
+#pragma unroll
+      for (int c = 0; c < 2 * NT; ++c) {
+        const int at = c * 32 + lane;  // 16-byte block: group, column, half
+        if (at / 2 % (8 * NT) < cols) cp_async_16(put + at * 16, rec + at * 16, 16u);
+      }
+      if (lane < (ENT + 1) * 2 * NT) cp_async_16(put + 1024 * NT + lane * 16, rec + 1024 * NT + lane * 16, 16u);
+    }
+    cp_async_commit();
+  };
+  const int tm = GATED ? lane >> 4 : 0, tn = min(n0 + (GATED ? lane & 15 : lane), p.N - 1);
+  const unsigned short* sc = static_cast<const unsigned short*>(p.scale[tm]) + tn * p.lds[tm];
+  const unsigned char* zc = p.zero[tm] == nullptr ? nullptr : p.zero[tm] + tn * p.ldz[tm];
+  const int groups = (p.K + p.per32 * 32 - 1) / (p.per32 * 32);
+  unsigned short sraw[ENT];
+  uint32_t zraw = 0x08080808u;
+  auto ask = [&](int s) {
+    if (GS == 1 && p.vec && s * 4 + 4 <= groups) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(sc + s * 4));
+      sraw[0] = static_cast<unsigned short>(v.x), sraw[1 % ENT] = static_cast<unsigned short>(v.x >> 16);
+      sraw[2 % ENT] = static_cast<unsigned short>(v.y), sraw[3 % ENT] = static_cast<unsigned short>(v.y >> 16);
+      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const uint32_t*>(zc + s * 4));
+      return;
+    }
+    if (GS == 2 && p.vec && s * 2 + 2 <= groups) {
+      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(sc + s * 2));
+      sraw[0] = static_cast<unsigned short>(v), sraw[1 % ENT] = static_cast<unsigned short>(v >> 16);
+      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const unsigned short*>(zc + s * 2));
+      return;
+    }
+    uint32_t z = 0;
+#pragma unroll
+    for (int e = 0; e < ENT; ++e) {
+      const int at = GS == 4 ? (p.rcp != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(s), p.rcp)) : s)
+                     : GS == 2 ? s * 2 + e : (s * 4 + e) / p.per32;
+      const int g = min(at, groups - 1);  // past K: unused
+      sraw[e] = __ldg(sc + g);
+      z |= (zc != nullptr ? static_cast<uint32_t>(__ldg(zc + g)) : 8u) << (8 * e);
+    }
+    zraw = z;
+  };
+
+  // The weights and scales are final before the digits' kernel ends (it began after whatever
+  // wrote them), the digits are not.
+  if (mine > 0) ask(first);
+#pragma unroll
+  for (; todo < S::kStages - 1; ++todo) weights(todo);
+  for (int i = lane; i < S::kStages * (S::kRec / 16); i += 32) {  // columns without a digit stay zero
+    const int st = i / (S::kRec / 16), b = i - st * (S::kRec / 16);
+    if (b < 64 * NT && b / 2 % (8 * NT) >= cols) *reinterpret_cast<uint4*>(own + st * S::kStep + kStepW + b * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+#pragma unroll
+  for (; xtodo < S::kStages - 1; ++xtodo) digits(xtodo);
+
+  float acc[2][NT][4] = {};
+  const int none[4] = {0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000};  // 1.5 * 2^23: an integer added to its bits
+  const Two none2 = two(-12582912.f);                                    // is added to its value
+  const uint32_t my_row = (lane >> 3) * 512u + (lane & 7) * 64u, my_rot = ((lane & 7) >> 1) & 3;
+  const uint32_t my_x = kStepW + lane * 8u;
+  int slot = 0;
+  for (int i = 0; i < mine; ++i) {
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();  // other lanes' copies, and their reads of the slot and the table refilled next
+#pragma unroll
+    for (int e = 0; e < ENT; ++e) {
+      const float v = unpack2<DT>(sraw[e]).x, z = static_cast<float>((zraw >> (8 * e)) & 255u);
+      *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v, -v * z);
+    }
+    __syncwarp();
+    weights(i + S::kStages - 1);
+    digits(i + S::kStages - 1);
+    if (i + 1 < mine) ask(first + (i + 1) * stride);
+    const uint32_t stage = ring + slot * S::kStep;
+    const uint8_t* stage_p = own + slot * S::kStep;
+    int dot[2][NT][4];
+    Two unit[NT];  // of this lane's two columns
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 v = *reinterpret_cast<const float2*>(stage_p + kStepW + 1024 * NT + ENT * (32 * NT) + (nt * 8 + 2 * t) * 4);
+      unit[nt] = two(v.x, v.y);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t b[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(b[nt][0]), "=r"(b[nt][1]) : "r"(stage + my_x + j * (256 * NT) + nt * 256) : "memory");
+      uint32_t w[4];
+      ldsm4(stage + my_row + ((j ^ my_rot) << 4), w);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        uint32_t a[4];  // rows r, r + 8 of the even nibbles, then of the odd ones
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          a[h] = w[2 * m + h] & 0x0F0F0F0Fu;
+          a[2 + h] = (w[2 * m + h] >> 4) & 0x0F0F0F0Fu;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) imma_16832(dot[m][nt], a, b[nt][0], b[nt][1], j % GS == 0 ? none : dot[m][nt]);
+      }
+      if ((j + 1) % GS == 0) {
+        Two sx[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 v = *reinterpret_cast<const float2*>(stage_p + kStepW + 1024 * NT + j / GS * (32 * NT) + (nt * 8 + 2 * t) * 4);
+          sx[nt] = two(v.x, v.y);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const float2 lo = *reinterpret_cast<const float2*>(table + (m * 16 + r) * 40 + j / GS * 8);
+          const float2 hi = *reinterpret_cast<const float2*>(table + (m * 16 + r + 8) * 40 + j / GS * 8);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const Two d01 = add2(two(__int_as_float(dot[m][nt][0]), __int_as_float(dot[m][nt][1])), none2);
+            const Two d23 = add2(two(__int_as_float(dot[m][nt][2]), __int_as_float(dot[m][nt][3])), none2);
+            const float2 u = both(fma2(sx[nt], two(lo.y), fma2(d01, mul2(two(lo.x), unit[nt]), two(acc[m][nt][0], acc[m][nt][1]))));
+            const float2 v = both(fma2(sx[nt], two(hi.y), fma2(d23, mul2(two(hi.x), unit[nt]), two(acc[m][nt][2], acc[m][nt][3]))));
+            acc[m][nt][0] = u.x, acc[m][nt][1] = u.y, acc[m][nt][2] = v.x, acc[m][nt][3] = v.y;
+          }
+        }
+      }
+    }
+    if (++slot == S::kStages) slot = 0;
+  }
+
+  constexpr int TW = 8 * NT;
+  cp_async_wait_all();
+  __syncwarp();  // the warp is done with its ring
+  float* red = reinterpret_cast<float*>(own);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[(m * 16 + (e >> 1) * 8 + r) * TW + nt * 8 + 2 * t + (e & 1)] = acc[m][nt][e];
+  __syncthreads();
+  auto of_tile = [&](int j, int i) {
+    float v = 0.f;
+    for (int w = 0; w < W; ++w) v += reinterpret_cast<const float*>(smem_w4 + (j * W + w) * S::kWarp)[i];
+    return v;
+  };
+  float* part = reinterpret_cast<float*>(smem_w4 + kWarps * S::kWarp);
+  if (Q > 1) {
+    for (int i = threadIdx.x; i < kRows * TW; i += 256) part[i] = of_tile(0, i);
+    cluster_sync();
+  }
+  const uint32_t pa = smem_u32(part);
+  auto total = [&](int j, int row, int tok) {  // a token's digits joined, lowest first
+    float v = 0.f;
+#pragma unroll
+    for (int q = kPlanes - 1; q >= 0; --q) {
+      const int i = row * TW + tok * kPlanes + q;
+      float d = 0.f;
+      if (Q == 1) d = of_tile(j, i);
+      else
+        for (int c = 0; c < Q; ++c) d += ld_cluster_f32(mapa_shared(pa + i * 4, c));
+      v += d;
+    }
+    return v;
+  };
+  for (int o = rank * 256 + threadIdx.x; o < per_cta * kOut * p.T; o += 256 * Q) {
+    const int j = o / (kOut * p.T), oo = o - j * (kOut * p.T);
+    const int tok = oo / kOut, f = oo % kOut, n = (tile0 + j) * kOut + f;
+    if (n >= p.N) continue;
+    float v = total(j, f, tok);
+    if constexpr (GATED) v = both(gate_act(p.act, two(v))).x * total(j, 16 + f, tok);
+    else if (p.bias != nullptr) v += load_vec(p.bias, DT, n);
+    if (p.f32) static_cast<float*>(p.out)[tok * p.ldo + n] = v;
+    else static_cast<unsigned short*>(p.out)[tok * p.ldo + n] = static_cast<unsigned short>(pack2<DT>(v, 0.f));
+  }
+  if (Q > 1) cluster_sync();  // the others may still read this CTA's sums
+}
+
 // ---------------------------------------------------------------------- host
-template <bool GATED, int NT, int XT, int GS, int DT>
-cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
-  static std::atomic<uint64_t> opted{0};
-  constexpr int kOut = GATED ? 16 : 32;
-  const long long tiles = (p.N + kOut - 1) / kOut;
-  const int chunks = (p.T + 8 * NT - 1) / (8 * NT), steps = (p.K + 127) / 128;
-  // About as many warps as fit at once; a warp keeps a step or more.
-  const long long fit = 7ll * W4Shape<NT, XT>::kCtas * sms;
+// Tiles, warps a tile and CTAs a tile: about as many warps as fit at once, each with a step or
+// more.
+struct W4Plan {
+  int share, q;
+  unsigned ctas;
+};
+
+W4Plan w4_plan(int N, int K, int out, int chunks, int ctas_a_sm, int sms) {
+  const long long tiles = (N + out - 1) / out, fit = 7ll * ctas_a_sm * sms;
+  const int steps = (K + 127) / 128;
   int W = 1, Q = 1;
   while (W < kWarps && tiles * chunks * W < fit && steps >= 2 * W) W *= 2;
   while (W == kWarps && Q < 8 && tiles * chunks * Q * W < 8ll * sms && steps >= kWarps * Q * 2) Q *= 2;
-  p.share = W;
-  const long long ctas = (tiles + kWarps / W - 1) / (kWarps / W) * Q;
-  return launch_pdl(fo_w4_kernel<GATED, NT, XT, GS, DT>, opted, dim3(static_cast<unsigned>(ctas), chunks), dim3(256), W4Shape<NT, XT>::kSmem,
-                    Q, stream, p);
+  return {W, Q, static_cast<unsigned>((tiles + kWarps / W - 1) / (kWarps / W) * Q)};
+}
+
+template <bool GATED, int NT, int GS, int DT>
+cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> opted{0};
+  const int chunks = (p.T + 8 * NT - 1) / (8 * NT);
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, sms);
+  p.share = l.share;
+  return launch_pdl(fo_w4_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas, chunks), dim3(256), W4Shape<NT>::kSmem, l.q, stream, p);
+}
+
+int digit_blocks(int64_t T) { return static_cast<int>(kPlanes * T + 7) / 8; }
+// Whether x travels as digits: two MMA columns' blocks cost a group of 128 little (4096 x 16384
+// gated block, 4 tokens: 45.0 -> 40.3 us), shorter groups too much.  Up to 2^24 weights the
+// second launch costs the caller more (3 us) than the GPU saves (4096 x 4096: 7.7 -> 7.0 us;
+// 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
+bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
+  return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 2 : 1);
+}
+// Bytes of the digit records.
+size_t digit_bytes(int64_t T, int64_t K, int per32) {
+  const int ent = per32 % 4 == 0 ? 1 : per32 == 2 ? 2 : 4;
+  return static_cast<size_t>((K + 127) / 128) * digit_blocks(T) * (1024 + (ent + 1) * 32);
+}
+
+// x_dt: of p.x.  `room` holds digit_bytes.
+template <bool GATED, int NT, int GS, int DT>
+cudaError_t launch_digits(W4Params p, int x_dt, void* room, int sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> opted{0}, none{0};
+  DigitParams d = {};
+  d.x = p.x, d.ldx = p.ldx, d.T = p.T, d.K = p.K, d.steps = (p.K + 127) / 128, d.dt = x_dt;
+  d.digits = static_cast<uint8_t*>(room);
+  const unsigned blocks = static_cast<unsigned>((d.T * d.steps + 15) / 16);
+  cudaError_t e = launch_pdl(fo_w4_digits_kernel<NT, GS>, none, dim3(blocks), dim3(256), 0, 1, stream, d);
+  if (e != cudaSuccess) return e;
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, 1, 2, sms);
+  p.share = l.share, p.digits = d.digits;
+  return launch_pdl(fo_w4i_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas), dim3(256), W4iShape<NT, GS>::kSmem, l.q, stream, p);
 }
 
 template <bool GATED, int GS, int DT>
-cudaError_t by_tokens(const W4Params& p, int sms, cudaStream_t s) {
-  if (p.T <= 2) return launch<GATED, 1, 2, GS, DT>(p, sms, s);
-  if (p.T <= 8) return launch<GATED, 1, 8, GS, DT>(p, sms, s);
-  if (p.T <= 16) return launch<GATED, 2, 16, GS, DT>(p, sms, s);
-  return launch<GATED, 4, 32, GS, DT>(p, sms, s);
+cudaError_t by_tokens(const W4Params& p, int x_dt, void* room, int sms, cudaStream_t s) {
+  if (room != nullptr) {
+    if (GS == 4 && digit_blocks(p.T) == 2) return launch_digits<GATED, GS == 4 ? 2 : 1, GS, DT>(p, x_dt, room, sms, s);
+    return launch_digits<GATED, 1, GS, DT>(p, x_dt, room, sms, s);
+  }
+  if (p.T <= 8) return launch<GATED, 1, GS, DT>(p, sms, s);
+  if (p.T <= 16) return launch<GATED, 2, GS, DT>(p, sms, s);
+  return launch<GATED, 4, GS, DT>(p, sms, s);
 }
 
 template <bool GATED, int DT>
-cudaError_t by_group(const W4Params& p, int sms, cudaStream_t s) {
-  if (p.per32 % 4 == 0) return by_tokens<GATED, 4, DT>(p, sms, s);
-  if (p.per32 == 2) return by_tokens<GATED, 2, DT>(p, sms, s);
-  return by_tokens<GATED, 1, DT>(p, sms, s);
+cudaError_t by_group(const W4Params& p, int x_dt, void* room, int sms, cudaStream_t s) {
+  if (p.per32 % 4 == 0) return by_tokens<GATED, 4, DT>(p, x_dt, room, sms, s);
+  if (p.per32 == 2) return by_tokens<GATED, 2, DT>(p, x_dt, room, sms, s);
+  return by_tokens<GATED, 1, DT>(p, x_dt, room, sms, s);
 }
 
 int check_weight(const FoW4* w, int64_t K, const char* name) {
@@ -387,23 +772,29 @@ int act_code(int act) {
   }
 }
 
-int run(W4Params p, bool gated, int dtype, const HostDevice& hd, cudaStream_t st) {
+// room: for the digits of x, of type x_dt; null: x as it is.
+int run(W4Params p, bool gated, int dtype, int x_dt, void* room, const HostDevice& hd, cudaStream_t st) {
   const uint32_t per = static_cast<uint32_t>(p.per32) / 4;  // steps a group
   p.rcp = per > 1 ? static_cast<uint32_t>((0x100000000ull + per - 1) / per) : 0u;
-  p.vec = p.per32 == 1;
+  p.vec = p.per32 <= 2;
   for (int m = 0; m < (gated ? 2 : 1); ++m)
     p.vec = p.vec && p.lds[m] % 4 == 0 && reinterpret_cast<uintptr_t>(p.scale[m]) % 8 == 0 &&
             (p.zero[m] == nullptr || (p.ldz[m] % 4 == 0 && reinterpret_cast<uintptr_t>(p.zero[m]) % 4 == 0));
   const bool bf = dtype == FO_DT_BF16;
-  const cudaError_t e = gated ? (bf ? by_group<true, DT_BF16>(p, hd.sms, st) : by_group<true, DT_F16>(p, hd.sms, st))
-                              : (bf ? by_group<false, DT_BF16>(p, hd.sms, st) : by_group<false, DT_F16>(p, hd.sms, st));
+  const cudaError_t e = gated ? (bf ? by_group<true, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<true, DT_F16>(p, x_dt, room, hd.sms, st))
+                              : (bf ? by_group<false, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<false, DT_F16>(p, x_dt, room, hd.sms, st));
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
-  host_count_launches(1);
+  host_count_launches(room != nullptr ? 2 : 1);
   return FO_OK;
 }
 
 }  // namespace
 }  // namespace fo
+
+extern "C" size_t fo_matvec_w4_workspace_size(const FoMatvecW4Desc* d) {
+  if (d == nullptr || d->K <= 0 || d->w.group < 32) return 0;
+  return fo::as_digits(d->T, d->N, d->K, d->w.group / 32) ? fo::digit_bytes(d->T, d->K, d->w.group / 32) : 0;
+}
 
 extern "C" int fo_matvec_w4(const FoMatvecW4Desc* d, void* stream) {
   using namespace fo;
@@ -414,6 +805,9 @@ extern "C" int fo_matvec_w4(const FoMatvecW4Desc* d, void* stream) {
   if (int rc = check_weight(&d->w, d->K, "w")) return rc;
   if (int rc = check_x(d->x, d->ldx, d->T, d->K)) return rc;
   if (d->out == nullptr || d->ldo < d->N) return host_fail(FO_EINVAL, "out must be a device pointer with rows of N values or more");
+  const size_t need = fo_matvec_w4_workspace_size(d);
+  if (need > 0 && (d->workspace == nullptr || d->workspace_bytes < need || !host_aligned16(d->workspace)))
+    return host_fail(FO_EINVAL, "needs a 16-byte aligned workspace of %zu bytes", need);
   HostDevice hd;
   if (int rc = host_device(&hd)) return rc;
   W4Params p = {};
@@ -421,13 +815,36 @@ extern "C" int fo_matvec_w4(const FoMatvecW4Desc* d, void* stream) {
   set_weight(&p, 0, &d->w);
   p.per32 = d->w.group / 32;
   p.bias = d->bias, p.out = d->out, p.ldo = d->ldo;
-  if (int rc = run(p, false, d->dtype, hd, static_cast<cudaStream_t>(stream))) return rc;
+  if (int rc = run(p, false, d->dtype, d->dtype == FO_DT_BF16 ? DT_BF16 : DT_F16, need > 0 ? d->workspace : nullptr, hd,
+                   static_cast<cudaStream_t>(stream)))
+    return rc;
   return host_ok();
 }
 
+namespace fo {
+namespace {
+
+// The gated block's workspace: the product between, in fp32 to become digits, else in two
+// 16-bit parts (either way 4 bytes a value); then the digits, x's and later the product's.
+struct GatedW4Plan {
+  bool digits;  // of x and of the product between
+  size_t h, room;
+  explicit GatedW4Plan(const FoGatedFfnW4Desc* d) {
+    const int g1 = d->w_gate.group / 32, g2 = d->w_down.group / 32;
+    digits = as_digits(d->T, 2 * d->F, d->D, g1) && as_digits(d->T, d->N, d->F, g2);
+    h = (static_cast<size_t>(d->T) * ((d->F + 7) / 8 * 8) * 4 + 255) / 256 * 256;
+    const size_t a = digit_bytes(d->T, d->D, g1), b = digit_bytes(d->T, d->F, g2);
+    room = digits ? (a > b ? a : b) : 0;
+  }
+};
+
+}  // namespace
+}  // namespace fo
+
 extern "C" size_t fo_gated_ffn_w4_workspace_size(const FoGatedFfnW4Desc* d) {
-  if (d == nullptr || d->T <= 0 || d->F <= 0) return 0;
-  return static_cast<size_t>(d->T) * 2 * ((d->F + 7) / 8 * 8) * 2;
+  if (d == nullptr || d->T <= 0 || d->D <= 0 || d->F <= 0 || d->w_gate.group < 32 || d->w_down.group < 32) return 0;
+  const fo::GatedW4Plan plan(d);
+  return plan.h + plan.room;
 }
 
 extern "C" int fo_gated_ffn_w4(const FoGatedFfnW4Desc* d, void* stream) {
@@ -456,15 +873,18 @@ extern "C" int fo_gated_ffn_w4(const FoGatedFfnW4Desc* d, void* stream) {
   p.per32 = d->w_gate.group / 32;
   p.act = act_code(d->act);
   p.out = d->workspace, p.ldo = (d->F + 7) / 8 * 8;
-  p.split = 1;
+  const int dt = d->dtype == FO_DT_BF16 ? DT_BF16 : DT_F16;
+  const GatedW4Plan plan(d);
+  char* const room = static_cast<char*>(d->workspace) + plan.h;
+  p.f32 = plan.digits, p.split = !plan.digits;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = run(p, true, d->dtype, hd, st)) return rc;
+  if (int rc = run(p, true, d->dtype, dt, plan.digits ? room : nullptr, hd, st)) return rc;
   W4Params o = {};
-  o.x = d->workspace, o.ldx = p.ldo, o.T = 2 * p.T, o.N = static_cast<int>(d->N), o.K = p.N;
+  o.x = d->workspace, o.ldx = p.ldo, o.T = plan.digits ? p.T : 2 * p.T, o.N = static_cast<int>(d->N), o.K = p.N;
   set_weight(&o, 0, &d->w_down);
   o.per32 = d->w_down.group / 32;
   o.out = d->out, o.ldo = d->ldo;
-  o.joint = 1;
-  if (int rc = run(o, false, d->dtype, hd, st)) return rc;
+  o.joint = !plan.digits;
+  if (int rc = run(o, false, d->dtype, plan.digits ? DT_F32 : dt, plan.digits ? room : nullptr, hd, st)) return rc;
   return host_ok();
 }

@@ -278,7 +278,10 @@ typedef struct FoW4 {
 } FoW4;
 
 /* out[T, N] = x[T, K] w^T (+ bias).  K a multiple of 32.  Any T; the weights are read once
- * for every 32 tokens, so it pays for few. */
+ * for every 32 tokens, so it pays for few.  A few tokens times large weights (those for which
+ * a workspace is asked) take x as fixed point of 23 bits relative to the largest magnitude of
+ * its 128 k's, with exact integer sums inside a group; a value that is not finite then makes
+ * its token's outputs NaN. */
 typedef struct FoMatvecW4Desc {
   int64_t T, N, K;
   const void* x;
@@ -287,13 +290,16 @@ typedef struct FoMatvecW4Desc {
   void* out;
   int64_t ldx, ldo;
   int32_t dtype; /* FO_DT_F16 or FO_DT_BF16: x, scales, bias and out                       */
+  void* workspace; /* fo_matvec_w4_workspace_size bytes, any content; null when that is 0   */
+  size_t workspace_bytes;
 } FoMatvecW4Desc;
 
 int fo_matvec_w4(const FoMatvecW4Desc* desc, void* stream);
+size_t fo_matvec_w4_workspace_size(const FoMatvecW4Desc* desc);
 
 /* out[T, N] = (act(x w_gate^T) * (x w_up^T)) w_down^T; w_gate, w_up [F, D] with one group
- * size, w_down [N, F].  D and F multiples of 32.  The product between is kept in two 16-bit
- * parts (its high and its low bits). */
+ * size, w_down [N, F].  D and F multiples of 32.  The product between is kept in fp32, or in
+ * two 16-bit parts (its high and its low bits). */
 typedef struct FoGatedFfnW4Desc {
   int64_t T, D, F, N;
   const void* x;

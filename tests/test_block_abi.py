@@ -105,6 +105,13 @@ def test_matvec_w4_rejects(w, kw, msg):
     assert msg in N.last_error()
 
 
+def test_matvec_w4_workspace():
+    small, large = _matvec(), _matvec(_w4(ldq=2048, lds=128), N=8192, K=4096, ldx=4096, ldo=8192)
+    need = N.lib().fo_matvec_w4_workspace_size
+    assert need(ctypes.byref(small)) == 0 and need(ctypes.byref(large)) > 0 and need(None) == 0
+    assert N.lib().fo_matvec_w4(ctypes.byref(large), None) == N.FO_EINVAL and "workspace" in N.last_error()
+
+
 def test_gated_ffn_w4_rejects():
     d = N.FoGatedFfnW4Desc()
     d.T, d.D, d.F, d.N, d.x, d.out, d.ldx, d.ldo, d.dtype, d.act = 1, 64, 64, 16, A, A, 64, 16, N.FO_DT_F16, N.FO_GATE_SILU

@@ -89,6 +89,68 @@ def test_gated(T, D, F, Nn, group, act):
     status_clean()
 
 
+def step_most(x):
+    """The largest magnitude of each value's 128 k's, which its fixed point is relative to."""
+    T, K = x.shape
+    pad = torch.nn.functional.pad(x.abs(), (0, -K % 128)).reshape(T, -1, 128)
+    return pad.amax(2, keepdim=True).expand_as(pad).reshape(T, -1)[:, :K]
+
+
+# large weights times a few tokens: x as digits; K off the steps, N off the tiles, every group
+# size's path, the sums of a tile cut over warps and CTAs, values that span seven decades
+LARGE = [(1, 8200, 2048, 32), (2, 16001, 1056, 64), (3, 4100, 4128, 128), (5, 1401, 12800, 256), (1, 129, 131072, 384), (4, 1070, 16000, 4096),
+         (2, 540, 32032, 96), (1, 34000, 512, 128)]
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("T,Nn,K,group", LARGE)
+def test_matvec_of_large_weights(T, Nn, K, group, wide):
+    dtype = torch.bfloat16 if (T + wide) % 2 else torch.float16
+    w = weight(Nn, K, group, dtype, K % 3 == 0, seed=K + Nn, pad=T % 3)
+    x = torch.randn(T, K, generator=gen(T)).to(dtype)
+    if wide:
+        x = (x * 10 ** (torch.rand(T, K, generator=gen(T + 2)) * 7 - 5)).to(dtype)
+    bias = torch.randn(Nn, generator=gen(T + 1)).to(dtype) if Nn % 2 else None
+    v, size = opened(w)
+    X = x.double()
+    ref, mag = X @ v.t(), X.abs() @ size.t()
+    if bias is not None:
+        ref, mag = ref + bias.double(), mag + bias.double().abs()
+    wd, args = gpu(w), dict(bias=None if bias is None else bias.cuda())
+    out = block.matvec_w4(x.cuda(), wd, **args)
+    within(out, ref, U[dtype] * ref.abs() * 1.01 + ACC * mag + 2.0 ** -22 * step_most(X) @ v.abs().t())
+    assert torch.equal(out, block.matvec_w4(x.cuda(), wd, **args))
+    bad = x.repeat(2, 1)[:T + 1] if T == 1 else x.clone()
+    bad[0, K - 1], bad[0, 0] = float("inf"), 0
+    got = block.matvec_w4(bad.cuda(), wd, **args)
+    assert not got[0].isfinite().any() and torch.equal(got[1:], out[:1] if T == 1 else out[1:])
+    status_clean()
+
+
+@pytest.mark.parametrize("T,D,F,Nn,group,down", [(1, 2048, 4160, 4100, 64, 32), (2, 1056, 8192, 2101, 32, 32), (4, 1024, 8224, 2100, 128, 128),
+                                                 (5, 2080, 4128, 4100, 256, 128), (3, 2048, 4160, 4100, 128, 32)])
+def test_gated_of_large_weights(T, D, F, Nn, group, down):
+    dtype = torch.float16 if T % 2 else torch.bfloat16
+    wg, wu = (weight(F, D, group, dtype, T == 2, seed=i + F) for i in range(2))
+    wd = weight(Nn, F, down, dtype, T != 2, seed=9)
+    x = torch.randn(T, D, generator=gen(T)).to(dtype)
+    (vg, sg), (vu, su), (vd, sd) = map(opened, (wg, wu, wd))
+    X = x.double()
+    g, p, most = X @ vg.t(), X @ vu.t(), 2.0 ** -22 * step_most(X)
+    eg, ep = ACC * (X.abs() @ sg.t()) + most @ vg.abs().t(), ACC * (X.abs() @ su.t()) + most @ vu.abs().t()
+    a, _ = act64("silu", g)
+    h = a * p
+    eh = 1.2 * eg * p.abs() + (a.abs() + 1.2 * eg) * ep + ACC * (h.abs() + p.abs()) + 2 * U[dtype] ** 2 * h.abs() + 2.0 ** -24
+    eh = eh + 2.0 ** -22 * step_most(h.abs() + eh)
+    ref = h @ vd.t()
+    bound = U[dtype] * ref.abs() * 1.01 + eh @ vd.abs().t() + ACC * (h.abs() @ sd.t())
+    args = [x.cuda(), gpu(wg), gpu(wu), gpu(wd)]
+    out = block.gated_ffn_w4(*args)
+    within(out, ref, bound * 1.01)
+    assert torch.equal(out, block.gated_ffn_w4(*args))
+    status_clean()
+
+
 def test_every_nibble_is_exact():
     """x a unit vector, scale 1: the weights themselves, q - zero, in both types."""
     for dtype in (torch.float16, torch.bfloat16):
