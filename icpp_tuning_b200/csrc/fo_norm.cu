@@ -205,9 +205,10 @@ struct Rows {
   int slot = 0;
   uint32_t ph = 0;
   bool ok = true;
-  // VEC 1: the current row's span of each tensor, and whether the ring holds all of them
-  int shift[VEC == 8 ? 1 : NT];
-  bool whole = true;
+  // VEC 1: the current row's offset in each tensor's blocks, by bytes, 64 added (the thread
+  // that asks for a row leaves it beside the row); the top bit: not all in the ring
+  uint32_t* codes;
+  uint32_t code = 0;
 
   // Tensor k: forward y, x; backward r, dz, y, dr (null: not there, read as zero).  Addresses
   // stay in the kernel's parameters, not in registers.
@@ -237,8 +238,8 @@ struct Rows {
     return {from, to > from ? static_cast<uint32_t>(to - from) : 0u, shift};
   }
   // The ring starts as zeros: what no copy fills (columns past the row, absent tensors) stays so.
-  __device__ __forceinline__ void init(uint8_t* smem, uint64_t* mbars) {
-    ring = smem_u32(smem), bars = smem_u32(mbars);
+  __device__ __forceinline__ void init(uint8_t* smem, uint64_t* mbars, uint32_t* row_codes) {
+    ring = smem_u32(smem), bars = smem_u32(mbars), codes = row_codes;
     if (VEC == 8 && NP * 2 * 32 * W != c.D) {
       for (int i = c.tid * 16; i < S * NT * kRow; i += 32 * W * 16) *reinterpret_cast<uint4*>(smem + i) = make_uint4(0u, 0u, 0u, 0u);
     } else if (VEC == 8 && base(NT - 1) == nullptr) {
@@ -261,7 +262,18 @@ struct Rows {
 #pragma unroll
       for (int k = 0; k < NT; ++k)
         if (base(k) != nullptr) sp[k] = span(k, row), bytes += sp[k].bytes;
-      mbar_arrive_expect_tx(bars + 8 * at, bytes);
+      if constexpr (VEC == 1) {
+        uint32_t v = 0;
+        bool whole = true;
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          if (base(k) == nullptr) continue;
+          v |= static_cast<uint32_t>(sp[k].shift + 64) << (8 * k);
+          whole = whole && sp[k].shift >= 0 && static_cast<int>(sp[k].bytes / 2) - sp[k].shift >= c.D;
+        }
+        codes[at] = whole ? v : v | 0x80000000u;
+      }
+      mbar_arrive_expect_tx(bars + 8 * at, bytes);  // (releases the code with the row)
 #pragma unroll
       for (int k = 0; k < NT; ++k)
         if (base(k) != nullptr && (VEC == 8 || sp[k].bytes > 0))
@@ -269,18 +281,7 @@ struct Rows {
     }
   }
   // Waits for the current stage's rows (bounded; once it ran out, no further wait).
-  __device__ __forceinline__ void take(int row) {
-    if constexpr (VEC == 1) {
-      whole = true;
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        shift[k] = 0;
-        if (base(k) == nullptr) continue;
-        const Span sp = span(k, row);
-        shift[k] = sp.shift;
-        whole = whole && sp.shift >= 0 && static_cast<int>(sp.bytes / 2) - sp.shift >= c.D;
-      }
-    }
+  __device__ __forceinline__ void take() {
     if (ok && !mbar_wait(bars + 8 * slot, ph, p.timeout_ns, nullptr)) {
       ok = false;
       if (atomicCAS(p.status, 0, kStatusTimeout) == 0) {
@@ -290,7 +291,9 @@ struct Rows {
       for (int i = 0; i < S; ++i)  // let the copies in flight land before the CTA can end
         mbar_wait(bars + 8 * ((slot + i) % S), ph ^ (slot + i >= S ? 1u : 0u), kDrainTimeoutNs, nullptr);
     }
+    if constexpr (VEC == 1) code = ok ? codes[slot] : 0x40404040u;
   }
+  __device__ __forceinline__ int shift(int k) const { return static_cast<int>((code >> (8 * k)) & 127u) - 64; }
   __device__ __forceinline__ void next() {
     if (++slot == S) slot = 0, ph ^= 1;
   }
@@ -312,19 +315,19 @@ struct Rows {
         return;
       }
       unsigned short raw[8];
-      const uint32_t src = at + 2 * (c.tid + shift[k]);
-      if (whole) {
+      const uint32_t src = at + 2 * (c.tid + shift(k));
+      if ((code & 0x80000000u) == 0) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)  // in the ring's bounds for any column a thread holds
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[i]) : "r"(src + (2 * e0 + i) * 64 * W) : "memory");
       } else {  // the tensor's first or last row: its first or last block is read directly
-        const int hi = static_cast<int>(span(k, row).bytes / 2) - shift[k];
+        const int hi = static_cast<int>(span(k, row).bytes / 2) - shift(k);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int col = c.tid + (2 * e0 + i) * 32 * W;
           raw[i] = 0;
           if (col < c.D) {
-            if (col + shift[k] >= 0 && col < hi)
+            if (col + shift(k) >= 0 && col < hi)
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[i]) : "r"(src + (2 * e0 + i) * 64 * W) : "memory");
             else
               raw[i] = __ldg(base(k) + row * ld(k) + col);
@@ -359,7 +362,7 @@ __device__ __forceinline__ void walk(const NormParams& p, R& rows, Fn&& fn) {
       if (lo + i * RG < hi) rows.ask(i, lo + i * RG);
     fn.unit(grp);
     for (int row = lo; row < hi; row += RG) {
-      rows.take(row);
+      rows.take();
       fn.row(row, [&] {
         if (row + (S - 1) * RG < hi) rows.ask(S - 1, row + (S - 1) * RG);
       });
@@ -475,8 +478,9 @@ __global__ void __launch_bounds__(32 * W * row_groups(W)) fo_norm_fwd_kernel(con
   extern __shared__ __align__(128) uint8_t smem_norm[];
   __shared__ float red[RG * 2 * 16 * W];
   __shared__ __align__(8) uint64_t bars[RG * S];
+  __shared__ uint32_t codes[RG * S];
   Rows<DT, 2, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
-  in.init(smem_norm + threadIdx.y * S * 2 * in.kRow, bars + threadIdx.y * S);
+  in.init(smem_norm + threadIdx.y * S * 2 * in.kRow, bars + threadIdx.y * S, codes + threadIdx.y * S);
   FwdRow<DT, W, NP, VEC, LAYER, S> f{p, in, {red + threadIdx.y * 2 * 16 * W, 0, 1 + static_cast<int>(threadIdx.y)}, {}, {}, {}, {}};
   griddep_wait();
   griddep_launch_dependents();
@@ -643,8 +647,9 @@ __global__ void __launch_bounds__(32 * W * row_groups(W), W == 16 ? 1 : 2) fo_no
   extern __shared__ __align__(128) uint8_t smem_norm[];
   __shared__ float red[RG * 2 * 16 * W];
   __shared__ __align__(8) uint64_t bars[RG * S];
+  __shared__ uint32_t codes[RG * S];
   Rows<DT, 4, NP, VEC, W, S> in{p, {static_cast<int>(threadIdx.x), p.D}};
-  in.init(smem_norm + threadIdx.y * S * 4 * in.kRow, bars + threadIdx.y * S);
+  in.init(smem_norm + threadIdx.y * S * 4 * in.kRow, bars + threadIdx.y * S, codes + threadIdx.y * S);
   float* joint = reinterpret_cast<float*>(smem_norm + RG * S * 4 * in.kRow);
   BwdRow<DT, W, NP, VEC, LAYER> f{p, in, {red + threadIdx.y * 2 * 16 * W, 0, 1 + static_cast<int>(threadIdx.y)}, joint, {}, {}, {}};
   griddep_wait();
