@@ -10,7 +10,7 @@
 //   dw_pre = sum dz rhat, dw_post = sum dn yhat, db_* = sum dz, sum dn, dgate = sum t n
 // ([.] in the LayerNorm form only; sums over rows).
 //
-// W warps own a row, 16 columns a thread (8 where a thread carries four sums a column).
+// W warps own a row, 8 or 16 columns a thread; the CTAs walk the rows side by side.
 // Rows arrive by bulk copies in a ring of shared memory, several rows ahead, so the copies
 // never wait for a row's reductions.  A row that does not start or end on a 16-byte boundary
 // is copied as the 16-byte blocks around it, as far as they lie inside its tensor; what is
@@ -39,9 +39,9 @@ struct NormParams {
   int rows_per_gate;  // rows sharing one gate row (T for a gate vector)
   int vec_dtype, layer;
   float scale, eps;
-  // work units: chunks of chunk_rows rows inside one gate group; backward, the sums of unit
-  // u go to part[u][k][ldp] (k: dz rhat, t yhat, dz, t)
-  int groups, chunks, chunk_rows;
+  // work units: `chunks` to a gate group, its rows in turn; backward, the sums of unit u go to
+  // part[u][k][ldp] (k: dz rhat, t yhat, dz, t)
+  int groups, chunks;
   int ldp;
   float* part;
   int* status;
@@ -355,16 +355,16 @@ __device__ __forceinline__ void walk(const NormParams& p, R& rows, Fn&& fn) {
   constexpr int RG = row_groups(W);
   for (int u = blockIdx.x; u < p.groups * p.chunks; u += gridDim.x) {
     const int grp = u / p.chunks, chunk = u - grp * p.chunks;
-    const int lo = grp * p.rows_per_gate + chunk * p.chunk_rows + static_cast<int>(threadIdx.y);
-    const int hi = min((grp + 1) * p.rows_per_gate, grp * p.rows_per_gate + (chunk + 1) * p.chunk_rows);
+    const int lo = grp * p.rows_per_gate + chunk * RG + static_cast<int>(threadIdx.y);
+    const int hi = (grp + 1) * p.rows_per_gate, by = p.chunks * RG;
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
-      if (lo + i * RG < hi) rows.ask(i, lo + i * RG);
+      if (lo + i * by < hi) rows.ask(i, lo + i * by);
     fn.unit(grp);
-    for (int row = lo; row < hi; row += RG) {
+    for (int row = lo; row < hi; row += by) {
       rows.take();
       fn.row(row, [&] {
-        if (row + (S - 1) * RG < hi) rows.ask(S - 1, row + (S - 1) * RG);
+        if (row + (S - 1) * by < hi) rows.ask(S - 1, row + (S - 1) * by);
       });
       rows.next();
     }
@@ -472,8 +472,13 @@ struct FwdRow {
   __device__ __forceinline__ void done(int) {}
 };
 
+// CTAs a SM: 64 registers a thread where it holds 4 pairs (80 in the LayerNorm form), else 128.
+// 16384 x 4096 RMS: 92 us with 4 pairs and 32 warps a SM, 98 with 8 and 16; LayerNorm 153 and
+// 115, but 77 and 107 at the odd width 1001.
+constexpr int fwd_ctas(int W, int NP, bool layer) { return NP == 4 && !layer ? (W == 16 ? 2 : 4) : W == 16 ? 1 : NP == 4 ? 3 : 2; }
+
 template <int DT, int W, int NP, int VEC, bool LAYER, int S>
-__global__ void __launch_bounds__(32 * W * row_groups(W)) fo_norm_fwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(32 * W * row_groups(W), NP == 8 ? 0 : fwd_ctas(W, NP, LAYER)) fo_norm_fwd_kernel(const __grid_constant__ NormParams p) {
   constexpr int RG = row_groups(W);
   extern __shared__ __align__(128) uint8_t smem_norm[];
   __shared__ float red[RG * 2 * 16 * W];
@@ -743,25 +748,24 @@ using NormKernel = void (*)(const NormParams);
 
 struct Shape {
   NormKernel kern;
-  int warps, smem;
+  int warps, smem, ctas;
   std::atomic<uint64_t>* opted;
 };
 
 template <int DT, int W, int NP, int VEC, bool LAYER, int S = 4>
 Shape fwd_entry(int) {
   static std::atomic<uint64_t> opted{0};
-  return {fo_norm_fwd_kernel<DT, W, NP, VEC, LAYER, S>, W, row_groups(W) * S * 2 * ring_row<W, NP, VEC>(), &opted};
+  return {fo_norm_fwd_kernel<DT, W, NP, VEC, LAYER, S>, W, row_groups(W) * S * 2 * ring_row<W, NP, VEC>(), fwd_ctas(W, NP, LAYER), &opted};
 }
 
 template <int DT, int W, int NP, int VEC, bool LAYER>
 Shape bwd_entry(int D) {
   static std::atomic<uint64_t> opted{0};
   const int joint = row_groups(W) > 1 ? (LAYER ? 4 : 2) * ((D + 3) / 4 * 4) * 4 : 0;
-  return {fo_norm_bwd_kernel<DT, W, NP, VEC, LAYER>, W, row_groups(W) * kBwdStages * 4 * ring_row<W, NP, VEC>() + joint, &opted};
+  return {fo_norm_bwd_kernel<DT, W, NP, VEC, LAYER>, W, row_groups(W) * kBwdStages * 4 * ring_row<W, NP, VEC>() + joint, 2, &opted};
 }
 
-// The row layout for D columns: the fewest warps whose threads hold at most 8 pairs; 4 pairs
-// where a thread carries four sums a column (with 8 the LayerNorm form's backward pass spills).
+// The row layout for D columns: the fewest warps whose threads hold at most 8 pairs, or 4.
 #define FO_NORM_SHAPES(entry, pairs4, vec)                 \
   if constexpr (!(pairs4)) {                               \
     if (D <= 256) return entry<DT, 1, 4, vec, LAYER>(D);   \
@@ -779,7 +783,7 @@ Shape bwd_entry(int D) {
 
 template <int DT, int VEC, bool LAYER>
 Shape fwd_shape(int D) {
-  FO_NORM_SHAPES(fwd_entry, false, VEC)
+  FO_NORM_SHAPES(fwd_entry, !LAYER || VEC == 1, VEC)
   if (D <= 8192) return fwd_entry<DT, 16, 8, VEC, LAYER>(D);
   return fwd_entry<DT, 16, 16, VEC, LAYER, 3>(D);
 }
@@ -849,12 +853,11 @@ void fill(NormParams* p, const FoBlockNormDesc* d) {
   p->scale = d->residual_scale, p->eps = d->eps;
 }
 
-// Work split: units of rows inside one gate group, about one a resident CTA (three a SM
-// forward, two backward, where a unit also costs its partial sums), whatever the device, so
-// that the workspace's size needs no device.  16 row-group turns or more a CTA keep its ring
-// and its sums worth while; shorter batches give each row group one row at least.
+// Work split: units of rows inside one gate group, one a resident CTA (backward, where a unit
+// also costs its partial sums, two a SM, one for wide rows, whatever the device, so that the
+// workspace's size needs no device); short batches give each row group one row at least.
 struct Plan {
-  int groups, chunks, chunk_rows, units, ldp;
+  int groups, chunks, units, ldp;
   size_t bytes;
 };
 
@@ -867,8 +870,7 @@ Plan plan(const FoBlockNormDesc* d, int per_sm, int row_groups) {
   const int turns = (rpg + row_groups - 1) / row_groups;
   if (chunks > turns) chunks = turns;
   if (chunks < 1) chunks = 1;
-  b.chunk_rows = (rpg + chunks - 1) / chunks;
-  b.chunks = (rpg + b.chunk_rows - 1) / b.chunk_rows;
+  b.chunks = chunks;
   b.units = b.groups * b.chunks;
   b.ldp = (static_cast<int>(d->D) + 3) / 4 * 4;
   b.bytes = 4 * static_cast<size_t>(b.units) * b.ldp * sizeof(float);
@@ -876,7 +878,7 @@ Plan plan(const FoBlockNormDesc* d, int per_sm, int row_groups) {
 }
 
 void set_plan(NormParams* p, const Plan& b) {
-  p->groups = b.groups, p->chunks = b.chunks, p->chunk_rows = b.chunk_rows, p->ldp = b.ldp;
+  p->groups = b.groups, p->chunks = b.chunks, p->ldp = b.ldp;
 }
 
 // The backward plan without a device or a dtype: the row groups of the 16-byte layout.
@@ -904,11 +906,10 @@ extern "C" int fo_block_norm(const FoBlockNormDesc* d, void* stream) {
   fill(&p, d);
   const bool v8 = vectors(d, false), bf = d->dtype == FO_DT_BF16;
   const Shape s = p.layer ? shape_of<false, true>(bf, v8, p.D) : shape_of<false, false>(bf, v8, p.D);
-  const int per_sm = s.warps == 16 ? 1 : 3;
-  const Plan b = plan(d, per_sm, row_groups(s.warps));
+  const Plan b = plan(d, s.ctas, row_groups(s.warps));
   set_plan(&p, b);
   p.status = hd.status, p.timeout_ns = hd.timeout_ns;
-  const cudaError_t e = launch_pdl(s.kern, *s.opted, dim3(min_grid(b, hd.sms * per_sm)), dim3(32 * s.warps, row_groups(s.warps)), s.smem, 1,
+  const cudaError_t e = launch_pdl(s.kern, *s.opted, dim3(min_grid(b, hd.sms * s.ctas)), dim3(32 * s.warps, row_groups(s.warps)), s.smem, 1,
                                    static_cast<cudaStream_t>(stream), p);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   host_count_launches(1);
