@@ -51,8 +51,9 @@ struct W4Params {
   long long ldq[2], lds[2], ldz[2];
   int per32;      // 32-k blocks a group
   uint32_t rcp;   // 2^32 / (steps a group), rounded up: GS 4, groups longer than a step
-  int vec;        // a step's scales (zeros) of a row are read at once
+  int vec;        // a batch's scales (zeros) of a row are read at once
   int share;      // W: warps that share a tile
+  int lg;         // steps of a batch
   const void* bias;
   int act;
   void* out;
@@ -102,6 +103,81 @@ constexpr int kRows = 32;                  // weight rows of a tile: two 16-row 
 constexpr int kStepW = kRows * 64;         // their bytes in a step
 constexpr int kTable = kRows * 40;         // a step's (scale, -scale * offset) pairs, up to 4 a row
 
+// Which steps a warp takes: batches of 2^lg steps, dealt to the warps in turn, so that a row's
+// scales of a whole batch come by one load (a load of every lane's own row costs the SM 32 tag
+// lookups whatever its width; 4096 x 16384 block of one token, groups of 64, step by step 47.3
+// us, by batches 37.2).  Short K: single steps.
+struct W4Steps {
+  int first, stride, lg, count;
+  __device__ __forceinline__ W4Steps(int warp, int warps, int lg_, int steps) : first(warp), stride(warps), lg(lg_) {
+    const int batches = (steps + (1 << lg) - 1) >> lg;
+    const int n = first < batches ? (batches - first + stride - 1) / stride : 0;
+    // (the last batch may be short)
+    count = n == 0 ? 0 : ((n - 1) << lg) + min(1 << lg, steps - ((first + (n - 1) * stride) << lg));
+  }
+  __device__ __forceinline__ int at(int i) const { return ((first + (i >> lg) * stride) << lg) + (i & ((1 << lg) - 1)); }
+};
+
+constexpr int batch_lg(int GS) { return GS == 1 ? 1 : 2; }  // 8 entries, or 4
+
+// A row's scales and zeros (lane l: row l of the tile): the current batch, the next one under way.
+template <int GS, int DT>
+struct W4Scales {
+  static constexpr int ENT = 4 / GS;  // a step
+  const unsigned short* sc;
+  const unsigned char* zc;
+  int groups;
+  uint64_t s[2], z, ns[2], nz;  // 16-bit scales, 8-bit zeros, the first lowest
+  __device__ __forceinline__ void ask(const W4Params& p, int step, int lg) {
+    constexpr int kAll = ENT << batch_lg(GS);
+    nz = 0x0808080808080808ull;
+    const int at = step * ENT;  // the entry, where a group is GS blocks
+    if (p.vec && lg == batch_lg(GS) && at + kAll <= groups) {
+      if (kAll == 8) {
+        const ulonglong2 v = __ldg(reinterpret_cast<const ulonglong2*>(sc + at));
+        ns[0] = v.x, ns[1] = v.y;
+        if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned long long*>(zc + at));
+      } else {
+        ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at)), ns[1] = 0;
+        if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned*>(zc + at));
+      }
+      return;
+    }
+    if (GS == 1 && p.vec && lg == 0 && at + 4 <= groups) {
+      ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at)), ns[1] = 0;
+      if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned*>(zc + at));
+      return;
+    }
+    if (GS == 2 && p.vec && lg == 0 && at + 2 <= groups) {
+      ns[0] = __ldg(reinterpret_cast<const unsigned*>(sc + at)), ns[1] = 0;
+      if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned short*>(zc + at));
+      return;
+    }
+    ns[0] = ns[1] = 0;
+    if (zc != nullptr) nz = 0;
+#pragma unroll
+    for (int e = 0; e < kAll; ++e) {
+      if (e >= ENT << lg) break;
+      const int i = at + e;
+      const int of = GS == 4 ? (p.rcp != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(i), p.rcp)) : i)
+                     : GS == 2 ? i : i / p.per32;
+      const int g = min(of, groups - 1);  // past K: unused
+      ns[e / 4] |= static_cast<uint64_t>(__ldg(sc + g)) << (16 * (e & 3));
+      if (zc != nullptr) nz |= static_cast<uint64_t>(__ldg(zc + g)) << (8 * e);
+    }
+  }
+  __device__ __forceinline__ void turn() { s[0] = ns[0], s[1] = ns[1], z = nz; }
+  __device__ __forceinline__ float scale(int e) const {
+    return unpack2<DT>(static_cast<uint32_t>(s[0] >> (16 * e)) & 0xFFFFu).x;
+  }
+  __device__ __forceinline__ float zero(int e) const { return static_cast<float>(static_cast<uint32_t>(z >> (8 * e)) & 255u); }
+  __device__ __forceinline__ void next() {  // to the next step of the batch
+    if constexpr (ENT == 4) s[0] = s[1];
+    else s[0] = s[0] >> (16 * ENT) | s[1] << (64 - 16 * ENT), s[1] >>= 16 * ENT;
+    z >>= 8 * ENT;
+  }
+};
+
 // NT: 8-token MMA blocks.
 template <int NT>
 struct W4Shape {
@@ -136,8 +212,8 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   const int tok0 = static_cast<int>(blockIdx.y) * 8 * NT;
   const int toks = min(8 * NT, p.T - tok0);
   const int steps = (p.K + 127) / 128;
-  const int first = rank * W + warp % W, stride = Q * W;  // this warp's steps
-  const int mine = n0 < p.N && first < steps ? (steps - first + stride - 1) / stride : 0;
+  const W4Steps turn(rank * W + warp % W, Q * W, p.lg, steps);
+  const int mine = n0 < p.N ? turn.count : 0;
   uint8_t* const own = smem_w4 + warp * S::kWarp;
   const uint32_t ring = smem_u32(own);
   uint8_t* const table = own + S::kWarp - kTable;
@@ -159,7 +235,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   uint32_t put = ring;        // where the next one goes
   auto issue = [&]() {        // this warp's next step (an empty group past the end)
     if (todo < mine) {
-      const int s = first + todo * stride;
+      const int s = turn.at(todo);
       // past K: zeros, and nothing is read
       const uint32_t wn = s * 128 + t * 32 < p.K ? 16u : 0u, xn = s * 128 + (lane & 15) * 8 < p.K ? 16u : 0u;
       const int wo = wn ? s * 64 : 0, xo = xn ? s * 128 : 0;
@@ -178,40 +254,15 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   };
   // A step's scales and zeros: lane l those of row l.
   const int tm = GATED ? lane >> 4 : 0, tn = min(n0 + (GATED ? lane & 15 : lane), p.N - 1);
-  const unsigned short* sc = static_cast<const unsigned short*>(p.scale[tm]) + tn * p.lds[tm];
-  const unsigned char* zc = p.zero[tm] == nullptr ? nullptr : p.zero[tm] + tn * p.ldz[tm];
-  const int groups = (p.K + p.per32 * 32 - 1) / (p.per32 * 32);
-  unsigned short sraw[ENT];
-  uint32_t zraw = 0x08080808u;
-  auto ask = [&](int s) {
-    if (GS == 1 && p.vec && s * 4 + 4 <= groups) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(sc + s * 4));
-      sraw[0] = static_cast<unsigned short>(v.x), sraw[1 % ENT] = static_cast<unsigned short>(v.x >> 16);
-      sraw[2 % ENT] = static_cast<unsigned short>(v.y), sraw[3 % ENT] = static_cast<unsigned short>(v.y >> 16);
-      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const uint32_t*>(zc + s * 4));
-      return;
-    }
-    if (GS == 2 && p.vec && s * 2 + 2 <= groups) {
-      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(sc + s * 2));
-      sraw[0] = static_cast<unsigned short>(v), sraw[1 % ENT] = static_cast<unsigned short>(v >> 16);
-      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const unsigned short*>(zc + s * 2));
-      return;
-    }
-    uint32_t z = 0;
-#pragma unroll
-    for (int e = 0; e < ENT; ++e) {
-      const int at = GS == 4 ? (p.rcp != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(s), p.rcp)) : s)
-                     : GS == 2 ? s * 2 + e : (s * 4 + e) / p.per32;
-      const int g = min(at, groups - 1);  // past K: unused
-      sraw[e] = __ldg(sc + g);
-      z |= (zc != nullptr ? static_cast<uint32_t>(__ldg(zc + g)) : 8u) << (8 * e);
-    }
-    zraw = z;
-  };
+  W4Scales<GS, DT> scales;
+  scales.sc = static_cast<const unsigned short*>(p.scale[tm]) + tn * p.lds[tm];
+  scales.zc = p.zero[tm] == nullptr ? nullptr : p.zero[tm] + tn * p.ldz[tm];
+  scales.groups = (p.K + p.per32 * 32 - 1) / (p.per32 * 32);
+  const int batch = (1 << p.lg) - 1;
 
   griddep_wait();
   griddep_launch_dependents();
-  if (mine > 0) ask(first);
+  if (mine > 0) scales.ask(p, turn.at(0), p.lg);
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) issue();
 
@@ -225,14 +276,17 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   for (int i = 0; i < mine; ++i) {
     cp_async_wait<S::kStages - 2>();
     __syncwarp();  // other lanes' copies, and their reads of the slot and the table refilled next
+    const bool fresh_batch = (i & batch) == 0;
+    if (fresh_batch) scales.turn();
 #pragma unroll
     for (int e = 0; e < ENT; ++e) {
-      const float v = unpack2<DT>(sraw[e]).x, z = static_cast<float>((zraw >> (8 * e)) & 255u);
+      const float v = scales.scale(e), z = scales.zero(e);
       *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v * kBack, -v * (kLeft + z));
     }
     __syncwarp();
     issue();
-    if (i + 1 < mine) ask(first + (i + 1) * stride);
+    if (fresh_batch && i + batch + 1 < mine) scales.ask(p, turn.at(i + batch + 1), p.lg);
+    scales.next();
     float dot[2][NT][4], sx[NT][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -450,8 +504,8 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
   const int n0 = (tile0 + warp / W) * kOut;
   const int cols = kPlanes * p.T;
   const int steps = (p.K + 127) / 128;
-  const int first = rank * W + warp % W, stride = Q * W;  // this warp's steps
-  const int mine = n0 < p.N && first < steps ? (steps - first + stride - 1) / stride : 0;
+  const W4Steps turn(rank * W + warp % W, Q * W, p.lg, steps);
+  const int mine = n0 < p.N ? turn.count : 0;
   uint8_t* const own = smem_w4 + warp * S::kWarp;
   const uint32_t ring = smem_u32(own);
   uint8_t* const table = own + S::kWarp - kTable;
@@ -466,7 +520,7 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
   int todo = 0, xtodo = 0;
   auto weights = [&](int i) {  // step i's weights
     if (i < mine) {
-      const int s = first + i * stride;
+      const int s = turn.at(i);
       const uint32_t put = ring + i % S::kStages * S::kStep, wn = s * 128 + t * 32 < p.K ? 16u : 0u;
       const int wo = wn ? s * 64 : 0;
 #pragma unroll
@@ -476,7 +530,7 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
   auto digits = [&](int i) {  // and its digits (used columns only) and their sums
     if (i < mine) {
       const uint32_t put = ring + i % S::kStages * S::kStep + kStepW;
-      const uint8_t* rec = p.digits + static_cast<long long>(first + i * stride) * S::kRec;
+      const uint8_t* rec = p.digits + static_cast<long long>(turn.at(i)) * S::kRec;
 #pragma unroll
       for (int c = 0; c < 2 * NT; ++c) {
         const int at = c * 32 + lane;  // 16-byte block: group, column, half
@@ -487,40 +541,15 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
     cp_async_commit();
   };
   const int tm = GATED ? lane >> 4 : 0, tn = min(n0 + (GATED ? lane & 15 : lane), p.N - 1);
-  const unsigned short* sc = static_cast<const unsigned short*>(p.scale[tm]) + tn * p.lds[tm];
-  const unsigned char* zc = p.zero[tm] == nullptr ? nullptr : p.zero[tm] + tn * p.ldz[tm];
-  const int groups = (p.K + p.per32 * 32 - 1) / (p.per32 * 32);
-  unsigned short sraw[ENT];
-  uint32_t zraw = 0x08080808u;
-  auto ask = [&](int s) {
-    if (GS == 1 && p.vec && s * 4 + 4 <= groups) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(sc + s * 4));
-      sraw[0] = static_cast<unsigned short>(v.x), sraw[1 % ENT] = static_cast<unsigned short>(v.x >> 16);
-      sraw[2 % ENT] = static_cast<unsigned short>(v.y), sraw[3 % ENT] = static_cast<unsigned short>(v.y >> 16);
-      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const uint32_t*>(zc + s * 4));
-      return;
-    }
-    if (GS == 2 && p.vec && s * 2 + 2 <= groups) {
-      const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(sc + s * 2));
-      sraw[0] = static_cast<unsigned short>(v), sraw[1 % ENT] = static_cast<unsigned short>(v >> 16);
-      if (zc != nullptr) zraw = __ldg(reinterpret_cast<const unsigned short*>(zc + s * 2));
-      return;
-    }
-    uint32_t z = 0;
-#pragma unroll
-    for (int e = 0; e < ENT; ++e) {
-      const int at = GS == 4 ? (p.rcp != 0 ? static_cast<int>(__umulhi(static_cast<uint32_t>(s), p.rcp)) : s)
-                     : GS == 2 ? s * 2 + e : (s * 4 + e) / p.per32;
-      const int g = min(at, groups - 1);  // past K: unused
-      sraw[e] = __ldg(sc + g);
-      z |= (zc != nullptr ? static_cast<uint32_t>(__ldg(zc + g)) : 8u) << (8 * e);
-    }
-    zraw = z;
-  };
+  W4Scales<GS, DT> scales;
+  scales.sc = static_cast<const unsigned short*>(p.scale[tm]) + tn * p.lds[tm];
+  scales.zc = p.zero[tm] == nullptr ? nullptr : p.zero[tm] + tn * p.ldz[tm];
+  scales.groups = (p.K + p.per32 * 32 - 1) / (p.per32 * 32);
+  const int batch = (1 << p.lg) - 1;
 
   // The weights and scales are final before the digits' kernel ends (it began after whatever
   // wrote them), the digits are not.
-  if (mine > 0) ask(first);
+  if (mine > 0) scales.ask(p, turn.at(0), p.lg);
 #pragma unroll
   for (; todo < S::kStages - 1; ++todo) weights(todo);
   for (int i = lane; i < S::kStages * (S::kRec / 16); i += 32) {  // columns without a digit stay zero
@@ -541,15 +570,18 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
   for (int i = 0; i < mine; ++i) {
     cp_async_wait<S::kStages - 2>();
     __syncwarp();  // other lanes' copies, and their reads of the slot and the table refilled next
+    const bool fresh_batch = (i & batch) == 0;
+    if (fresh_batch) scales.turn();
 #pragma unroll
     for (int e = 0; e < ENT; ++e) {
-      const float v = unpack2<DT>(sraw[e]).x, z = static_cast<float>((zraw >> (8 * e)) & 255u);
+      const float v = scales.scale(e), z = scales.zero(e);
       *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v, -v * z);
     }
     __syncwarp();
     weights(i + S::kStages - 1);
     digits(i + S::kStages - 1);
-    if (i + 1 < mine) ask(first + (i + 1) * stride);
+    if (fresh_batch && i + batch + 1 < mine) scales.ask(p, turn.at(i + batch + 1), p.lg);
+    scales.next();
     const uint32_t stage = ring + slot * S::kStep;
     const uint8_t* stage_p = own + slot * S::kStep;
     int dot[2][NT][4];
@@ -655,25 +687,26 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
 // Tiles, warps a tile and CTAs a tile: about as many warps as fit at once, each with a step or
 // more.
 struct W4Plan {
-  int share, q;
+  int share, q, lg;
   unsigned ctas;
 };
 
-W4Plan w4_plan(int N, int K, int out, int chunks, int ctas_a_sm, int sms) {
+W4Plan w4_plan(int N, int K, int out, int chunks, int ctas_a_sm, int batch, int sms) {
   const long long tiles = (N + out - 1) / out, fit = 7ll * ctas_a_sm * sms;
   const int steps = (K + 127) / 128;
   int W = 1, Q = 1;
   while (W < kWarps && tiles * chunks * W < fit && steps >= 2 * W) W *= 2;
   while (W == kWarps && Q < 8 && tiles * chunks * Q * W < 8ll * sms && steps >= kWarps * Q * 2) Q *= 2;
-  return {W, Q, static_cast<unsigned>((tiles + kWarps / W - 1) / (kWarps / W) * Q)};
+  // batches only where every warp has whole ones
+  return {W, Q, steps >> batch >= W * Q ? batch : 0, static_cast<unsigned>((tiles + kWarps / W - 1) / (kWarps / W) * Q)};
 }
 
 template <bool GATED, int NT, int GS, int DT>
 cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
   static std::atomic<uint64_t> opted{0};
   const int chunks = (p.T + 8 * NT - 1) / (8 * NT);
-  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, sms);
-  p.share = l.share;
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, batch_lg(GS), sms);
+  p.share = l.share, p.lg = l.lg;
   return launch_pdl(fo_w4_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas, chunks), dim3(256), W4Shape<NT>::kSmem, l.q, stream, p);
 }
 
@@ -701,8 +734,8 @@ cudaError_t launch_digits(W4Params p, int x_dt, void* room, int sms, cudaStream_
   const unsigned blocks = static_cast<unsigned>((d.T * d.steps + 15) / 16);
   cudaError_t e = launch_pdl(fo_w4_digits_kernel<NT, GS>, none, dim3(blocks), dim3(256), 0, 1, stream, d);
   if (e != cudaSuccess) return e;
-  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, 1, 2, sms);
-  p.share = l.share, p.digits = d.digits;
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, 1, 2, batch_lg(GS), sms);
+  p.share = l.share, p.lg = l.lg, p.digits = d.digits;
   return launch_pdl(fo_w4i_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas), dim3(256), W4iShape<NT, GS>::kSmem, l.q, stream, p);
 }
 
@@ -776,10 +809,10 @@ int act_code(int act) {
 int run(W4Params p, bool gated, int dtype, int x_dt, void* room, const HostDevice& hd, cudaStream_t st) {
   const uint32_t per = static_cast<uint32_t>(p.per32) / 4;  // steps a group
   p.rcp = per > 1 ? static_cast<uint32_t>((0x100000000ull + per - 1) / per) : 0u;
-  p.vec = p.per32 <= 2;
+  p.vec = p.per32 == 1 || p.per32 == 2 || p.per32 == 4;
   for (int m = 0; m < (gated ? 2 : 1); ++m)
-    p.vec = p.vec && p.lds[m] % 4 == 0 && reinterpret_cast<uintptr_t>(p.scale[m]) % 8 == 0 &&
-            (p.zero[m] == nullptr || (p.ldz[m] % 4 == 0 && reinterpret_cast<uintptr_t>(p.zero[m]) % 4 == 0));
+    p.vec = p.vec && p.lds[m] % 8 == 0 && reinterpret_cast<uintptr_t>(p.scale[m]) % 16 == 0 &&
+            (p.zero[m] == nullptr || (p.ldz[m] % 8 == 0 && reinterpret_cast<uintptr_t>(p.zero[m]) % 8 == 0));
   const bool bf = dtype == FO_DT_BF16;
   const cudaError_t e = gated ? (bf ? by_group<true, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<true, DT_F16>(p, x_dt, room, hd.sms, st))
                               : (bf ? by_group<false, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<false, DT_F16>(p, x_dt, room, hd.sms, st));
