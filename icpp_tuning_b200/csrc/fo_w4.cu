@@ -28,12 +28,14 @@
 // steps.  Partial sums meet in shared memory (distributed across the cluster) and are added in
 // a fixed order.
 //
-// Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (101 MB of
-// weights) 37.5 us with its digits' kernels, 4.9 TB/s in the gated product (16-bit operands:
-// 51.9); 16384 x 4096 product 13.8 us (16.5); 8 tokens, block 51.3 us; 5 tokens, fp16, groups
-// of 32 with zeros, 57.7 us (113 MB).  The 16-bit form keeps the integer and logic pipe busy
-// 61% of the time, which bounds it; short products are bound by the launch and the start and
-// end of their few steps a warp (4096 x 4096, one token: 6.7 us for 8.7 MB).
+// Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
+// weights and scales) 34.4 us with its digits' kernels, 5.0 TB/s in the gated product (16-bit
+// operands: 51.9); 16384 x 4096 product 13.8 us; 8 tokens, block 47.9 us; 5 tokens, fp16,
+// groups of 32 with zeros, 56.6 us (120 MB).  That last form is bound by the latencies of a
+// step's chain (copies, table, MMAs, sums) at 14 warps a SM: its integer pipe is busy 43% of
+// the time, issue 37%; without the products its copies alone take 44 us.  Short products are
+// bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
+// 6.9 us for 8.7 MB).
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   if (Q > 1) cluster_sync();  // the others may still read this CTA's sums
 }
 
-// ---------------------------------------------------------------------- up to 8 tokens
+// ---------------------------------------------------------------------- x as digits
 constexpr int kPlanes = 3;
 
 // A step's record: 4 groups x 8 NT columns x 32 digits, then every column's sums over the
@@ -711,12 +713,13 @@ cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
 }
 
 int digit_blocks(int64_t T) { return static_cast<int>(kPlanes * T + 7) / 8; }
-// Whether x travels as digits: two MMA columns' blocks cost a group of 128 little (4096 x 16384
-// gated block, 4 tokens: 45.0 -> 40.3 us), shorter groups too much.  Up to 2^24 weights the
-// second launch costs the caller more (3 us) than the GPU saves (4096 x 4096: 7.7 -> 7.0 us;
-// 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
+// Whether x travels as digits: always where the tokens' digits fill one block of 8 columns (4096
+// x 16384 block, one token: groups of 128 51.9 -> 34.4 us, of 64 63 -> 37.7); up to three where
+// a group is a step or longer (4 tokens 45.0 -> 37.7, 8 tokens 52.5 -> 47.9; groups of 32, 3
+// tokens: 50.7 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
+// the GPU saves (4096 x 4096: 7.7 -> 7.0 us; 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
 bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
-  return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 2 : 1);
+  return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1);
 }
 // Bytes of the digit records.
 size_t digit_bytes(int64_t T, int64_t K, int per32) {
@@ -742,7 +745,10 @@ cudaError_t launch_digits(W4Params p, int x_dt, void* room, int sms, cudaStream_
 template <bool GATED, int GS, int DT>
 cudaError_t by_tokens(const W4Params& p, int x_dt, void* room, int sms, cudaStream_t s) {
   if (room != nullptr) {
-    if (GS == 4 && digit_blocks(p.T) == 2) return launch_digits<GATED, GS == 4 ? 2 : 1, GS, DT>(p, x_dt, room, sms, s);
+    if constexpr (GS == 4) {
+      if (digit_blocks(p.T) == 3) return launch_digits<GATED, 3, GS, DT>(p, x_dt, room, sms, s);
+      if (digit_blocks(p.T) == 2) return launch_digits<GATED, 2, GS, DT>(p, x_dt, room, sms, s);
+    }
     return launch_digits<GATED, 1, GS, DT>(p, x_dt, room, sms, s);
   }
   if (p.T <= 8) return launch<GATED, 1, GS, DT>(p, sms, s);
