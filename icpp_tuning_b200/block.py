@@ -71,11 +71,18 @@ def _sixteen_bit(dt: torch.dtype, name: str) -> int:
     raise ValueError(f"{name} must be float16 or bfloat16, got {dt}")
 
 
+def _new(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous [rows, cols] of like's type."""
+    if like.shape == (rows, cols) and like.is_contiguous():
+        return torch.empty_like(like)  # the cheapest call
+    return like.new_empty((rows, cols))
+
+
 # ---------------------------------------------------------------------- gated feed-forward block
 def _matrix(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """An uninitialised [rows, cols] whose row stride is a multiple of 8 elements."""
     if cols % 8 == 0:
-        return like.new_empty((rows, cols))
+        return _new(rows, cols, like)
     return like.new_empty((rows, (cols + 7) // 8 * 8))[:, :cols]
 
 
@@ -127,7 +134,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     lib = N.lib()
     ref = ctypes.byref(d)
     need = lib.fo_gated_ffn_workspace_size(ref, 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = x.new_empty((need + 1) // 2)  # x's dtype has two bytes
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
     _run(dev, lib.fo_gated_ffn, ref)
     return (y, g, u) if save else y
@@ -152,7 +159,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     lib = N.lib()
     ref = ctypes.byref(d)
     need = lib.fo_gated_ffn_workspace_size(ref, 1)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = x.new_empty((need + 1) // 2)  # x's dtype has two bytes
     d.workspace, d.workspace_bytes = ws.data_ptr(), need
     _run(dev, lib.fo_gated_ffn_backward, ref)
     return dx, dwg, dwu, dwd
@@ -168,10 +175,6 @@ def _param(v: Optional[torch.Tensor], D: int, dt: torch.dtype, name: str) -> Opt
         _vec(v, D, name)  # raises
     return v.data_ptr()
 
-
-def _rows_like(y: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor of y's shape."""
-    return torch.empty_like(y) if y.is_contiguous() else y.new_empty(y.shape)
 
 
 def _norm_desc(y, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps) -> N.FoBlockNormDesc:
@@ -225,7 +228,7 @@ def block_norm(y: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tensor],
         raise ValueError("x and y must share one dtype")
     T, D = y.shape
     d.x, d.ldx = x.data_ptr(), _ld(x, T, D, "x")
-    r, z = _rows_like(y), _rows_like(y)
+    r, z = _new(T, D, y), _new(T, D, y)
     d.r, d.z, d.ldr, d.ldz = r.data_ptr(), z.data_ptr(), D, D
     _run(dev, N.lib().fo_block_norm, ctypes.byref(d))
     return r, z
@@ -253,7 +256,7 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: torch.Tensor, y: torch.T
         d.dr, d.lddr = dr.data_ptr(), _ld(dr, T, D, "dr")
     d.dz, d.lddz = dz.data_ptr(), _ld(dz, T, D, "dz")
     d.r, d.ldr = r.data_ptr(), _ld(r, T, D, "r")
-    out = {"dy": _rows_like(y), "dx": _rows_like(y)}
+    out = {"dy": _new(T, D, y), "dx": _new(T, D, y)}
     d.lddy = d.lddx = D
     # the parameters' gradients share one allocation, gate rows last
     names = [n for n, p in (("dw_pre", w_pre), ("dw_post", w_post), ("db_pre", b_pre), ("db_post", b_post)) if p is not None]
@@ -345,7 +348,7 @@ def matvec_w4(x: torch.Tensor, w: W4, *, bias: Optional[torch.Tensor] = None, st
         if bias.dtype is not dt:
             raise ValueError("bias must have the activations' dtype")
         d.bias = _vec(bias, n, "bias").data_ptr()
-    out = x.new_empty((T, n))
+    out = _new(T, n, x)
     d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
     lib = N.lib()
     ref = ctypes.byref(d)
@@ -377,7 +380,7 @@ def gated_ffn_w4(x: torch.Tensor, w_gate: W4, w_up: W4, w_down: W4, *, act: str 
         raise ValueError(f"w_gate has {F} rows, w_up {F_up}")
     d.w_down, n = _w4(w_down, F, dt, "w_down")
     d.T, d.D, d.F, d.N = T, D, F, n
-    out = x.new_empty((T, n))
+    out = _new(T, n, x)
     d.x, d.out, d.ldo = x.data_ptr(), out.data_ptr(), n
     lib = N.lib()
     ref = ctypes.byref(d)
