@@ -31,7 +31,7 @@
 // Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
 // weights and scales) 34.4 us with its digits' kernels, 5.0 TB/s in the gated product (16-bit
 // operands: 51.9); 16384 x 4096 product 13.8 us; 8 tokens, block 47.9 us; 5 tokens, fp16,
-// groups of 32 with zeros, 56.6 us (120 MB).  That last form is bound by the latencies of a
+// groups of 32 with zeros, 55.4 us (120 MB).  That last form is bound by the latencies of a
 // step's chain (copies, table, MMAs, sums) at 14 warps a SM: its integer pipe is busy 43% of
 // the time, issue 37%; without the products its copies alone take 44 us.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
@@ -55,7 +55,7 @@ struct W4Params {
   uint32_t rcp;   // 2^32 / (steps a group), rounded up: GS 4, groups longer than a step
   int vec;        // a batch's scales (zeros) of a row are read at once
   int share;      // W: warps that share a tile
-  int lg;         // steps of a batch
+  int lg;         // lg of a batch's steps: kBatch or 0
   const void* bias;
   int act;
   void* out;
@@ -120,7 +120,7 @@ struct W4Steps {
   __device__ __forceinline__ int at(int i) const { return ((first + (i >> lg) * stride) << lg) + (i & ((1 << lg) - 1)); }
 };
 
-constexpr int batch_lg(int GS) { return GS == 1 ? 1 : 2; }  // 8 entries, or 4
+constexpr int kBatch = 2;  // lg of a batch's steps
 
 // A row's scales and zeros (lane l: row l of the tile): the current batch, the next one under way.
 template <int GS, int DT>
@@ -129,34 +129,47 @@ struct W4Scales {
   const unsigned short* sc;
   const unsigned char* zc;
   int groups;
-  uint64_t s[2], z, ns[2], nz;  // 16-bit scales, 8-bit zeros, the first lowest
+  static constexpr int kAll = ENT << kBatch, kS = kAll / 4, kZ = kAll > 8 ? 2 : 1;
+  uint64_t s[kS], z[kZ], ns[kS], nz[kZ];  // 16-bit scales, 8-bit zeros, the first lowest
   __device__ __forceinline__ void ask(const W4Params& p, int step, int lg) {
-    constexpr int kAll = ENT << batch_lg(GS);
-    nz = 0x0808080808080808ull;
+#pragma unroll
+    for (int i = 0; i < kS; ++i) ns[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kZ; ++i) nz[i] = 0x0808080808080808ull;
     const int at = step * ENT;  // the entry, where a group is GS blocks
-    if (p.vec && lg == batch_lg(GS) && at + kAll <= groups) {
-      if (kAll == 8) {
-        const ulonglong2 v = __ldg(reinterpret_cast<const ulonglong2*>(sc + at));
-        ns[0] = v.x, ns[1] = v.y;
-        if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned long long*>(zc + at));
+    if (p.vec && lg == kBatch && at + kAll <= groups) {
+      if constexpr (kS == 1) {
+        ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at));
+        if (zc != nullptr) nz[0] = __ldg(reinterpret_cast<const unsigned*>(zc + at));
       } else {
-        ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at)), ns[1] = 0;
-        if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned*>(zc + at));
+#pragma unroll
+        for (int i = 0; i < kS; i += 2) {
+          const ulonglong2 v = __ldg(reinterpret_cast<const ulonglong2*>(sc + at + 4 * i));
+          ns[i] = v.x, ns[i + 1] = v.y;
+        }
+        if (zc != nullptr) {
+          if constexpr (kZ == 1) nz[0] = __ldg(reinterpret_cast<const unsigned long long*>(zc + at));
+          else {
+            const ulonglong2 v = __ldg(reinterpret_cast<const ulonglong2*>(zc + at));
+            nz[0] = v.x, nz[1] = v.y;
+          }
+        }
       }
       return;
     }
     if (GS == 1 && p.vec && lg == 0 && at + 4 <= groups) {
-      ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at)), ns[1] = 0;
-      if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned*>(zc + at));
+      ns[0] = __ldg(reinterpret_cast<const unsigned long long*>(sc + at));
+      if (zc != nullptr) nz[0] = __ldg(reinterpret_cast<const unsigned*>(zc + at));
       return;
     }
     if (GS == 2 && p.vec && lg == 0 && at + 2 <= groups) {
-      ns[0] = __ldg(reinterpret_cast<const unsigned*>(sc + at)), ns[1] = 0;
-      if (zc != nullptr) nz = __ldg(reinterpret_cast<const unsigned short*>(zc + at));
+      ns[0] = __ldg(reinterpret_cast<const unsigned*>(sc + at));
+      if (zc != nullptr) nz[0] = __ldg(reinterpret_cast<const unsigned short*>(zc + at));
       return;
     }
-    ns[0] = ns[1] = 0;
-    if (zc != nullptr) nz = 0;
+    if (zc != nullptr)
+#pragma unroll
+      for (int i = 0; i < kZ; ++i) nz[i] = 0;
 #pragma unroll
     for (int e = 0; e < kAll; ++e) {
       if (e >= ENT << lg) break;
@@ -165,18 +178,30 @@ struct W4Scales {
                      : GS == 2 ? i : i / p.per32;
       const int g = min(of, groups - 1);  // past K: unused
       ns[e / 4] |= static_cast<uint64_t>(__ldg(sc + g)) << (16 * (e & 3));
-      if (zc != nullptr) nz |= static_cast<uint64_t>(__ldg(zc + g)) << (8 * e);
+      if (zc != nullptr) nz[e / 8] |= static_cast<uint64_t>(__ldg(zc + g)) << (8 * (e & 7));
     }
   }
-  __device__ __forceinline__ void turn() { s[0] = ns[0], s[1] = ns[1], z = nz; }
+  __device__ __forceinline__ void turn() {
+#pragma unroll
+    for (int i = 0; i < kS; ++i) s[i] = ns[i];
+#pragma unroll
+    for (int i = 0; i < kZ; ++i) z[i] = nz[i];
+  }
   __device__ __forceinline__ float scale(int e) const {
     return unpack2<DT>(static_cast<uint32_t>(s[0] >> (16 * e)) & 0xFFFFu).x;
   }
-  __device__ __forceinline__ float zero(int e) const { return static_cast<float>(static_cast<uint32_t>(z >> (8 * e)) & 255u); }
+  __device__ __forceinline__ float zero(int e) const { return static_cast<float>(static_cast<uint32_t>(z[0] >> (8 * e)) & 255u); }
   __device__ __forceinline__ void next() {  // to the next step of the batch
-    if constexpr (ENT == 4) s[0] = s[1];
-    else s[0] = s[0] >> (16 * ENT) | s[1] << (64 - 16 * ENT), s[1] >>= 16 * ENT;
-    z >>= 8 * ENT;
+    if constexpr (ENT == 4) {
+#pragma unroll
+      for (int i = 0; i + 1 < kS; ++i) s[i] = s[i + 1];
+    } else if constexpr (kS == 2) {
+      s[0] = s[0] >> (16 * ENT) | s[1] << (64 - 16 * ENT), s[1] >>= 16 * ENT;
+    } else {
+      s[0] >>= 16 * ENT;
+    }
+    if constexpr (kZ == 2) z[0] = z[0] >> (8 * ENT) | z[1] << (64 - 8 * ENT), z[1] >>= 8 * ENT;
+    else z[0] >>= 8 * ENT;
   }
 };
 
@@ -707,7 +732,7 @@ template <bool GATED, int NT, int GS, int DT>
 cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
   static std::atomic<uint64_t> opted{0};
   const int chunks = (p.T + 8 * NT - 1) / (8 * NT);
-  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, batch_lg(GS), sms);
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, kBatch, sms);
   p.share = l.share, p.lg = l.lg;
   return launch_pdl(fo_w4_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas, chunks), dim3(256), W4Shape<NT>::kSmem, l.q, stream, p);
 }
@@ -716,7 +741,7 @@ int digit_blocks(int64_t T) { return static_cast<int>(kPlanes * T + 7) / 8; }
 // Whether x travels as digits: always where the tokens' digits fill one block of 8 columns (4096
 // x 16384 block, one token: groups of 128 51.9 -> 34.4 us, of 64 63 -> 37.7); up to three where
 // a group is a step or longer (4 tokens 45.0 -> 37.7, 8 tokens 52.5 -> 47.9; groups of 32, 3
-// tokens: 50.7 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
+// tokens: 49.3 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
 // the GPU saves (4096 x 4096: 7.7 -> 7.0 us; 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
 bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
   return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1);
@@ -737,7 +762,7 @@ cudaError_t launch_digits(W4Params p, int x_dt, void* room, int sms, cudaStream_
   const unsigned blocks = static_cast<unsigned>((d.T * d.steps + 15) / 16);
   cudaError_t e = launch_pdl(fo_w4_digits_kernel<NT, GS>, none, dim3(blocks), dim3(256), 0, 1, stream, d);
   if (e != cudaSuccess) return e;
-  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, 1, 2, batch_lg(GS), sms);
+  const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, 1, 2, kBatch, sms);
   p.share = l.share, p.lg = l.lg, p.digits = d.digits;
   return launch_pdl(fo_w4i_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas), dim3(256), W4iShape<NT, GS>::kSmem, l.q, stream, p);
 }
@@ -815,10 +840,12 @@ int act_code(int act) {
 int run(W4Params p, bool gated, int dtype, int x_dt, void* room, const HostDevice& hd, cudaStream_t st) {
   const uint32_t per = static_cast<uint32_t>(p.per32) / 4;  // steps a group
   p.rcp = per > 1 ? static_cast<uint32_t>((0x100000000ull + per - 1) / per) : 0u;
+  // a batch's scales and zeros of a row: `all` entries, loads of up to 16 bytes
   p.vec = p.per32 == 1 || p.per32 == 2 || p.per32 == 4;
+  const int all = p.vec ? 16 / p.per32 : 1, part = all < 8 ? all : 8;
   for (int m = 0; m < (gated ? 2 : 1); ++m)
-    p.vec = p.vec && p.lds[m] % 8 == 0 && reinterpret_cast<uintptr_t>(p.scale[m]) % 16 == 0 &&
-            (p.zero[m] == nullptr || (p.ldz[m] % 8 == 0 && reinterpret_cast<uintptr_t>(p.zero[m]) % 8 == 0));
+    p.vec = p.vec && p.lds[m] % part == 0 && reinterpret_cast<uintptr_t>(p.scale[m]) % (2 * part) == 0 &&
+            (p.zero[m] == nullptr || (p.ldz[m] % all == 0 && reinterpret_cast<uintptr_t>(p.zero[m]) % all == 0));
   const bool bf = dtype == FO_DT_BF16;
   const cudaError_t e = gated ? (bf ? by_group<true, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<true, DT_F16>(p, x_dt, room, hd.sms, st))
                               : (bf ? by_group<false, DT_BF16>(p, x_dt, room, hd.sms, st) : by_group<false, DT_F16>(p, x_dt, room, hd.sms, st));
