@@ -333,7 +333,10 @@ def _w4(w: W4, K: int, dtype: torch.dtype, name: str) -> Tuple[N.FoW4, int]:
 
 
 def matvec_w4(x: torch.Tensor, w: W4, *, bias: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-    """x [T, K] @ w^T (+ bias) for a few tokens, w in 4 bits: [T, N] of x's dtype."""
+    """x [T, K] @ w^T (+ bias) for a few tokens, w in 4 bits: [T, N] of x's dtype.
+
+    Sums are fp32.  One token, or a few, times large weights takes x as fixed point of 23 bits
+    relative to the largest of its 128 values: an infinity in x then gives NaN in its row."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return matvec_w4(x, w, bias=bias)

@@ -826,7 +826,7 @@ bool vectors(const FoBlockNormDesc* d, bool bwd) {
 int check(const FoBlockNormDesc* d, bool bwd) {
   if (d == nullptr) return host_fail(FO_EINVAL, "null descriptor");
   if (d->T < 0 || d->D < 0) return host_fail(FO_EINVAL, "negative problem size");
-  if (d->T > (1ll << 31) - 1) return host_fail(FO_EINVAL, "T = %lld exceeds 2^31 - 1", static_cast<long long>(d->T));
+  if (d->T > 1ll << 30) return host_fail(FO_EINVAL, "T = %lld exceeds 2^30", static_cast<long long>(d->T));  // rows ahead stay in 31 bits
   if (d->dtype != FO_DT_F16 && d->dtype != FO_DT_BF16) return host_fail(FO_EINVAL, "dtype must be FO_DT_F16 or FO_DT_BF16");
   if (d->vec_dtype < FO_DT_F16 || d->vec_dtype > FO_DT_F32) return host_fail(FO_EINVAL, "bad vec_dtype %d", d->vec_dtype);
   if (d->norm != FO_NORM_RMS && d->norm != FO_NORM_LAYER) return host_fail(FO_EINVAL, "norm must be FO_NORM_RMS or FO_NORM_LAYER");

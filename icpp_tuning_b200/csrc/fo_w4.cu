@@ -31,7 +31,7 @@
 // Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
 // weights and scales) 34.4 us with its digits' kernels, 5.0 TB/s in the gated product (16-bit
 // operands: 51.9); 16384 x 4096 product 13.8 us; 8 tokens, block 47.9 us; 5 tokens, fp16,
-// groups of 32 with zeros, 55.4 us (120 MB).  That last form is bound by the latencies of a
+// groups of 32 with zeros, 52.8 us (120 MB).  That last form is bound by the latencies of a
 // step's chain (copies, table, MMAs, sums) at 14 warps a SM: its integer pipe is busy 43% of
 // the time, issue 37%; without the products its copies alone take 44 us.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
@@ -219,9 +219,12 @@ struct W4Shape {
 };
 
 // GS: 32-k blocks whose sums share a scale in one step (1, 2 or 4; 1 serves any group size).
-template <bool GATED, int NT, int GS, int DT>
+// JOINT: x's rows are the two parts of half as many tokens; the ring takes the high ones first,
+// and a token's parts meet in one accumulator.
+template <bool GATED, int NT, int GS, int DT, bool JOINT>
 __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __grid_constant__ W4Params p) {
   using S = W4Shape<NT>;
+  constexpr int NA = JOINT ? NT / 2 : NT;                     // blocks of sums
   constexpr int ENT = 4 / GS, kOut = GATED ? 16 : 32;         // outputs of a tile
   constexpr float kLeft = DT == DT_BF16 ? 128.f : 0.f;        // offset that stays in the opened weights
   constexpr float kBack = DT == DT_BF16 ? 1.f : 16777216.f;   // what their scale lacks
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
     const int m = GATED ? c >> 1 : 0, n = n0 + r + 8 * (GATED ? c & 1 : c);
     src[c] = static_cast<const char*>(p.q[m]) + min(n, p.N - 1) * p.ldq[m] + t * 16;
   }
-  const unsigned short* xs = static_cast<const unsigned short*>(p.x) + (tok0 + (lane >> 4)) * p.ldx + (lane & 15) * 8;
+  const unsigned short* xs = static_cast<const unsigned short*>(p.x) + (tok0 + (JOINT ? 2 : 1) * (lane >> 4)) * p.ldx + (lane & 15) * 8;
   // The four 16-byte blocks of a weight row are stored rotated, odd tokens' halves swapped, so
   // that the reads below fall into distinct banks.
   const uint32_t w_at = (r * 4 + (t ^ ((r >> 1) & 3))) * 16;
@@ -270,8 +273,9 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
       for (int c = 0; c < 4; ++c) cp_async_16(put + w_at + c * 512, src[c] + wo, wn);
 #pragma unroll
       for (int c = 0; c < 4 * NT; ++c) {  // two tokens a copy, 16 blocks each
-        if (c > 0 && 2 * c >= toks) break;
-        if (2 * c + (lane >> 4) < toks) cp_async_16(put + x_at + c * 512, xs + 2 * c * p.ldx + xo, xn);
+        const int row = !JOINT ? 2 * c : c < 2 * NT ? 4 * c : 4 * c - 8 * NT + 1;  // of its first token
+        if (!JOINT && c > 0 && row >= toks) break;
+        if (row + (JOINT ? 2 : 1) * (lane >> 4) < toks) cp_async_16(put + x_at + c * 512, xs + row * p.ldx + xo, xn);
       }
     }
     cp_async_commit();
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) issue();
 
-  float acc[2][NT][4] = {};
+  float acc[2][NA][4] = {};
   const float none[4] = {0.f, 0.f, 0.f, 0.f};
   const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
   // ldmatrix: lane l addresses row l % 8 of row block l / 8
@@ -314,14 +318,14 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
     issue();
     if (fresh_batch && i + batch + 1 < mine) scales.ask(p, turn.at(i + batch + 1), p.lg);
     scales.next();
-    float dot[2][NT][4], sx[NT][4];
+    float dot[2][NA][4], sx[NA][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t xb[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         uint4 d = make_uint4(0u, 0u, 0u, 0u);
-        if (nt * 8 + r < toks) d = lds128(stage + my_x + nt * 2048 + ((4 * j + t) ^ x_rot) * 16);
+        if ((JOINT ? 2 * (nt % NA * 8 + r) : nt * 8 + r) < toks) d = lds128(stage + my_x + nt * 2048 + ((4 * j + t) ^ x_rot) * 16);
         xb[nt][0] = __byte_perm(d.x, d.z, 0x5410u), xb[nt][1] = __byte_perm(d.x, d.z, 0x7632u);
         xb[nt][2] = __byte_perm(d.y, d.w, 0x5410u), xb[nt][3] = __byte_perm(d.y, d.w, 0x7632u);
       }
@@ -330,8 +334,8 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
       const bool fresh = j % GS == 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma_16816<DT>(sx[nt], ones, xb[nt][0], xb[nt][1], fresh ? none : sx[nt]);
-        mma_16816<DT>(sx[nt], ones, xb[nt][2], xb[nt][3], sx[nt]);
+        mma_16816<DT>(sx[nt % NA], ones, xb[nt][0], xb[nt][1], fresh && nt < NA ? none : sx[nt % NA]);
+        mma_16816<DT>(sx[nt % NA], ones, xb[nt][2], xb[nt][3], sx[nt % NA]);
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -342,8 +346,8 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
           for (int e = 0; e < 4; ++e) a[e >> 1][(e & 1) * 2 + h] = ((w[2 * m + h] >> (4 * e)) & 0x000F000Fu) | kMagic;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma_16816<DT>(dot[m][nt], a[0], xb[nt][0], xb[nt][1], fresh ? none : dot[m][nt]);
-          mma_16816<DT>(dot[m][nt], a[1], xb[nt][2], xb[nt][3], dot[m][nt]);
+          mma_16816<DT>(dot[m][nt % NA], a[0], xb[nt][0], xb[nt][1], fresh && nt < NA ? none : dot[m][nt % NA]);
+          mma_16816<DT>(dot[m][nt % NA], a[1], xb[nt][2], xb[nt][3], dot[m][nt % NA]);
         }
       }
       if ((j + 1) % GS == 0) {
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
           const float2 lo = *reinterpret_cast<const float2*>(table + (m * 16 + r) * 40 + j / GS * 8);
           const float2 hi = *reinterpret_cast<const float2*>(table + (m * 16 + r + 8) * 40 + j / GS * 8);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < NA; ++nt) {
             const Two x01 = two(sx[nt][0], sx[nt][1]);
             const float2 u = both(fma2(x01, two(lo.y), fma2(two(dot[m][nt][0], dot[m][nt][1]), two(lo.x), two(acc[m][nt][0], acc[m][nt][1]))));
             const float2 v = both(fma2(x01, two(hi.y), fma2(two(dot[m][nt][2], dot[m][nt][3]), two(hi.x), two(acc[m][nt][2], acc[m][nt][3]))));
@@ -366,14 +370,14 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   }
 
   // Partial sums: the warps of a tile, then the CTAs of the cluster (whose tile is one).
-  constexpr int TW = 8 * NT;
+  constexpr int TW = 8 * NA;
   cp_async_wait_all();
   __syncwarp();  // the warp is done with its ring
   float* red = reinterpret_cast<float*>(own);
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NA; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) red[(m * 16 + (e >> 1) * 8 + r) * TW + nt * 8 + 2 * t + (e & 1)] = acc[m][nt][e];
   __syncthreads();
@@ -394,18 +398,19 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
     for (int c = 0; c < Q; ++c) v += ld_cluster_f32(mapa_shared(pa + i * 4, c));
     return v;
   };
-  const int fold = p.joint ? 2 : 1, each = kOut * ((toks + fold - 1) / fold);
+  const bool fold = !JOINT && p.joint;  // a token's parts are two columns
+  const int tokens = p.joint ? (toks + 1) / 2 : toks, each = kOut * tokens;
   for (int o = rank * 256 + threadIdx.x; o < per_cta * each; o += 256 * Q) {
     const int j = o / each, oo = o - j * each;
-    const int tok = oo / kOut * fold, f = oo % kOut;
-    const int n = (tile0 + j) * kOut + f, row = tok0 + tok;
-    if (n >= p.N || row >= p.T) continue;
-    float v = total(j, f * TW + tok);
-    if (p.joint) v += total(j, f * TW + tok + 1);
-    if constexpr (GATED) v = both(gate_act(p.act, two(v))).x * total(j, (16 + f) * TW + tok);
+    const int tok = oo / kOut, f = oo % kOut, col = fold ? 2 * tok : tok;
+    const int n = (tile0 + j) * kOut + f, row = (p.joint ? tok0 / 2 : tok0) + tok;
+    if (n >= p.N) continue;
+    float v = total(j, f * TW + col);
+    if (fold) v += total(j, f * TW + col + 1);
+    if constexpr (GATED) v = both(gate_act(p.act, two(v))).x * total(j, (16 + f) * TW + col);
     else if (p.bias != nullptr) v += load_vec(p.bias, DT, n);
     const uint32_t hi = pack2<DT>(v, 0.f);
-    unsigned short* out = static_cast<unsigned short*>(p.out) + (p.split ? 2 * row : p.joint ? row / 2 : row) * p.ldo + n;
+    unsigned short* out = static_cast<unsigned short*>(p.out) + (p.split ? 2 * row : row) * p.ldo + n;
     *out = static_cast<unsigned short>(hi);
     if (p.split) out[p.ldo] = static_cast<unsigned short>(pack2<DT>(v - unpack2<DT>(hi).x, 0.f));
   }
@@ -728,20 +733,20 @@ W4Plan w4_plan(int N, int K, int out, int chunks, int ctas_a_sm, int batch, int 
   return {W, Q, steps >> batch >= W * Q ? batch : 0, static_cast<unsigned>((tiles + kWarps / W - 1) / (kWarps / W) * Q)};
 }
 
-template <bool GATED, int NT, int GS, int DT>
+template <bool GATED, int NT, int GS, int DT, bool JOINT = false>
 cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
   static std::atomic<uint64_t> opted{0};
   const int chunks = (p.T + 8 * NT - 1) / (8 * NT);
   const W4Plan l = w4_plan(p.N, p.K, GATED ? 16 : 32, chunks, W4Shape<NT>::kCtas, kBatch, sms);
   p.share = l.share, p.lg = l.lg;
-  return launch_pdl(fo_w4_kernel<GATED, NT, GS, DT>, opted, dim3(l.ctas, chunks), dim3(256), W4Shape<NT>::kSmem, l.q, stream, p);
+  return launch_pdl(fo_w4_kernel<GATED, NT, GS, DT, JOINT>, opted, dim3(l.ctas, chunks), dim3(256), W4Shape<NT>::kSmem, l.q, stream, p);
 }
 
-int digit_blocks(int64_t T) { return static_cast<int>(kPlanes * T + 7) / 8; }
+int64_t digit_blocks(int64_t T) { return (kPlanes * T + 7) / 8; }
 // Whether x travels as digits: always where the tokens' digits fill one block of 8 columns (4096
 // x 16384 block, one token: groups of 128 51.9 -> 34.4 us, of 64 63 -> 37.7); up to three where
 // a group is a step or longer (4 tokens 45.0 -> 37.7, 8 tokens 52.5 -> 47.9; groups of 32, 3
-// tokens: 49.3 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
+// tokens: 48.6 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
 // the GPU saves (4096 x 4096: 7.7 -> 7.0 us; 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
 bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
   return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1);
@@ -749,7 +754,7 @@ bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
 // Bytes of the digit records.
 size_t digit_bytes(int64_t T, int64_t K, int per32) {
   const int ent = per32 % 4 == 0 ? 1 : per32 == 2 ? 2 : 4;
-  return static_cast<size_t>((K + 127) / 128) * digit_blocks(T) * (1024 + (ent + 1) * 32);
+  return static_cast<size_t>((K + 127) / 128 * digit_blocks(T) * (1024 + (ent + 1) * 32));
 }
 
 // x_dt: of p.x.  `room` holds digit_bytes.
@@ -777,6 +782,9 @@ cudaError_t by_tokens(const W4Params& p, int x_dt, void* room, int sms, cudaStre
     return launch_digits<GATED, 1, GS, DT>(p, x_dt, room, sms, s);
   }
   if (p.T <= 8) return launch<GATED, 1, GS, DT>(p, sms, s);
+  if constexpr (!GATED) {
+    if (p.joint) return p.T <= 16 ? launch<GATED, 2, GS, DT, true>(p, sms, s) : launch<GATED, 4, GS, DT, true>(p, sms, s);
+  }
   if (p.T <= 16) return launch<GATED, 2, GS, DT>(p, sms, s);
   return launch<GATED, 4, GS, DT>(p, sms, s);
 }
