@@ -34,21 +34,18 @@ cudaError_t by_act(int act, const FewMaps& m, const FewParams& p, const FewPlan&
 }  // namespace
 
 FewPlan few_plan(int mode, int64_t F, int64_t columns, int kb, int sms) {
-  // The time of a split: the bytes that the busiest SM takes in, at the 85-100 B/ns that a SM
-  // takes from L2, and the exchange of the sums (two cluster barriers, then about 15 B/ns).
-  // Measured, 1 x 1024 x 4096: 30.8, 20.9, 15.0, 13.7 us for 1, 2, 4, 8 CTAs a tile; 24 x 4096 x
-  // 16384: 127, 95, 88, 93 us.
+  // As many CTAs as are resident at once, two a SM: one CTA keeps 110 KB under way, 43 B/ns of
+  // HBM; but K blocks enough that the exchange of the sums stays small beside them.  Measured,
+  // for 1, 2, 4, 8 CTAs a tile: gated product 4096 x 16384 (128 tiles), one token 51.6, 45.3,
+  // 50.6, 55.8 us, 24 tokens 52.9, 51.1, 57.0, 65.3; 2048 x 8192 (64 tiles) 22.5, 20.3, 17.2,
+  // 22.1; block 1 x 1024 x 4096 (32 tiles, 16 K blocks) 16.7, 15.2, 13.8, 14.5; blocks' second
+  // product alone changed, 1 x 4096 x 16384 132, 98, 83, 79; dh 64 x 1024 x 4096 42, 34, 21, 17.
   const int products = mode == FEW_GATED ? 2 : 1;
   FewPlan best{};
   best.nt = columns <= 16 ? 16 : columns <= 32 ? 32 : 64;
   best.tiles = static_cast<int>((F + 127) / 128);
-  double best_ns = 0;
-  for (int q = 1; q <= 8 && q <= kb; q *= 2) {
-    const long long turns = (static_cast<long long>(best.tiles) * q + sms - 1) / sms;
-    const double bytes = static_cast<double>((kb + q - 1) / q) * (products * 16384 + best.nt * 128);
-    const double ns = turns * bytes / 100.0 + (q > 1 ? 1200.0 + best.nt * products * 512.0 * (q - 1) / q / 15.0 : 0.0);
-    if (q == 1 || ns < best_ns) best.q = q, best_ns = ns;
-  }
+  best.q = 1;
+  while (best.q < 8 && 2ll * best.tiles * best.q <= 2 * sms && 4 * products * best.q <= kb) best.q *= 2;
   return best;
 }
 
