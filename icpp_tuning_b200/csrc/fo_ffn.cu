@@ -45,7 +45,7 @@ int cut(int64_t M, int64_t N, int64_t kb, int64_t others, int pairs) {
   for (int s = 1; s <= kFfnMaxParts && s <= kb; ++s) {
     const int64_t unit = (kb + s - 1) / s + 8, units = tiles * s;
     const int64_t mean = (units * unit + others + pairs - 1) / pairs;
-    const int64_t rounds = others > 0 ? (units + pairs - 1) / pairs * unit : (units + pairs - 1) / pairs * unit;
+    const int64_t rounds = (units + pairs - 1) / pairs * unit;
     const int64_t cost = (mean > rounds ? mean : rounds) + (s > 1 ? 10 + s : 0);
     if (best_cost == 0 || cost < best_cost) best = s, best_cost = cost;
   }
@@ -129,12 +129,24 @@ struct Build {
                       dim3(256), 0, 1, st, join);
   }
 
-  // Names each unit's pair when the problems' K differ: longest first, to the pair with the
-  // least work so far (dx of a short batch has few, long tiles; the weight gradients many,
-  // short ones).  Above kFfnOwners units the tiles per pair are many enough to walk them in
-  // turn.
+  // Spreads units of different K.  Few: each gets its pair by name, longest first, to the pair
+  // with the least work so far (dx of a short batch has few, long tiles; the weight gradients
+  // many, short ones).  Many: in turn, but for the pairs that the first problem's longer units
+  // leave without one (4096 x 16384 backward, 65 tokens 357 -> 269 us, 512 tokens 445 -> 390;
+  // 4096 x 4096 x 8192 1266 -> 1232).
   void schedule(int pairs) {
-    if (p.nprob < 2 || p.units > kFfnOwners) return;
+    if (p.nprob < 2) return;
+    if (p.units > kFfnOwners) {
+      const FfnProblem &l = p.prob[0], &s = p.prob[1];
+      const int long_cost = l.kb / l.parts + 8, short_cost = s.kb / s.parts + 8;
+      if (pairs > p.units || long_cost <= short_cost) return;
+      p.longs = l.tiles_m * l.tiles_n * l.parts;
+      p.over = p.longs % pairs;
+      const int rest = pairs - p.over, most = (p.units - p.longs) / rest;
+      p.extra = p.over == 0 ? 0 : (long_cost + short_cost / 2) / short_cost;
+      if (p.extra > most) p.extra = most;
+      return;
+    }
     int load[256] = {0};
     if (pairs > 256) pairs = 256;
     if (pairs > p.units) pairs = p.units;
@@ -186,9 +198,9 @@ int fail_launch(cudaError_t e) { return host_fail(FO_ECUDA, "kernel launch faile
 namespace fo {
 namespace {
 
-
-// Tokens up to which the short-token kernels run.  Forward, T = 32 and 48 at 1024 x 4096: 14 and
-// 23 us there, 25 and 25 us on CTA pairs; backward, T = 64 and 256: 52 and 89 against 85 and 55.
+// Tokens up to which the short-token kernels run.  Forward at 1024 x 4096, 32 tokens 18.4 us
+// there and 24.7 us on CTA pairs (33 tokens; the parts of more would not fit one tile); backward
+// 64 tokens 50.8 and 51.2 us, at 4096 x 16384 217 and 269.
 constexpr int kFewForward = 32, kFewBackward = 64;
 
 constexpr int kSms = 148;

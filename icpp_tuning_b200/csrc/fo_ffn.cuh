@@ -61,7 +61,11 @@ struct FfnParams {
   long long ldo;
   int* status;
   unsigned long long timeout_ns;
-  int owned;  // owner[u] names the pair that runs unit u (else pair u % pairs)
+  // Which pair runs a unit: the one that owner[] names (owned), else the pairs take them in turn.
+  // Where the first `longs` units are longer and do not come out even (over pairs have one
+  // more), the others first take `extra` more of the rest.
+  int longs, over, extra;
+  int owned;
   unsigned char owner[kFfnOwners];
 };
 
@@ -102,12 +106,22 @@ __device__ __forceinline__ FfnUnit ffn_unit(const FfnParams& p, int u) {
   return r;
 }
 
-// This pair's next unit at or after u.
-__device__ __forceinline__ int ffn_next(const FfnParams& p, int u, int cid, int ncl) {
-  (void)ncl;
-  if (!p.owned) return u;
-  while (u < p.units && p.owner[u] != cid) ++u;
-  return u;
+// This pair's next unit after u, and its first one.
+__device__ __forceinline__ int ffn_after(const FfnParams& p, int u, int cid, int ncl) {
+  if (p.owned) {
+    do ++u;
+    while (u < p.units && p.owner[u] != cid);
+    return u;
+  }
+  if (p.extra == 0) return u + ncl;
+  const int rest = ncl - p.over, mid = p.longs + rest * p.extra;
+  if (u < p.longs) return u + ncl < p.longs ? u + ncl : cid >= p.over ? p.longs + cid - p.over : mid + cid;
+  if (u < mid) return u + rest < mid ? u + rest : mid + cid;
+  return u + ncl;
+}
+__device__ __forceinline__ int ffn_first(const FfnParams& p, int cid, int ncl) {
+  if (p.owned) return ffn_after(p, -1, cid, ncl);
+  return p.extra == 0 || cid < p.longs ? cid : p.longs + cid - p.over;
 }
 
 template <int EPI, int ACT, int DT>
@@ -125,8 +139,6 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int cid = static_cast<int>(blockIdx.x >> 1), ncl = static_cast<int>(gridDim.x >> 1);
-  const int step = p.owned ? 1 : ncl;       // units are walked from `first` with this step,
-  const int first = p.owned ? 0 : cid;      // skipping other pairs' when owners are named
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kFfnStages; ++s) {
@@ -165,7 +177,7 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
       int s = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
+      for (int u = ffn_first(p, cid, ncl); u < p.units && ok; u = ffn_after(p, u, cid, ncl)) {
         const FfnUnit un = ffn_unit(p, u);
         const FfnProblem& q = p.prob[un.pr];
         const int arow = un.tm * kFfnTile + static_cast<int>(rank) * 128;
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
       uint32_t ph = 0, acc_ph = 0;
       uint64_t off = 0;  // of stage s, in descriptor units (A and B stages are alike)
       bool ok = true;
-      for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
+      for (int u = ffn_first(p, cid, ncl); u < p.units && ok; u = ffn_after(p, u, cid, ncl)) {
         const FfnUnit un = ffn_unit(p, u);
         const FfnProblem& q = p.prob[un.pr];
         const int a_mn = q.a_mn, b_mn = q.b_mn;
@@ -370,10 +382,10 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
       }
     };
     if (EPI == FFN_DGATE) {
-      const int u = ffn_next(p, first, cid, ncl);
+      const int u = ffn_first(p, cid, ncl);
       if (u < p.units) ask_gu(u, 0);
     }
-    for (int u = ffn_next(p, first, cid, ncl); u < p.units && ok; u = ffn_next(p, u + step, cid, ncl)) {
+    for (int u = ffn_first(p, cid, ncl); u < p.units && ok; u = ffn_after(p, u, cid, ncl)) {
       const FfnUnit un = ffn_unit(p, u);
       const FfnProblem& q = p.prob[un.pr];
       const int row0 = un.tm * kFfnTile + static_cast<int>(rank) * 128 + quarter * 32;
@@ -446,7 +458,7 @@ __global__ void __launch_bounds__(320, 1) fo_ffn_kernel(const __grid_constant__ 
           own_row(pu, uq);
           {  // the next 32 columns, of this tile or of this pair's next one
             int un2 = u;
-            if (ch == 3) un2 = ffn_next(p, u + step, cid, ncl);
+            if (ch == 3) un2 = ffn_after(p, u, cid, ncl);
             if (un2 < p.units) ask_gu(un2, (ch + 1) & 3);
           }
           uint32_t r[32];

@@ -73,6 +73,12 @@ def test_backward(T, D, F, Nn, layout):
     status_clean()
 
 
+@pytest.mark.parametrize("T,D,F,Nn", [(70, 7304, 2048, 520), (300, 7304, 2048, 520), (600, 4104, 2040, 2080)])
+def test_backward_of_many_units(T, D, F, Nn):
+    """More output tiles than are spread by name, those of dx longer or shorter than the rest."""
+    test_backward(T, D, F, Nn, "kn")
+
+
 def _strided(t):
     """Rows that start every multiple of 8 elements."""
     c = t.shape[1]
