@@ -36,10 +36,10 @@ cudaError_t by_act(int act, const FewMaps& m, const FewParams& p, const FewPlan&
 FewPlan few_plan(int mode, int64_t F, int64_t columns, int kb, int sms) {
   // As many CTAs as are resident at once, two a SM: one CTA keeps 110 KB under way, 43 B/ns of
   // HBM; but K blocks enough that the exchange of the sums stays small beside them.  Measured,
-  // for 1, 2, 4, 8 CTAs a tile: gated product 4096 x 16384 (128 tiles), one token 51.6, 45.3,
-  // 50.6, 55.8 us, 24 tokens 52.9, 51.1, 57.0, 65.3; 2048 x 8192 (64 tiles) 22.5, 20.3, 17.2,
-  // 22.1; block 1 x 1024 x 4096 (32 tiles, 16 K blocks) 16.7, 15.2, 13.8, 14.5; blocks' second
-  // product alone changed, 1 x 4096 x 16384 132, 98, 83, 79; dh 64 x 1024 x 4096 42, 34, 21, 17.
+  // blocks with the gated product in 1, 2, 4, 8 CTAs a tile: 1 x 4096 x 16384 (128 tiles) 71, 67,
+  // 71, 74 us; 24 tokens 84, 79, 85, 92; 8 x 2048 x 8192 (64 tiles) 33, 31, 28, 34; 1 x 1024 x
+  // 4096 (32 tiles, 16 K blocks) 15.1, 13.0, 11.7, 11.7.  With the second product so (32 tiles),
+  // 1 x 4096 x 16384: 120, 85, 73, 67; backward, 64 x 1024 x 4096: 111, 88, 62, 50.
   const int products = mode == FEW_GATED ? 2 : 1;
   FewPlan best{};
   best.nt = columns <= 16 ? 16 : columns <= 32 ? 32 : 64;

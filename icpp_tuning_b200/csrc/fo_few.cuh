@@ -18,8 +18,8 @@
 // 2 t and 2 t + 1: twice the token columns of an MMA that is not the bound, and h costs no
 // precision.
 //
-// Measured, both products of the block, bf16: 4096 x 16384, 403 MB, one token in 69 us (5.8
-// TB/s), 24 tokens in 77 us; 1 x 1024 x 4096, 25 MB in 13 us, bound by the launches and the
+// Measured, both products of the block, bf16: 4096 x 16384, 403 MB, one token in 67 us (6.0
+// TB/s), 24 tokens in 78 us; 1 x 1024 x 4096, 25 MB in 11.7 us, bound by the launches and the
 // first copies' latency.
 #pragma once
 #include "fo_ffn.cuh"

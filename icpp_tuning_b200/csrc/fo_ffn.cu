@@ -200,7 +200,7 @@ namespace {
 
 // Tokens up to which the short-token kernels run.  Forward at 1024 x 4096, 32 tokens 18.4 us
 // there and 24.7 us on CTA pairs (33 tokens; the parts of more would not fit one tile); backward
-// 64 tokens 50.8 and 51.2 us, at 4096 x 16384 217 and 269.
+// 64 tokens 50.1 and 51.2 us, at 4096 x 16384 217 and 269.
 constexpr int kFewForward = 32, kFewBackward = 64;
 
 constexpr int kSms = 148;
