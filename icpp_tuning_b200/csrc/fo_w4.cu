@@ -29,13 +29,12 @@
 // a fixed order.
 //
 // Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
-// weights and scales) 34.4 us with its digits' kernels, 5.0 TB/s in the gated product (16-bit
-// operands: 51.9); 16384 x 4096 product 13.8 us; 8 tokens, block 47.9 us; 5 tokens, fp16,
-// groups of 32 with zeros, 52.8 us (120 MB).  That last form is bound by the latencies of a
-// step's chain (copies, table, MMAs, sums) at 14 warps a SM: its integer pipe is busy 43% of
-// the time, issue 37%; without the products its copies alone take 44 us.  Short products are
+// weights and scales) 30.6 us with its digits' kernels (16-bit operands: 42.1); 16384 x 4096
+// product 10.8 us; 8 tokens, block 44.9 us; 5 tokens, fp16, groups of 32 with zeros, 51 us (120
+// MB).  That last form is bound by the latencies of a step's chain (copies, table, MMAs, sums)
+// at 14 warps a SM: its integer pipe is busy 48% of the time, issue 41%.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
-// 6.9 us for 8.7 MB).
+// 5.1 us for 8.7 MB).
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"
@@ -716,19 +715,24 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------- host
-// Tiles, warps a tile and CTAs a tile: about as many warps as fit at once, each with a step or
-// more.
+// Tiles, warps a tile and CTAs a tile: as many warps as fit at once (a fifth more is better
+// than half as many), then CTAs for a tile of long K, or where most SMs would have none.  Of one
+// token 4096 x 4096: 8 warps 5.1 us, 16 in two CTAs 6.5; 16384 x 4096: 4 warps a tile 10.8, 8
+// (two waves) 13.0; 64 tokens 4096 x 4096: 8 warps 23.6, 16 29.4.
 struct W4Plan {
   int share, q, lg;
   unsigned ctas;
 };
 
 W4Plan w4_plan(int N, int K, int out, int chunks, int ctas_a_sm, int batch, int sms) {
-  const long long tiles = (N + out - 1) / out, fit = 7ll * ctas_a_sm * sms;
+  const long long tiles = (N + out - 1) / out, fit = 6ll * kWarps * ctas_a_sm * sms / 5;
   const int steps = (K + 127) / 128;
   int W = 1, Q = 1;
-  while (W < kWarps && tiles * chunks * W < fit && steps >= 2 * W) W *= 2;
-  while (W == kWarps && Q < 8 && tiles * chunks * Q * W < 8ll * sms && steps >= kWarps * Q * 2) Q *= 2;
+  while (W < kWarps && 2 * tiles * chunks * W <= fit && steps >= 2 * W) W *= 2;
+  auto ctas = [&] { return tiles * chunks * Q; };
+  while (W == kWarps && Q < 8 && 2 * ctas() <= ctas_a_sm * sms &&
+         (steps >= 16 * kWarps * Q || (2 * ctas() <= sms && steps >= 2 * kWarps * Q)))
+    Q *= 2;
   // batches only where every warp has whole ones
   return {W, Q, steps >> batch >= W * Q ? batch : 0, static_cast<unsigned>((tiles + kWarps / W - 1) / (kWarps / W) * Q)};
 }
@@ -743,13 +747,14 @@ cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
 }
 
 int64_t digit_blocks(int64_t T) { return (kPlanes * T + 7) / 8; }
-// Whether x travels as digits: always where the tokens' digits fill one block of 8 columns (4096
-// x 16384 block, one token: groups of 128 51.9 -> 34.4 us, of 64 63 -> 37.7); up to three where
-// a group is a step or longer (4 tokens 45.0 -> 37.7, 8 tokens 52.5 -> 47.9; groups of 32, 3
-// tokens: 48.6 -> 54.5).  Up to 2^24 weights the second launch costs the caller more (3 us) than
-// the GPU saves (4096 x 4096: 7.7 -> 7.0 us; 1024 x 4096: 4.9 -> 6.3; 16384 x 4096: 16.5 -> 13.8).
+// Whether x travels as digits: where the tokens' digits fill one block of 8 columns (4096 x
+// 16384 block, one token: groups of 128 42.1 -> 30.6 us, of 64 45.9 -> 34.6, of 32 51 -> 42); up
+// to three where a group is a step or longer (4 tokens 44.1 -> 34.4, 8 tokens 49.7 -> 44.9;
+// groups of 32, 3 tokens: 48.6 -> 54.5).  Up to 2^24 weights a block the second launch costs
+// the caller more (3 us) than the GPU saves (one token 4096 x 4096 5.2 -> 5.8, 8192 x 4096 8.2 ->
+// 7.9, 16384 x 4096 14.7 -> 10.8; 4 tokens 8192 x 4096 8.6 -> 9.9).
 bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
-  return T > 0 && N * K > (1 << 24) && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1);
+  return T > 0 && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1) && N * K > digit_blocks(T) << 24;
 }
 // Bytes of the digit records.
 size_t digit_bytes(int64_t T, int64_t K, int per32) {

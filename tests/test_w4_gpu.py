@@ -99,7 +99,8 @@ def step_most(x):
 # large weights times a few tokens: x as digits; K off the steps, N off the tiles, every group
 # size's path, the sums of a tile cut over warps and CTAs, values that span seven decades
 LARGE = [(1, 8200, 2048, 32), (2, 16001, 1056, 64), (3, 4100, 4128, 128), (5, 1401, 12800, 256), (1, 129, 131072, 384), (4, 1070, 16000, 4096),
-         (2, 540, 32032, 96), (1, 34000, 512, 128), (6, 2080, 8160, 128), (8, 4097, 4128, 512)]
+         (2, 540, 32032, 96), (1, 34000, 512, 128), (6, 2080, 8160, 128), (8, 4097, 4128, 512),
+         (3, 8200, 4128, 128), (5, 2700, 12800, 256), (8, 12300, 4128, 512)]
 
 
 @pytest.mark.parametrize("wide", [False, True])
@@ -129,7 +130,8 @@ def test_matvec_of_large_weights(T, Nn, K, group, wide):
 
 @pytest.mark.parametrize("T,D,F,Nn,group,down", [(1, 2048, 4160, 4100, 64, 32), (2, 1056, 8192, 2101, 32, 32), (4, 1024, 8224, 2100, 128, 128),
                                                  (5, 2080, 4128, 4100, 256, 128), (3, 2048, 4160, 4100, 128, 32),
-                                                 (8, 1056, 8192, 2101, 128, 256)])
+                                                 (8, 1056, 8192, 2101, 128, 256), (4, 2080, 8224, 4104, 128, 128),
+                                                 (8, 3104, 8192, 6200, 128, 256)])
 def test_gated_of_large_weights(T, D, F, Nn, group, down):
     dtype = torch.float16 if T % 2 else torch.bfloat16
     wg, wu = (weight(F, D, group, dtype, T == 2, seed=i + F) for i in range(2))
