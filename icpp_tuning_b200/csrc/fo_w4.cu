@@ -4,20 +4,20 @@
 // Bound by the weights' bytes, and close behind by issue: a SM has to open about 46 weights
 // a cycle to keep up with HBM.  So
 //   * a warp streams 32 rows (16 and their 16 partners of a gated pair) and its tokens' x in
-//     steps of 128 k, by 16-byte cp.async into a ring it keeps for itself, and asks for a
-//     step's scales one step ahead: no block-wide barrier in the loop, and no load whose
+//     steps of 128 k, by 16-byte cp.async into a ring it keeps for itself, and asks for
+//     scales a batch of steps ahead: no block-wide barrier in the loop, and no load whose
 //     latency the loop sees;
 //   * one ldmatrix hands every lane the 32-bit words (8 weights each) of a 32-k group: of
 //     weight row lane / 4, word lane % 4 -- the fragment layout of the m16n8 MMAs when the k
 //     order inside a group is that of the words.  The order is free as long as both operands
 //     share it.
-// A token or a few times large weights (fo_w4i_kernel): the MMA is m16n8k32 on 8-bit integers: a word opens into two
-// fragment registers by one shift and two masks, where 16-bit operands take three shifts and
-// four masks and half the k an MMA.  x becomes integers first (fo_w4_digits_kernel): each
-// token's 128 k's of a step as fixed point of 23 bits, relative to the power of two below
+// A token or a few times large weights (fo_w4i_kernel): the MMA is m16n8k32 on 8-bit integers.
+// A word opens into two fragment registers by one shift and two masks, where 16-bit operands
+// take three shifts and four masks and half the k an MMA.  x becomes integers first
+// (fo_w4_digits_kernel): each token's 128 k's of a step as fixed point of 23 bits, relative to the power of two below
 // their largest magnitude, in three 8-bit digits, which are three columns of the MMA.  A
 // group's integer sum is exact, and so are 16-bit values within 2^11 of the step's largest; a
-// smaller one is off by 2^-22 of that power at most, no more than a fp32 sum loses.
+// smaller one is off by 2^-22 of that power at most, about what a fp32 sum loses.
 // All else (fo_w4_kernel) takes m16n8k16 on 16-bit floats: a word's nibbles pair as (0,4),
 // (1,5), (2,6), (3,7), x to match; in fp16 the bits of q alone are the subnormal q 2^-24,
 // exact, and the scale takes 2^24 back; in bf16 the bits of 128 + q (its subnormals would
@@ -32,7 +32,7 @@
 // weights and scales) 30.6 us with its digits' kernels (16-bit operands: 42.1); 16384 x 4096
 // product 10.8 us; 8 tokens, block 44.9 us; 5 tokens, fp16, groups of 32 with zeros, 51 us (120
 // MB).  That last form is bound by the latencies of a step's chain (copies, table, MMAs, sums)
-// at 14 warps a SM: its integer pipe is busy 48% of the time, issue 41%.  Short products are
+// at 14 warps a SM: its integer pipe is busy 47% of the time, issue 39%.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
 // 5.1 us for 8.7 MB).
 #include "fo_host.cuh"
