@@ -834,6 +834,9 @@ int check(const FoBlockNormDesc* d, bool bwd) {
   if (d->w_post == nullptr && d->b_post != nullptr) return host_fail(FO_EINVAL, "b_post without w_post");
   if (d->norm == FO_NORM_RMS && (d->b_post != nullptr || d->b_pre != nullptr))
     return host_fail(FO_EINVAL, "the rms norm has no bias");
+  if (bwd && d->norm == FO_NORM_RMS && (d->db_pre != nullptr || d->db_post != nullptr))
+    return host_fail(FO_EINVAL, "the rms norm has no bias: db_pre and db_post must be null");
+  if (bwd && d->w_post == nullptr && d->db_post != nullptr) return host_fail(FO_EINVAL, "db_post without w_post");
   if (d->gate_rows < 0 || (d->gate_rows == 0) != (d->gate == nullptr))
     return host_fail(FO_EINVAL, "gate_rows must be 0 without a gate and >= 1 with one");
   if (d->gate_rows > 0 && d->T % d->gate_rows != 0)

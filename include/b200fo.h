@@ -186,8 +186,9 @@ size_t fo_conv2d_workspace_size(const FoConvDesc* desc, const FoTileCfg* cfg);
  * gate: NULL (gate_rows 0) or [gate_rows, D] with row stride ldgate, each row shared by
  * T / gate_rows consecutive rows.  Parameters and their gradients are of vec_dtype; biases
  * (may be NULL) belong to FO_NORM_LAYER.  Backward reads y, r, dr (may be NULL: zero) and
- * dz and writes dy, dx, dw_pre, dw_post (with w_post), db_pre and db_post (where not NULL)
- * and dgate ([gate_rows, D], contiguous).  Sums over rows run in a fixed order.
+ * dz and writes dy, dx, dw_pre, dw_post (with w_post), db_pre and db_post (where not NULL:
+ * FO_NORM_LAYER only, db_post only with w_post) and dgate ([gate_rows, D], contiguous).  Sums
+ * over rows run in a fixed order.
  * D <= 16384 forward, 8192 backward (FO_EUNSUPPORTED above). */
 typedef struct FoBlockNormDesc {
   int64_t T, D;
