@@ -810,6 +810,7 @@ Shape shape_of(bool bf, bool v8, int D) {
 }
 
 constexpr int kMaxFwd = 16384, kMaxBwd = 8192;
+constexpr int64_t kMaxRows = 1ll << 30;  // rows ahead stay in 31 bits
 
 int esize(int dt) { return dt == FO_DT_F32 ? 4 : 2; }
 
@@ -826,7 +827,7 @@ bool vectors(const FoBlockNormDesc* d, bool bwd) {
 int check(const FoBlockNormDesc* d, bool bwd) {
   if (d == nullptr) return host_fail(FO_EINVAL, "null descriptor");
   if (d->T < 0 || d->D < 0) return host_fail(FO_EINVAL, "negative problem size");
-  if (d->T > 1ll << 30) return host_fail(FO_EINVAL, "T = %lld exceeds 2^30", static_cast<long long>(d->T));  // rows ahead stay in 31 bits
+  if (d->T > kMaxRows) return host_fail(FO_EINVAL, "T = %lld exceeds 2^30", static_cast<long long>(d->T));
   if (d->dtype != FO_DT_F16 && d->dtype != FO_DT_BF16) return host_fail(FO_EINVAL, "dtype must be FO_DT_F16 or FO_DT_BF16");
   if (d->vec_dtype < FO_DT_F16 || d->vec_dtype > FO_DT_F32) return host_fail(FO_EINVAL, "bad vec_dtype %d", d->vec_dtype);
   if (d->norm != FO_NORM_RMS && d->norm != FO_NORM_LAYER) return host_fail(FO_EINVAL, "norm must be FO_NORM_RMS or FO_NORM_LAYER");
@@ -924,7 +925,9 @@ extern "C" int fo_block_norm(const FoBlockNormDesc* d, void* stream) {
 }
 
 extern "C" size_t fo_block_norm_backward_workspace_size(const FoBlockNormDesc* d) {
-  if (d == nullptr || d->T <= 0 || d->D <= 0 || d->gate_rows < 0) return 0;
+  // sizes that the entry refuses ask for nothing (and may not fit the plan's integers)
+  if (d == nullptr || d->T <= 0 || d->T > fo::kMaxRows || d->D <= 0 || d->D > fo::kMaxBwd || d->gate_rows < 0) return 0;
+  if (d->gate_rows > 0 && d->T % d->gate_rows != 0) return 0;
   return fo::bwd_plan(d).bytes;
 }
 

@@ -1,11 +1,16 @@
 """What the decoder-block operators promise at their C entries and in their autograd functions,
 without a GPU."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
 from icpp_tuning_b200 import _native as N
 from test_block_abi import A, _norm
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 @pytest.mark.parametrize("T", [0, 4])
@@ -17,3 +22,20 @@ def test_norm_backward_refuses_gradients_of_absent_biases(kw, msg, T):
     d = _norm(T=T, workspace=A, workspace_bytes=1 << 30, **kw)
     assert N.lib().fo_block_norm_backward(ctypes.byref(d), None) == N.FO_EINVAL
     assert msg in N.last_error()
+
+
+SIZE_QUERY = """
+import ctypes
+from icpp_tuning_b200 import _native as N
+d = N.FoBlockNormDesc()
+d.T, d.D, d.gate_rows, d.norm = {T}, 64, {rows}, N.FO_NORM_LAYER
+print(N.lib().fo_block_norm_backward_workspace_size(ctypes.byref(d)))
+"""
+
+
+@pytest.mark.parametrize("T,rows", [(1 << 32, 1 << 32), (4, 1 << 32), (4, 3), (4, 8), (1 << 31, 1), (4, -1), (0, 0)])
+def test_norm_workspace_size_of_what_the_entry_refuses_is_zero(T, rows):
+    # in a process of its own: a division by zero would end it
+    r = subprocess.run([sys.executable, "-c", SIZE_QUERY.format(T=T, rows=rows)], capture_output=True, text=True, cwd=ROOT, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert int(r.stdout) == 0
