@@ -86,6 +86,14 @@ def _matrix(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     return like.new_empty((rows, (cols + 7) // 8 * 8))[:, :cols]
 
 
+def aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a copy of it, as the gated block takes a matrix: unit column stride, rows that
+    start on 16-byte boundaries (a row stride that is a multiple of 8 elements)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return _matrix(*t.shape, t).copy_(t)
+
+
 def _ffn_desc(x, w_gate, w_up, w_down, act, b_layout, others) -> N.FoGatedFfnDesc:
     code = GATE_ACTS.get(act)
     if code is None:

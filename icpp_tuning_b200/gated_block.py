@@ -29,7 +29,7 @@ class GatedFFN(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return (*block.gated_ffn_backward(dy.contiguous(), *ctx.saved_tensors, act=ctx.act, b_layout=ctx.b_layout), None, None)
+        return (*block.gated_ffn_backward(block.aligned_rows(dy), *ctx.saved_tensors, act=ctx.act, b_layout=ctx.b_layout), None, None)
 
 
 class BlockNorm(torch.autograd.Function):

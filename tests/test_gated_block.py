@@ -1,0 +1,60 @@
+"""The autograd functions of gated_block without a GPU: the operators are stand-ins on CPU
+tensors that hold their callers to the real ones' argument rules."""
+import pytest
+import torch
+
+from icpp_tuning_b200 import block, gated_block
+
+
+def _rows(*ts):
+    for t in ts:
+        assert t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0, (t.shape, t.stride())
+
+
+def _ffn(x, w_gate, w_up, w_down, *, act, b_layout, save):
+    assert act == "relu" and b_layout == "nk" and save
+    _rows(x, w_gate, w_up, w_down)
+    y, g, u = (block._matrix(x.shape[0], n, x) for n in (w_down.shape[0], w_gate.shape[0], w_gate.shape[0]))
+    g.copy_(x @ w_gate.t()), u.copy_(x @ w_up.t())
+    y.copy_((g.relu() * u) @ w_down.t())
+    return y, g, u
+
+
+def _ffn_backward(dy, x, w_gate, w_up, w_down, g, u, *, act, b_layout):
+    _rows(dy, x, w_gate, w_up, w_down, g, u)
+    dh, a = dy @ w_down, g.relu()
+    dg, du = dh * u * (g > 0), dh * a
+    return dg @ w_gate + du @ w_up, dg.t() @ x, du.t() @ x, dy.t() @ (a * u)
+
+
+@pytest.fixture
+def operators(monkeypatch):
+    monkeypatch.setattr(block, "gated_ffn", _ffn)
+    monkeypatch.setattr(block, "gated_ffn_backward", _ffn_backward)
+
+
+def _ffn_inputs(T=5, D=16, F=24, N=64):
+    g = torch.Generator().manual_seed(N)
+    return [(torch.randn(*s, generator=g) * 0.5).requires_grad_() for s in ((T, D), (F, D), (F, D), (N, F))]
+
+
+@pytest.mark.parametrize("N", [8, 64, 100, 3])
+@pytest.mark.parametrize("how", ["plain", "rows", "transposed", "broadcast", "sliced"])
+def test_gated_ffn_passes_any_gradient_on(operators, N, how):
+    """dy as autograd may bring it, at output widths that are no multiple of 8 too."""
+    args = _ffn_inputs(N=N)
+    y = gated_block.GatedFFN.apply(*args, "relu", "nk")
+    dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(1))
+    if how == "rows":  # as y lies
+        dy = block._matrix(*y.shape, y).copy_(dy)
+    if how == "transposed":
+        dy = dy.t().contiguous().t()
+    if how == "broadcast":
+        dy = torch.ones(()).expand(y.shape)
+    if how == "sliced":
+        dy = torch.cat((dy, dy), 1)[:, 1:N + 1]
+    got = torch.autograd.grad(y, args, dy)
+    ref = [t.detach().clone().requires_grad_() for t in args]
+    want = torch.autograd.grad(((ref[0] @ ref[1].t()).relu() * (ref[0] @ ref[2].t())) @ ref[3].t(), ref, dy)
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b)
