@@ -17,8 +17,21 @@ import torch
 from . import block
 
 
+class _FirstDerivatives(torch.autograd.Function):
+    """Runs a backward pass.  Under create_graph its results depend on every tensor that it
+    was given, and differentiating them raises: the operators have no second derivatives."""
+
+    @staticmethod
+    def forward(ctx, run, *tensors):
+        return run(*tensors)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the decoder-block operators have first derivatives only")
+
+
 class GatedFFN(torch.autograd.Function):
-    """y = (act(x Wg) * (x Wu)) Wd with its gradients; keeps x and the two products."""
+    """y = (act(x Wg) * (x Wu)) Wd with its first derivatives; keeps x and the two products."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, b_layout):
@@ -29,11 +42,14 @@ class GatedFFN(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return (*block.gated_ffn_backward(block.aligned_rows(dy), *ctx.saved_tensors, act=ctx.act, b_layout=ctx.b_layout), None, None)
+        def run(dy, *saved):
+            return block.gated_ffn_backward(block.aligned_rows(dy), *saved, act=ctx.act, b_layout=ctx.b_layout)
+
+        return (*_FirstDerivatives.apply(run, dy, *ctx.saved_tensors), None, None)
 
 
 class BlockNorm(torch.autograd.Function):
-    """(r, z) of `block.block_norm` with their gradients; keeps y and r."""
+    """(r, z) of `block.block_norm` with their first derivatives; keeps y and r."""
 
     @staticmethod
     def forward(ctx, y, x, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps):
@@ -45,11 +61,13 @@ class BlockNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dr, dz):
-        y, r, w_post, w_pre, b_post, b_pre, gate = ctx.saved_tensors
-        dz = torch.zeros_like(r) if dz is None else dz.contiguous()
-        d = block.block_norm_backward(None if dr is None else dr.contiguous(), dz, y, r, w_post, w_pre, b_post=b_post, b_pre=b_pre,
-                                      gate=gate, **ctx.kw)
-        return (d["dy"], d["dx"], d.get("dw_post"), d["dw_pre"], d.get("db_post"), d.get("db_pre"), d.get("dgate"), None, None, None)
+        def run(dr, dz, y, r, w_post, w_pre, b_post, b_pre, gate):
+            dz = torch.zeros_like(r) if dz is None else dz.contiguous()
+            d = block.block_norm_backward(None if dr is None else dr.contiguous(), dz, y, r, w_post, w_pre, b_post=b_post, b_pre=b_pre,
+                                          gate=gate, **ctx.kw)
+            return tuple(d.get(k) for k in ("dy", "dx", "dw_post", "dw_pre", "db_post", "db_pre", "dgate"))
+
+        return (*_FirstDerivatives.apply(run, dr, dz, *ctx.saved_tensors), None, None, None)
 
 
 def make_weights(layers: int, dim: int, inner: int, dtype=torch.bfloat16, device="cuda", seed: int = 0) -> List[Dict[str, torch.Tensor]]:

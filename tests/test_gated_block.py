@@ -58,3 +58,42 @@ def test_gated_ffn_passes_any_gradient_on(operators, N, how):
     want = torch.autograd.grad(((ref[0] @ ref[1].t()).relu() * (ref[0] @ ref[2].t())) @ ref[3].t(), ref, dy)
     for a, b in zip(got, want):
         torch.testing.assert_close(a, b)
+
+
+def _norm(y, x, w_post, w_pre, *, b_post, b_pre, gate, residual_scale, norm, eps):
+    assert w_post is None and gate is None and b_pre is None and norm == "rms"
+    r = residual_scale * x + y
+    return r, r * torch.rsqrt((r * r).mean(1, keepdim=True) + eps) * w_pre
+
+
+def _norm_backward(dr, dz, y, r, w_post, w_pre, *, b_post, b_pre, gate, residual_scale, norm, eps):
+    rho = torch.rsqrt((r * r).mean(1, keepdim=True) + eps)
+    c = dz * w_pre
+    t = rho * (c - r * rho * (c * r * rho).mean(1, keepdim=True)) + (0 if dr is None else dr)
+    return {"dy": t, "dx": residual_scale * t, "dw_pre": (dz * r * rho).sum(0)}
+
+
+@pytest.mark.parametrize("into", [0, 1, 3])
+def test_second_derivatives_raise(operators, monkeypatch, into):
+    """The operators have none: a loss with a gradient in it is an error, whatever it is
+    differentiated by, not a sum that lacks that term."""
+    monkeypatch.setattr(block, "block_norm", _norm)
+    monkeypatch.setattr(block, "block_norm_backward", _norm_backward)
+    args = _ffn_inputs()
+    y = gated_block.GatedFFN.apply(*args, "relu", "nk")
+    (dx,) = torch.autograd.grad(y.sum(), args[:1], create_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(y.square().sum() + dx.square().sum(), args[into])
+    x, w = torch.randn(4, 8).requires_grad_(), torch.ones(8).requires_grad_()
+    r, z = gated_block.BlockNorm.apply(x, x, None, w, None, None, None, 0.5, "rms", 1e-5)
+    (dx,) = torch.autograd.grad(z.square().sum() + r.sum(), (x,), create_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(r.sum() + dx.square().sum(), w if into else x)
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        (r.sum() + dx.square().sum()).backward()
+
+
+def test_gradients_without_a_graph_carry_none(operators):
+    args = _ffn_inputs()
+    got = torch.autograd.grad(gated_block.GatedFFN.apply(*args, "relu", "nk").square().sum(), args)
+    assert not any(t.requires_grad for t in got)
