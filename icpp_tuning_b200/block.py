@@ -24,6 +24,7 @@ from .fused import _require_cuda, _vec, dtype_code
 GATE_ACTS = {"silu": N.FO_GATE_SILU, "gelu_tanh": N.FO_GATE_GELU_TANH, "gelu_erf": N.FO_GATE_GELU_ERF,
              "relu": N.FO_GATE_RELU}
 NORMS = {"rms": N.FO_NORM_RMS, "layer": N.FO_NORM_LAYER}
+MAX_NORM_BACKWARD = 8192  # columns of a row in block_norm_backward (block_norm: 16384)
 
 
 def _run(dev: torch.device, fn, desc) -> None:

@@ -51,6 +51,13 @@ class GatedFFN(torch.autograd.Function):
 class BlockNorm(torch.autograd.Function):
     """(r, z) of `block.block_norm` with their first derivatives; keeps y and r."""
 
+    @classmethod
+    def apply(cls, y, *rest):
+        if y.shape[1] > block.MAX_NORM_BACKWARD and torch.is_grad_enabled() and any(
+                isinstance(t, torch.Tensor) and t.requires_grad for t in (y, *rest)):
+            raise ValueError(f"the norms' backward pass takes rows of at most {block.MAX_NORM_BACKWARD} columns, got {y.shape[1]}")
+        return super().apply(y, *rest)
+
     @staticmethod
     def forward(ctx, y, x, w_post, w_pre, b_post, b_pre, gate, residual_scale, norm, eps):
         ctx.kw = dict(residual_scale=residual_scale, norm=norm, eps=eps)

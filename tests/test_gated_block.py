@@ -97,3 +97,16 @@ def test_gradients_without_a_graph_carry_none(operators):
     args = _ffn_inputs()
     got = torch.autograd.grad(gated_block.GatedFFN.apply(*args, "relu", "nk").square().sum(), args)
     assert not any(t.requires_grad for t in got)
+
+
+def test_widths_without_a_backward_pass_are_refused_forward(monkeypatch):
+    """The backward kernels hold rows of at most 8192 columns, the forward ones 16384."""
+    monkeypatch.setattr(block, "block_norm", _norm)
+    x, w = torch.randn(2, 8193), torch.ones(8193)
+    call = lambda: gated_block.BlockNorm.apply(x, x, None, w, None, None, None, 0.5, "rms", 1e-5)  # noqa: E731
+    want = call()
+    w.requires_grad_()
+    with pytest.raises(ValueError, match="8192"):
+        call()
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(call(), want))
