@@ -49,13 +49,14 @@ def _cuda(*ts: Optional[torch.Tensor]) -> torch.device:
 
 
 def _ld(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
-    """Row stride of a 2-D operand that must be [rows, cols] with unit column stride."""
+    """Row stride of a 2-D operand that must be [rows, cols] with unit column stride.  A single
+    row may carry any: it counts as one that every operator takes."""
     if t.shape != (rows, cols):
         raise ValueError(f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
     st = t.stride()
     if st[1] != 1 and cols != 1:
         raise ValueError(f"{name} must be a 2-D tensor with unit column stride")
-    return st[0]
+    return st[0] if rows != 1 else (cols + 15) // 16 * 16
 
 
 def _shape2(t: torch.Tensor, name: str) -> Tuple[int, int]:
@@ -75,7 +76,7 @@ def _sixteen_bit(dt: torch.dtype, name: str) -> int:
 def _new(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """An uninitialised contiguous [rows, cols] of like's type."""
     if like.shape == (rows, cols) and like.is_contiguous():
-        return torch.empty_like(like)  # the cheapest call
+        return torch.empty_like(like, memory_format=torch.contiguous_format)  # the cheapest call
     return like.new_empty((rows, cols))
 
 

@@ -6,8 +6,10 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 from icpp_tuning_b200 import _native as N
+from icpp_tuning_b200 import block
 from test_block_abi import A, _norm
 
 ROOT = Path(__file__).resolve().parents[1]
@@ -39,3 +41,14 @@ def test_norm_workspace_size_of_what_the_entry_refuses_is_zero(T, rows):
     r = subprocess.run([sys.executable, "-c", SIZE_QUERY.format(T=T, rows=rows)], capture_output=True, text=True, cwd=ROOT, timeout=120)
     assert r.returncode == 0, r.stderr
     assert int(r.stdout) == 0
+
+
+@pytest.mark.parametrize("cols", [1, 8, 60, 64])
+def test_the_row_stride_of_a_single_row_does_not_count(cols):
+    """A matrix of one row may carry any row stride (PyTorch calls it contiguous all the same)."""
+    for one in (torch.zeros(cols, 1).t(), torch.zeros(3 * cols)[None, :cols], torch.zeros(1, cols)):
+        ld = block._ld(one, 1, cols, "x")
+        assert ld % 16 == 0 and ld >= cols
+        assert block._matrix(1, cols, one).stride(0) % 8 == 0 and block._new(1, cols, one).stride(0) == cols
+    two = torch.zeros(2, cols + 3)[:, :cols]
+    assert block._ld(two, 2, cols, "x") == cols + 3

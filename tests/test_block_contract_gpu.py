@@ -1,0 +1,36 @@
+"""What the decoder-block operators accept beyond plain contiguous matrices."""
+import pytest
+import torch
+
+from gpu_util import gen, status_clean
+
+from icpp_tuning_b200 import block
+from test_w4_gpu import gpu, weight
+
+pytestmark = pytest.mark.gpu
+
+
+def odd(t):
+    """The one-row matrix `t` with a row stride of 1: contiguous, as PyTorch counts."""
+    out = t.as_strided(t.shape, (1, 1))
+    assert out.shape[0] == 1 and out.is_contiguous()
+    return out
+
+
+def test_one_row_of_any_stride():
+    D, F, dt = 64, 128, torch.bfloat16
+    x, y = (torch.randn(1, D, generator=gen(i)).to(dt).cuda() for i in range(2))
+    w = [(torch.randn(*s, generator=gen(9)) * 0.1).to(dt).cuda() for s in ((F, D), (F, D), (D, F))]
+    v = torch.ones(D, dtype=dt, device="cuda")
+    saved = block.gated_ffn(x, *w, b_layout="nk", save=True)
+    same = lambda a, b: all(torch.equal(p, q) for p, q in zip(a, b))  # noqa: E731
+    assert same(saved, block.gated_ffn(odd(x), *w, b_layout="nk", save=True))
+    back = block.gated_ffn_backward(y, x, *w, *saved[1:], b_layout="nk")
+    assert same(back, block.gated_ffn_backward(odd(y), odd(x), *w, *map(odd, saved[1:]), b_layout="nk"))
+    assert same(block.block_norm(y, x, v, v), block.block_norm(odd(y), odd(x), v, v))
+    a, b = block.block_norm_backward(y, x, y, x, v, v), block.block_norm_backward(odd(y), odd(x), odd(y), odd(x), v, v)
+    assert same(a.values(), b.values())
+    q, one = gpu(weight(96, D, 32, dt, True, seed=1)), gpu(weight(1, D, 32, dt, True, seed=2))
+    assert torch.equal(block.matvec_w4(x, q), block.matvec_w4(odd(x), q))
+    assert torch.equal(block.matvec_w4(x, one), block.matvec_w4(x, one._replace(q=odd(one.q), scales=odd(one.scales), zeros=odd(one.zeros))))
+    status_clean()
