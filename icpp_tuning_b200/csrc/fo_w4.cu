@@ -422,7 +422,7 @@ constexpr int kPlanes = 3;
 // A step's record: 4 groups x 8 NT columns x 32 digits, then every column's sums over the
 // step's ENT blocks, then its scale.  Column 3 t + p is digit p of token t, the first the
 // highest; a group's digits are ordered like the fragments: for each word the k of its even
-// nibbles, then of its odd ones.  Sums are scaled already.
+// nibbles, then of its odd ones.  Sums are of the digits, whole numbers.
 template <int NT, int GS>
 struct W4iShape {
   static constexpr int kEnt = 4 / GS;
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(256) fo_w4_digits_kernel(const __grid_constant
     float* tail = reinterpret_cast<float*>(rec + 1024 * NT) + col;
     // the digit's unit; it may be subnormal, and its integers still scale exactly
     const float unit_q = fine ? ldexpf(1.f, 8 * (kPlanes - 1 - q) - up) : __int_as_float(0x7FC00000);
-    if ((l & (4 * GS - 1)) == 0) tail[l / (4 * GS) * (8 * NT)] = static_cast<float>(sum[q]) * unit_q;
+    if ((l & (4 * GS - 1)) == 0) tail[l / (4 * GS) * (8 * NT)] = static_cast<float>(sum[q]);
     if (l == 0) tail[S::kEnt * 8 * NT] = unit_q;
   }
 }
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
 #pragma unroll
     for (int e = 0; e < ENT; ++e) {
       const float v = scales.scale(e), z = scales.zero(e);
-      *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v, -v * z);
+      *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v, -z);
     }
     __syncwarp();
     weights(i + S::kStages - 1);
@@ -656,8 +656,9 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
           for (int nt = 0; nt < NT; ++nt) {
             const Two d01 = add2(two(__int_as_float(dot[m][nt][0]), __int_as_float(dot[m][nt][1])), none2);
             const Two d23 = add2(two(__int_as_float(dot[m][nt][2]), __int_as_float(dot[m][nt][3])), none2);
-            const float2 u = both(fma2(sx[nt], two(lo.y), fma2(d01, mul2(two(lo.x), unit[nt]), two(acc[m][nt][0], acc[m][nt][1]))));
-            const float2 v = both(fma2(sx[nt], two(hi.y), fma2(d23, mul2(two(hi.x), unit[nt]), two(acc[m][nt][2], acc[m][nt][3]))));
+            // sums of (q - zero) digit: whole numbers below 2^23, exact
+            const float2 u = both(fma2(fma2(sx[nt], two(lo.y), d01), mul2(two(lo.x), unit[nt]), two(acc[m][nt][0], acc[m][nt][1])));
+            const float2 v = both(fma2(fma2(sx[nt], two(hi.y), d23), mul2(two(hi.x), unit[nt]), two(acc[m][nt][2], acc[m][nt][3])));
             acc[m][nt][0] = u.x, acc[m][nt][1] = u.y, acc[m][nt][2] = v.x, acc[m][nt][3] = v.y;
           }
         }
