@@ -19,22 +19,25 @@
 // group's integer sum is exact, and so are 16-bit values within 2^11 of the step's largest; a
 // smaller one is off by 2^-22 of that power at most, about what a fp32 sum loses.
 // All else (fo_w4_kernel) takes m16n8k16 on 16-bit floats: a word's nibbles pair as (0,4),
-// (1,5), (2,6), (3,7), x to match; in fp16 the bits of q alone are the subnormal q 2^-24,
-// exact, and the scale takes 2^24 back; in bf16 the bits of 128 + q (its subnormals would
-// leave fp32's range).
-// In both an offset of the opened weights, and their zero, leave by a product with sum(x) of
-// the group.  W of a CTA's 8 warps share a tile of rows and split its K (and, for few tiles,
-// the CTAs of a cluster): as many as fill the SMs with warps, so that each still walks many
-// steps.  Partial sums meet in shared memory (distributed across the cluster) and are added in
-// a fixed order.
+// (1,5), (2,6), (3,7), x to match.  A mask and a second constant make each pair the last bits of
+// a number whose difference from one of the row's, by its zero, is q - zero, exact: a product is
+// x (q - zero) itself, for an infinite x too.  (Opened without the zero, which then left by a
+// product with the group's sum(x), a pair took one operation less and a word two MMAs more:
+// 4096 x 16384 block, groups of 32 with zeros, 5 tokens fp16 51.0 us against 52.3 now, bf16 57.3
+// against 54.8, 32 tokens 149 against 132; and any infinite x gave NaN.)  The digits' zero
+// leaves by their sum: both are whole numbers, exact.
+// W of a CTA's 8 warps share a tile of rows and split its K (and, for few tiles, the CTAs of a
+// cluster): as many as fill the SMs with warps, so that each still walks many steps.  Partial
+// sums meet in shared memory (distributed across the cluster) and are added in a fixed order.
 //
 // Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
-// weights and scales) 30.6 us with its digits' kernels (16-bit operands: 42.1); 16384 x 4096
-// product 10.8 us; 8 tokens, block 44.9 us; 5 tokens, fp16, groups of 32 with zeros, 51 us (120
+// weights and scales) 30 us with its digits' kernels (16-bit operands: 42.1); 16384 x 4096
+// product 11.3 us; 8 tokens, block 44.2 us; 5 tokens, fp16, groups of 32 with zeros, 52 us (120
 // MB).  That last form is bound by the latencies of a step's chain (copies, table, MMAs, sums)
 // at 14 warps a SM: its integer pipe is busy 47% of the time, issue 39%.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
-// 5.1 us for 8.7 MB).
+// 5.6 us for 8.7 MB; 5.3 in fp16).  More tokens cost MMAs, 32 of them as much as 4 times
+// the bytes: block 64 us at 9 tokens, 122 at 32.
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"
@@ -84,6 +87,43 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
   }
 }
 
+// A word's nibbles as kUnit (q - zero), in 16-bit pairs (0,4), (1,5), (2,6), (3,7).  Exact for
+// any zero of 8 bits: all that appears is a whole number of kUnits that the type holds.
+template <int DT>
+struct W4Open;
+template <>
+struct W4Open<DT_BF16> {  // the nibble's complement in the last bits of 128: (143 - zero) - (143 - q)
+  // in units that keep a step's sum, 128 (q - zero) x, below x: any finite x stays in range
+  static constexpr float kUnit = 1.f / 2048;
+  uint32_t top;
+  __device__ __forceinline__ static uint32_t off(uint32_t zero) {
+    const float v = (143.f - static_cast<float>(zero)) * kUnit;
+    return pack2<DT_BF16>(v, v);
+  }
+  __device__ __forceinline__ void set(uint32_t v) { top = v; }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v[e]) : "r"(top), "r"(((w >> (4 * e)) & 0x000F000Fu) ^ 0x3D8F3D8Fu));
+  }
+};
+template <>
+struct W4Open<DT_F16> {  // a byte's lower nibble in the last bits of 1024, its higher one, as it lies, in those of 64
+  static constexpr float kUnit = 1.f;
+  uint32_t low, high;    // -(1024 + zero), -(64 + zero)
+  __device__ __forceinline__ static uint32_t off(uint32_t zero) { return 0xE400E400u + zero * 0x10001u; }
+  __device__ __forceinline__ void set(uint32_t v) {
+    low = v;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(high) : "r"(low), "r"(0x63806380u));  // 960
+  }
+  __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
+#pragma unroll
+    for (int b = 0; b < 2; ++b, w >>= 8) {
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(v[2 * b]) : "r"((w & 0x000F000Fu) | 0x64006400u), "r"(low));
+      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(v[2 * b + 1]) : "r"((w & 0x00F000F0u) | 0x54005400u), "r"(high));
+    }
+  }
+};
+
 // Four 8 x 16-byte blocks: lane l gives the address of row l % 8 of block l / 8 and
 // gets word l % 4 of row l / 4 of each block.
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&w)[4]) {
@@ -102,7 +142,6 @@ constexpr int kWarps = 8;
 
 constexpr int kRows = 32;                  // weight rows of a tile: two 16-row MMA blocks
 constexpr int kStepW = kRows * 64;         // their bytes in a step
-constexpr int kTable = kRows * 40;         // a step's (scale, -scale * offset) pairs, up to 4 a row
 
 // Which steps a warp takes: batches of 2^lg steps, dealt to the warps in turn, so that a row's
 // scales of a whole batch come by one load (a load of every lane's own row costs the SM 32 tag
@@ -189,7 +228,7 @@ struct W4Scales {
   __device__ __forceinline__ float scale(int e) const {
     return unpack2<DT>(static_cast<uint32_t>(s[0] >> (16 * e)) & 0xFFFFu).x;
   }
-  __device__ __forceinline__ float zero(int e) const { return static_cast<float>(static_cast<uint32_t>(z[0] >> (8 * e)) & 255u); }
+  __device__ __forceinline__ uint32_t zero(int e) const { return static_cast<uint32_t>(z[0] >> (8 * e)) & 255u; }
   __device__ __forceinline__ void next() {  // to the next step of the batch
     if constexpr (ENT == 4) {
 #pragma unroll
@@ -209,6 +248,8 @@ template <int NT>
 struct W4Shape {
   static constexpr int kStep = kStepW + 2048 * NT;
   static constexpr int kCtas = NT <= 2 ? 2 : 1;    // a SM
+  static constexpr int kTableRow = 48;             // keeps 16-byte stores and 8-byte reads of 8 rows off each other's banks
+  static constexpr int kTable = kRows * kTableRow; // a step's (scale, what takes the zero off) pairs, up to 4 a row
   static constexpr int kBudget = (NT <= 2 ? 110 : 200) * 1024 / kWarps - kTable;
   static constexpr int kStages = kBudget / kStep < 6 ? kBudget / kStep : 6;
   static constexpr int kRed = kRows * 8 * NT * 4;  // one warp's sums: its idle ring at the end
@@ -225,10 +266,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   using S = W4Shape<NT>;
   constexpr int NA = JOINT ? NT / 2 : NT;                     // blocks of sums
   constexpr int ENT = 4 / GS, kOut = GATED ? 16 : 32;         // outputs of a tile
-  constexpr float kLeft = DT == DT_BF16 ? 128.f : 0.f;        // offset that stays in the opened weights
-  constexpr float kBack = DT == DT_BF16 ? 1.f : 16777216.f;   // what their scale lacks
-  constexpr uint32_t kMagic = DT == DT_BF16 ? 0x43004300u : 0u;
-  constexpr uint32_t kOne = DT == DT_BF16 ? 0x3F803F80u : 0x3C003C00u;
+  constexpr int kTableRow = S::kTableRow;
   extern __shared__ __align__(128) uint8_t smem_w4[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -245,7 +283,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
   const int mine = n0 < p.N ? turn.count : 0;
   uint8_t* const own = smem_w4 + warp * S::kWarp;
   const uint32_t ring = smem_u32(own);
-  uint8_t* const table = own + S::kWarp - kTable;
+  uint8_t* const table = own + S::kWarp - S::kTable;
 
   // Sources of this lane.  Rows past N repeat the last one: nothing of them is stored.  Row
   // block b: the gate's and the up weights' 16 rows, or rows 16 b of the one matrix.
@@ -298,26 +336,31 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
 
   float acc[2][NA][4] = {};
   const float none[4] = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
   // ldmatrix: lane l addresses row l % 8 of row block l / 8
   const uint32_t my_row = (lane >> 3) * 512u + (lane & 7) * 64u, my_rot = ((lane & 7) >> 1) & 3;
   const uint32_t my_x = kStepW + r * 256u, x_rot = (r & 1) << 2;
   uint32_t stage = ring;
   for (int i = 0; i < mine; ++i) {
-    cp_async_wait<S::kStages - 2>();
-    __syncwarp();  // other lanes' copies, and their reads of the slot and the table refilled next
+    __syncwarp();  // the other lanes have read the slot and the table that are refilled next
     const bool fresh_batch = (i & batch) == 0;
     if (fresh_batch) scales.turn();
+    uint32_t entry[2 * ENT];
 #pragma unroll
-    for (int e = 0; e < ENT; ++e) {
-      const float v = scales.scale(e), z = scales.zero(e);
-      *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v * kBack, -v * (kLeft + z));
+    for (int e = 0; e < ENT; ++e) entry[2 * e] = __float_as_uint(scales.scale(e) * (1.f / W4Open<DT>::kUnit)), entry[2 * e + 1] = W4Open<DT>::off(scales.zero(e));
+    if constexpr (ENT == 1) {
+      *reinterpret_cast<uint2*>(table + lane * kTableRow) = make_uint2(entry[0], entry[1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < ENT; e += 2)
+        *reinterpret_cast<uint4*>(table + lane * kTableRow + e * 8) = make_uint4(entry[2 * e], entry[2 * e + 1], entry[2 * e + 2], entry[2 * e + 3]);
     }
-    __syncwarp();
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();  // the other lanes' copies and table rows
     issue();
     if (fresh_batch && i + batch + 1 < mine) scales.ask(p, turn.at(i + batch + 1), p.lg);
     scales.next();
-    float dot[2][NA][4], sx[NA][4];
+    float dot[2][NA][4], by[2][2];  // by: the scales of rows r, r + 8 of both blocks
+    W4Open<DT> open[2][2];          // and what takes their zeros off
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t xb[NT][4];
@@ -332,17 +375,22 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
       ldsm4(stage + my_row + ((j ^ my_rot) << 4), w);
       const bool fresh = j % GS == 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_16816<DT>(sx[nt % NA], ones, xb[nt][0], xb[nt][1], fresh && nt < NA ? none : sx[nt % NA]);
-        mma_16816<DT>(sx[nt % NA], ones, xb[nt][2], xb[nt][3], sx[nt % NA]);
-      }
-#pragma unroll
       for (int m = 0; m < 2; ++m) {
+        if (fresh) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint2 v = *reinterpret_cast<const uint2*>(table + (m * 16 + h * 8 + r) * kTableRow + j / GS * 8);
+            by[m][h] = __uint_as_float(v.x), open[m][h].set(v.y);
+          }
+        }
         uint32_t a[2][4];  // {row r, row r + 8} x {pairs 0, 1}, {pairs 2, 3}
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[4];
+          open[m][h](w[2 * m + h], v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e >> 1][(e & 1) * 2 + h] = ((w[2 * m + h] >> (4 * e)) & 0x000F000Fu) | kMagic;
+          for (int e = 0; e < 4; ++e) a[e >> 1][(e & 1) * 2 + h] = v[e];
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mma_16816<DT>(dot[m][nt % NA], a[0], xb[nt][0], xb[nt][1], fresh && nt < NA ? none : dot[m][nt % NA]);
@@ -352,13 +400,10 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
       if ((j + 1) % GS == 0) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const float2 lo = *reinterpret_cast<const float2*>(table + (m * 16 + r) * 40 + j / GS * 8);
-          const float2 hi = *reinterpret_cast<const float2*>(table + (m * 16 + r + 8) * 40 + j / GS * 8);
 #pragma unroll
           for (int nt = 0; nt < NA; ++nt) {
-            const Two x01 = two(sx[nt][0], sx[nt][1]);
-            const float2 u = both(fma2(x01, two(lo.y), fma2(two(dot[m][nt][0], dot[m][nt][1]), two(lo.x), two(acc[m][nt][0], acc[m][nt][1]))));
-            const float2 v = both(fma2(x01, two(hi.y), fma2(two(dot[m][nt][2], dot[m][nt][3]), two(hi.x), two(acc[m][nt][2], acc[m][nt][3]))));
+            const float2 u = both(fma2(two(dot[m][nt][0], dot[m][nt][1]), two(by[m][0]), two(acc[m][nt][0], acc[m][nt][1])));
+            const float2 v = both(fma2(two(dot[m][nt][2], dot[m][nt][3]), two(by[m][1]), two(acc[m][nt][2], acc[m][nt][3])));
             acc[m][nt][0] = u.x, acc[m][nt][1] = u.y, acc[m][nt][2] = v.x, acc[m][nt][3] = v.y;
           }
         }
@@ -428,6 +473,7 @@ struct W4iShape {
   static constexpr int kEnt = 4 / GS;
   static constexpr int kRec = 1024 * NT + (kEnt + 1) * 32 * NT;
   static constexpr int kStep = kStepW + kRec;
+  static constexpr int kTable = kRows * 40;        // a step's (scale, -zero) pairs, up to 4 a row
   static constexpr int kBudget = 113 * 1024 / kWarps - kTable;  // two CTAs a SM
   static constexpr int kStages = kBudget / kStep < 6 ? kBudget / kStep : 6;
   static constexpr int kRed = kRows * 8 * NT * 4;
@@ -539,7 +585,7 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
   const int mine = n0 < p.N ? turn.count : 0;
   uint8_t* const own = smem_w4 + warp * S::kWarp;
   const uint32_t ring = smem_u32(own);
-  uint8_t* const table = own + S::kWarp - kTable;
+  uint8_t* const table = own + S::kWarp - S::kTable;
 
   const char* src[4];
 #pragma unroll
@@ -605,7 +651,7 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
     if (fresh_batch) scales.turn();
 #pragma unroll
     for (int e = 0; e < ENT; ++e) {
-      const float v = scales.scale(e), z = scales.zero(e);
+      const float v = scales.scale(e), z = static_cast<float>(scales.zero(e));
       *reinterpret_cast<float2*>(table + lane * 40 + e * 8) = make_float2(v, -z);
     }
     __syncwarp();
