@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kFewThreads) fo_few_kernel(const __grid_consta
       const float h = both(gate_act<ACT>(two(v))).x * w;
       const unsigned short hi = to16(h, p.bf16);
       *out = hi;
-      if (p.split) out[p.ldo] = to16(h - from16(hi, p.bf16), p.bf16);
+      if (p.split) out[p.ldo] = to16(low_part(h, from16(hi, p.bf16)), p.bf16);
     } else if constexpr (MODE == FEW_DGATE) {
       const float sg = from16(__ldg(static_cast<const unsigned short*>(p.sg) + t * p.ldsg + f), p.bf16);
       const float su = from16(__ldg(static_cast<const unsigned short*>(p.su) + t * p.ldsu + f), p.bf16);

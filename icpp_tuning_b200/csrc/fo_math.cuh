@@ -54,6 +54,13 @@ __device__ __forceinline__ uint32_t pack2(Two a) {
   return pack2<DT>(f.x, f.y);
 }
 
+// What 16 bits leave of v, high being its first part: nothing where that is not finite, so that
+// the parts of an infinity add up to it.
+__device__ __forceinline__ float low_part(float v, float high) {
+  const float rest = v - high;
+  return fabsf(rest) < __builtin_huge_valf() ? rest : 0.f;
+}
+
 // The gated activations and their derivatives, in forms whose error stays at fp32's: the
 // sigmoid ones take one exponential and one reciprocal a value (gelu_tanh(g) = g sigmoid(2 w),
 // w = sqrt(2 / pi) (g + 0.044715 g^3)), the erf one a reciprocal (erf by Abramowitz & Stegun

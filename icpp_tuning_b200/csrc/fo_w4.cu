@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(256, W4Shape<NT>::kCtas) fo_w4_kernel(const __
     const uint32_t hi = pack2<DT>(v, 0.f);
     unsigned short* out = static_cast<unsigned short*>(p.out) + (p.split ? 2 * row : row) * p.ldo + n;
     *out = static_cast<unsigned short>(hi);
-    if (p.split) out[p.ldo] = static_cast<unsigned short>(pack2<DT>(v - unpack2<DT>(hi).x, 0.f));
+    if (p.split) out[p.ldo] = static_cast<unsigned short>(pack2<DT>(low_part(v, unpack2<DT>(hi).x), 0.f));
   }
   if (Q > 1) cluster_sync();  // the others may still read this CTA's sums
 }

@@ -34,3 +34,22 @@ def test_one_row_of_any_stride():
     assert torch.equal(block.matvec_w4(x, q), block.matvec_w4(odd(x), q))
     assert torch.equal(block.matvec_w4(x, one), block.matvec_w4(x, one._replace(q=odd(one.q), scales=odd(one.scales), zeros=odd(one.zeros))))
     status_clean()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T", [1, 5, 32, 40])
+def test_an_infinity_between_the_products(T, dtype):
+    """h = inf stays an infinity on its way through the second product, in parts or whole."""
+    D, F = 64, 128
+    x = torch.rand(T, D, generator=gen(T)).to(dtype).cuda() + 0.5
+    x[0, 3] = float("inf")
+    w = [(torch.rand(F, D, generator=gen(i)).to(dtype).cuda() + 0.25) / 8 for i in range(3)]
+    y = block.gated_ffn(x, w[0], w[1], w[2].t().contiguous(), b_layout="nk")
+    assert (y[0] == float("inf")).all()
+    up = block.W4(torch.full((F, D // 2), 0x99, dtype=torch.uint8, device="cuda"), torch.full((F, 2), 2.0 ** -6, dtype=dtype, device="cuda"), None, 32)
+    down = block.W4(torch.full((D, F // 2), 0x99, dtype=torch.uint8, device="cuda"), torch.full((D, 4), 2.0 ** -6, dtype=dtype, device="cuda"), None, 32)
+    z = block.gated_ffn_w4(x, up, up, down)
+    assert (z[0] == float("inf")).all()
+    if T > 1:
+        assert y[1:].isfinite().all() and z[1:].isfinite().all()
+    status_clean()
