@@ -852,6 +852,9 @@ int check_weight(const FoW4* w, int64_t K, const char* name) {
   if (w->q == nullptr || w->scales == nullptr || !host_aligned16(w->q))
     return host_fail(FO_EINVAL, "%s: q and scales must be device pointers, q 16-byte aligned", name);
   if (w->group <= 0 || w->group % 32 != 0) return host_fail(FO_EINVAL, "%s: group must be a positive multiple of 32, got %d", name, w->group);
+  // a step's group comes from a 32-bit reciprocal, exact while steps * steps a group <= 2^32
+  if (w->group < K && K / 128 * (w->group / 128) > (1ll << 32))
+    return host_fail(FO_EUNSUPPORTED, "%s: K = %lld in groups of %d exceeds K * group = 2^46", name, static_cast<long long>(K), w->group);
   const int64_t groups = (K + w->group - 1) / w->group;
   if (w->ldq < K / 2 || w->ldq % 16 != 0)
     return host_fail(FO_EINVAL, "%s: ldq must be a multiple of 16 bytes and >= K / 2, got %lld", name, static_cast<long long>(w->ldq));

@@ -270,7 +270,8 @@ size_t fo_gated_ffn_workspace_size(const FoGatedFfnDesc* desc, int32_t backward)
 /* w[n, k] = scales[n, k / group] * (q[n, k] - zeros[n, k / group]).  q: two weights to a
  * byte, the lower nibble the even k, rows ldq bytes apart (a multiple of 16, 16-byte aligned
  * base); scales: dtype of x, rows lds apart; zeros: one byte each, rows ldz apart, or NULL
- * (every zero is 8).  group: a multiple of 32; the last group of a row may be short. */
+ * (every zero is 8).  group: a multiple of 32; the last group of a row may be short.  More
+ * than one group a row: K * group <= 2^46 (FO_EUNSUPPORTED above). */
 typedef struct FoW4 {
   const void* q;
   const void* scales;

@@ -10,7 +10,7 @@ import torch
 
 from icpp_tuning_b200 import _native as N
 from icpp_tuning_b200 import block
-from test_block_abi import A, _norm
+from test_block_abi import A, _matvec, _norm, _w4
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -52,3 +52,25 @@ def test_the_row_stride_of_a_single_row_does_not_count(cols):
         assert block._matrix(1, cols, one).stride(0) % 8 == 0 and block._new(1, cols, one).stride(0) == cols
     two = torch.zeros(2, cols + 3)[:, :cols]
     assert block._ld(two, 2, cols, "x") == cols + 3
+
+
+def test_w4_groups_longer_than_the_index_division_holds_are_refused():
+    """A step's group is found by a product with a 32-bit reciprocal, exact while steps x steps
+    a group stay within 2^32; one group for the whole row needs none."""
+    def call(K, group):
+        d = _matvec(_w4(ldq=K // 2, lds=K // 32, group=group), K=K, ldx=K, out=None)  # nothing can run
+        return N.lib().fo_matvec_w4(ctypes.byref(d), None)
+
+    K = 1 << 25
+    assert call(K, (1 << 21) + 128) == N.FO_EUNSUPPORTED and "group" in N.last_error()
+    for fine in (1 << 21, 128, K, 2 * K):
+        assert call(K, fine) == N.FO_EINVAL and "out" in N.last_error()
+    # the bound itself, on the integers of the kernel: the worst reciprocals of 2^32 / per
+    for per in (3, 7, 641, 6700417 % 65536, 40503, 65535, 16385):
+        rcp = -(-(1 << 32) // per)
+        last = (1 << 32) // per
+        at = sorted({i for q in (1, 2, 3, last // per, last // per - 1) for i in (q * per - 1, q * per, q * per + 1) if 0 <= i <= last})
+        assert all((i * rcp) >> 32 == i // per for i in at), per
+    per = (1 << 18) - 5  # and past it
+    rcp = -(-(1 << 32) // per)
+    assert any((i * rcp) >> 32 != i // per for i in range(per - 1, 1 << 20, per))
