@@ -44,7 +44,7 @@ struct NormParams {
   int vec_dtype, layer;
   float scale, eps;
   // work units: `chunks` to a gate group, its rows in turn; backward, the sums of unit u go to
-  // part[u][k][ldp] (k: dz rhat, t yhat, dz, t)
+  // part[u][k][ldp] (k: dz rhat, t yhat; in the LayerNorm form dz, t)
   int groups, chunks;
   int ldp;
   float* part;
@@ -626,7 +626,7 @@ struct BwdRow {
   }
   __device__ __forceinline__ void done(int u) {
     constexpr int RG = row_groups(W);
-    float* out = p.part + static_cast<long long>(u) * 4 * p.ldp;
+    float* out = p.part + static_cast<long long>(u) * kSums * p.ldp;
 #pragma unroll 1
     for (int g = 0; g < RG; ++g) {  // the row groups add up in turn, the last one writes
       if (g == static_cast<int>(threadIdx.y)) {
@@ -675,6 +675,7 @@ struct JoinParams {
   const void *w_post, *b_post, *gate;
   long long ldgate;
   int units, chunks, ldp, D, vec_dtype;
+  int sums;  // a unit: BwdRow's kSums
 };
 
 constexpr int kJoinSplit = 32;
@@ -704,8 +705,8 @@ __global__ void __launch_bounds__(8 * kJoinSplit) fo_norm_join_kernel(const Join
         const int u = u0 + i * kJoinSplit;
         q[i] = t[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (u < hi) {
-          q[i] = __ldcg(reinterpret_cast<const float4*>(src + static_cast<long long>(u) * 4 * p.ldp));
-          if (k == 4 && p.b_post != nullptr) t[i] = __ldcg(reinterpret_cast<const float4*>(src + (static_cast<long long>(u) * 4 + 2) * p.ldp));
+          q[i] = __ldcg(reinterpret_cast<const float4*>(src + static_cast<long long>(u) * p.sums * p.ldp));
+          if (k == 4 && p.b_post != nullptr) t[i] = __ldcg(reinterpret_cast<const float4*>(src + (static_cast<long long>(u) * p.sums + 2) * p.ldp));
         }
       }
 #pragma unroll
@@ -865,8 +866,8 @@ void fill(NormParams* p, const FoBlockNormDesc* d) {
 // also costs its partial sums, two a SM, one for wide rows, whatever the device, so that the
 // workspace's size needs no device); short batches give each row group one row at least.
 struct Plan {
-  int groups, chunks, units, ldp;
-  size_t bytes;
+  int groups, chunks, units, ldp, sums;
+  size_t bytes;  // of the units' sums: 8 (LayerNorm form: 16) a column of each
 };
 
 Plan plan(const FoBlockNormDesc* d, int per_sm, int row_groups) {
@@ -881,7 +882,8 @@ Plan plan(const FoBlockNormDesc* d, int per_sm, int row_groups) {
   b.chunks = chunks;
   b.units = b.groups * b.chunks;
   b.ldp = (static_cast<int>(d->D) + 3) / 4 * 4;
-  b.bytes = 4 * static_cast<size_t>(b.units) * b.ldp * sizeof(float);
+  b.sums = d->norm == FO_NORM_LAYER ? 4 : 2;
+  b.bytes = static_cast<size_t>(b.units) * b.sums * b.ldp * sizeof(float);
   return b;
 }
 
@@ -970,7 +972,7 @@ extern "C" int fo_block_norm_backward(const FoBlockNormDesc* d, void* stream) {
   j.out[0] = d->dw_pre, j.out[1] = d->w_post != nullptr ? d->dw_post : nullptr, j.out[2] = d->db_pre, j.out[3] = d->db_post;
   j.out[4] = d->gate != nullptr ? d->dgate : nullptr;
   j.w_post = d->w_post, j.b_post = d->b_post, j.gate = d->gate, j.ldgate = d->ldgate;
-  j.units = b.units, j.chunks = b.chunks, j.ldp = b.ldp, j.D = D, j.vec_dtype = d->vec_dtype;
+  j.units = b.units, j.chunks = b.chunks, j.ldp = b.ldp, j.sums = b.sums, j.D = D, j.vec_dtype = d->vec_dtype;
   const unsigned outs = 4u + (d->gate != nullptr ? static_cast<unsigned>(b.groups) : 0u);
   e = launch_pdl(fo_norm_join_kernel, g_no_opt, dim3(outs, (D + 31) / 32), dim3(8 * kJoinSplit), 0, 1, st, j);
   if (e != cudaSuccess) return host_fail(FO_ECUDA, "kernel launch failed: %s", cudaGetErrorString(e));

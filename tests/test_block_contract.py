@@ -74,3 +74,17 @@ def test_w4_groups_longer_than_the_index_division_holds_are_refused():
     per = (1 << 18) - 5  # and past it
     rcp = -(-(1 << 32) // per)
     assert any((i * rcp) >> 32 != i // per for i in range(per - 1, 1 << 20, per))
+
+
+@pytest.mark.parametrize("T,D,rows", [(16384, 4096, 16384), (4096, 1001, 4), (7, 64, 0)])
+def test_norm_workspace_holds_the_sums_that_the_form_has(T, D, rows):
+    """Per unit of rows, fp32: two sums a column in the rms form, four in the other."""
+    d = _norm(T=T, D=D, gate_rows=rows, gate=A if rows else None)
+    need = N.lib().fo_block_norm_backward_workspace_size
+    rms = need(ctypes.byref(d))
+    units, odd = divmod(rms, 2 * 4 * ((D + 3) // 4 * 4))
+    assert odd == 0 and units >= max(1, rows)
+    if rows == T:
+        assert units == rows  # one row a unit
+    d.norm = N.FO_NORM_LAYER
+    assert need(ctypes.byref(d)) == 2 * rms
