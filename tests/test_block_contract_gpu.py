@@ -2,9 +2,11 @@
 import pytest
 import torch
 
+from block_util import U, within
 from gpu_util import gen, status_clean
 
 from icpp_tuning_b200 import block
+from test_block_norm_gpu import backward64, d64, gpu as norm_gpu, make as norm_inputs
 from test_w4_gpu import gpu, weight
 
 pytestmark = pytest.mark.gpu
@@ -52,4 +54,23 @@ def test_an_infinity_between_the_products(T, dtype):
     assert (z[0] == float("inf")).all()
     if T > 1:
         assert y[1:].isfinite().all() and z[1:].isfinite().all()
+    status_clean()
+
+
+@pytest.mark.parametrize("layer", [False, True])
+@pytest.mark.parametrize("T,D,rows", [(700, 129, 700), (900, 264, 300), (400, 1030, 200), (333, 64, 111)])
+def test_norm_gradients_of_many_gate_rows(T, D, rows, layer):
+    """A gate a token, and groups on both sides of one unit of work a gate row."""
+    dtype, vec = torch.bfloat16, torch.float32
+    v = norm_inputs(T, D, dtype, vec, layer, True, rows, seed=T)
+    v["r"] = v.pop("x")
+    dr, dz = ((torch.randn(T, D, generator=gen(i)) * 0.5).to(dtype) for i in range(2))
+    w = d64(v)
+    ref = backward64(w, dr.double(), dz.double(), w["r"], 0.5, layer, U[dtype], U[vec])
+    c = {k: norm_gpu(t) for k, t in v.items()}
+    out = block.block_norm_backward(dr.cuda(), dz.cuda(), c["y"], c["r"], c["w_post"], c["w_pre"], b_post=c["b_post"], b_pre=c["b_pre"],
+                                    gate=c["gate"], residual_scale=0.5, norm="layer" if layer else "rms")
+    assert set(out) == set(ref)
+    for k, (r, b) in ref.items():
+        within(out[k], r, b, k)
     status_clean()
