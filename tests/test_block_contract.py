@@ -88,3 +88,11 @@ def test_norm_workspace_holds_the_sums_that_the_form_has(T, D, rows):
         assert units == rows  # one row a unit
     d.norm = N.FO_NORM_LAYER
     assert need(ctypes.byref(d)) == 2 * rms
+
+
+@pytest.mark.parametrize("D,layer,units", [(4096, False, 296), (4096, True, 148), (2049, False, 148), (2048, True, 296), (8192, False, 148)])
+def test_norm_backward_plans_the_units_that_run_at_once(D, layer, units):
+    """Two CTAs a SM, one where the kernel has 512 threads of 128 registers."""
+    d = _norm(T=16384, D=D, norm=N.FO_NORM_LAYER if layer else N.FO_NORM_RMS)
+    need = N.lib().fo_block_norm_backward_workspace_size(ctypes.byref(d))
+    assert need == units * (4 if layer else 2) * 4 * ((D + 3) // 4 * 4)
