@@ -61,10 +61,10 @@ __device__ __forceinline__ float low_part(float v, float high) {
   return fabsf(rest) < __builtin_huge_valf() ? rest : 0.f;
 }
 
-// The gated activations and their derivatives, in forms whose error stays at fp32's: the
-// sigmoid ones take one exponential and one reciprocal a value (gelu_tanh(g) = g sigmoid(2 w),
-// w = sqrt(2 / pi) (g + 0.044715 g^3)), the erf one a reciprocal (erf by Abramowitz & Stegun
-// 7.1.28, |error| <= 3e-7) and, for the derivative, an exponential.
+// The gated activations and their derivatives.  The sigmoid ones take one exponential and one
+// reciprocal a value (gelu_tanh(g) = g sigmoid(2 w), w = sqrt(2 / pi) (g + 0.044715 g^3)); the
+// erf one takes the same two.  Errors are a few units of fp32, relative to the value, the
+// exponential's argument x adding |x| 2^-24: tests/test_gate_math_gpu.py holds the bounds.
 __device__ __forceinline__ Two exp_of(Two x) {
   const float2 f = both(mul2(x, two(1.4426950408889634f)));
   float a, b;
@@ -81,23 +81,25 @@ __device__ __forceinline__ Two rcp_of(Two x) {
 }
 __device__ __forceinline__ Two sigmoid(Two x) { return rcp_of(add2(two(1.0f), exp_of(mul2(x, two(-1.0f))))); }
 
-__device__ __forceinline__ Two normal_cdf(Two g) {  // (1 + erf(g / sqrt 2)) / 2
-  const Two z = mul2(g, two(0.7071067811865476f));
-  const float2 f = both(z);
-  const Two az = two(fabsf(f.x), fabsf(f.y));
-  Two p = fma2(two(4.30638e-5f), az, two(2.765672e-4f));
-  p = fma2(p, az, two(1.520143e-4f));
-  p = fma2(p, az, two(9.2705272e-3f));
-  p = fma2(p, az, two(4.22820123e-2f));
-  p = fma2(p, az, two(7.05230784e-2f));
-  p = fma2(p, az, two(1.0f));
-  Two r = rcp_of(p);
-  r = mul2(r, r);
-  r = mul2(r, r);
-  r = mul2(r, r);
-  r = mul2(r, r);
-  const float2 e = both(fma2(r, two(-1.0f), two(1.0f)));
-  return fma2(two(0.5f), two(copysignf(e.x, f.x), copysignf(e.y, f.y)), two(0.5f));
+// (1 + erf(g / sqrt 2)) / 2 and bell = e^(-g^2 / 2): the tail below -|g| is bell times a
+// polynomial in t = 1 / (1 + 0.3 |g|), the minimax fit of degree 8 to the tail / bell over |g| <=
+// 14 (relative error 6e-8; a Remez iteration on 0.5 erfcx(|g| / sqrt 2)).  So the tail keeps its
+// relative accuracy where 1 + erf cancels.
+__device__ __forceinline__ Two normal_cdf(Two g, Two& bell) {
+  const float2 f = both(g);
+  const Two t = rcp_of(fma2(two(0.3f), two(fabsf(f.x), fabsf(f.y)), two(1.0f)));
+  Two p = fma2(two(3.837832828e-2f), t, two(-1.691660597e-1f));
+  p = fma2(p, t, two(2.286599804e-1f));
+  p = fma2(p, t, two(-7.650637060e-2f));
+  p = fma2(p, t, two(1.425354567e-1f));
+  p = fma2(p, t, two(9.468354909e-2f));
+  p = fma2(p, t, two(1.219203362e-1f));
+  p = fma2(p, t, two(1.194876897e-1f));
+  p = fma2(p, t, two(7.168838789e-6f));
+  bell = exp_of(mul2(mul2(g, two(-0.5f)), g));
+  const Two tail = mul2(p, bell);
+  const float2 lo = both(tail), hi = both(fma2(tail, two(-1.0f), two(1.0f)));
+  return two(f.x < 0.f ? lo.x : hi.x, f.y < 0.f ? lo.y : hi.y);
 }
 
 template <int ACT>
@@ -105,7 +107,10 @@ __device__ __forceinline__ Two gate_act(Two g) {
   if constexpr (ACT == ACT_SILU) return mul2(g, sigmoid(g));
   if constexpr (ACT == ACT_GELU_TANH)
     return mul2(g, sigmoid(mul2(mul2(two(1.5957691216057308f), g), fma2(two(0.044715f), mul2(g, g), two(1.0f)))));
-  if constexpr (ACT == ACT_GELU_ERF) return mul2(g, normal_cdf(g));
+  if constexpr (ACT == ACT_GELU_ERF) {
+    Two bell;
+    return mul2(g, normal_cdf(g, bell));
+  }
   const float2 f = both(g);
   return two(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);
 }
@@ -133,9 +138,10 @@ __device__ __forceinline__ void gate_grad(Two dh, Two g, Two u, Two& dg, Two& du
     const Two w = mul2(two(1.5957691216057308f), fma2(two(0.134145f), g2, two(1.0f)));
     ds = fma2(mul2(s, fma2(p, two(-1.0f), two(1.0f))), w, p);
   } else if constexpr (ACT == ACT_GELU_ERF) {
-    const Two c = normal_cdf(g);
+    Two bell;
+    const Two c = normal_cdf(g, bell);
     s = mul2(g, c);
-    ds = fma2(mul2(g, two(0.3989422804014327f)), exp_of(mul2(mul2(g, two(-0.5f)), g)), c);
+    ds = fma2(mul2(g, two(0.3989422804014327f)), bell, c);
   } else {
     const float2 f = both(g);
     s = two(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);
