@@ -132,8 +132,11 @@ __device__ __forceinline__ void gate_grad(Two dh, Two g, Two u, Two& dg, Two& du
     ds = fma2(s, fma2(p, two(-1.0f), two(1.0f)), p);
   } else if constexpr (ACT == ACT_GELU_TANH) {
     // s = g p, p = sigmoid(2 w): s' = p + s (1 - p) 2 w'
-    const Two g2 = mul2(g, g);
-    const Two p = sigmoid(mul2(mul2(two(1.5957691216057308f), g), fma2(two(0.044715f), g2, two(1.0f))));
+    // (past +-64, where p is 1 or 0 and s' with it, g^3 and w' stay those of 64: an infinity would
+    // meet 1 - p = 0)
+    const float2 f = both(g);
+    const Two near = two(fminf(fmaxf(f.x, -64.f), 64.f), fminf(fmaxf(f.y, -64.f), 64.f)), g2 = mul2(near, near);
+    const Two p = sigmoid(mul2(mul2(two(1.5957691216057308f), near), fma2(two(0.044715f), g2, two(1.0f))));
     s = mul2(g, p);
     const Two w = mul2(two(1.5957691216057308f), fma2(two(0.134145f), g2, two(1.0f)));
     ds = fma2(mul2(s, fma2(p, two(-1.0f), two(1.0f))), w, p);

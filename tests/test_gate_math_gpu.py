@@ -84,3 +84,22 @@ def test_derivatives(act, short):
                     for i in range(0, n, size)])
     within(dx[:, 0], da, U1 * da.abs() + unit * terms, "act'")
     within(dx[:, 1], a, U1 * a.abs() + (unit * a.abs()).clamp(max=1.0) + 2.0 ** -25, "act")
+
+
+@pytest.mark.parametrize("short", [True, False])
+@pytest.mark.parametrize("act", ACTS)
+def test_saturation_of_bfloat16(act, short):
+    """Finite g of any size: act' is 1 or 0 there, act is g or 0."""
+    dtype = torch.bfloat16
+    g = torch.tensor([1e9, 1e14, 1e19, 1e20, 1e30, 3e38], dtype=torch.float64).to(dtype)
+    g = torch.cat([g, -g]).repeat(1 if short else 20)
+    n = len(g)
+    G, Up, x, dy = (torch.zeros(n, D, dtype=dtype) for _ in range(4))
+    G[:, 0], Up[:, 0], dy[:, 0] = g, 1, 1
+    w = [m.to(dtype).cuda() for m in (one(0, 0), one(0, 1), one(0, 0))]
+    dx = block.gated_ffn_backward(dy.cuda(), x.cuda(), *w, G.cuda(), Up.cuda(), act=act, b_layout="nk")[0].cpu()
+    assert torch.equal(dx[:, 0].float(), (g > 0).float())
+    assert torch.equal(dx[:, 1].float(), g.float().clamp(min=0))
+    x[:, 0], x[:, 1] = g, 1
+    y = block.gated_ffn(x.cuda(), *w, act=act, b_layout="nk")[:, 0].cpu()
+    assert torch.equal(y.float(), g.float().clamp(min=0))
