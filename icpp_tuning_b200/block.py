@@ -129,7 +129,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     x [T, D] float16 / bfloat16; w_gate, w_up [D, F] and w_down [F, N] when b_layout == "kn",
     [F, D] and [N, F] when "nk" (nn.Linear).  act: one of GATE_ACTS.  Returns y [T, N], or with
     save=True (y, g, u): the products before the activation, for gated_ffn_backward.  The
-    intermediate act(g) * u is rounded to x's dtype.  Row strides must be multiples of 8."""
+    intermediate act(g) * u is rounded to x's dtype; up to 32 tokens it is held in two parts of
+    that dtype, its high and its low bits.  Row strides must be multiples of 8."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout, save=save)

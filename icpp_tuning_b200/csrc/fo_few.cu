@@ -14,11 +14,11 @@ cudaError_t launch(const FewMaps& m, const FewParams& p, const FewPlan& l, cudaS
 
 template <int MODE, int ACT>
 cudaError_t by_tokens(const FewMaps& m, const FewParams& p, const FewPlan& l, cudaStream_t s) {
-  switch (l.nt) {
-    case 16: return launch<MODE, ACT, 16>(m, p, l, s);
-    case 32: return launch<MODE, ACT, 32>(m, p, l, s);
-    default: return launch<MODE, ACT, 64>(m, p, l, s);
+  if (l.nt == 16) return launch<MODE, ACT, 16>(m, p, l, s);
+  if constexpr (MODE != FEW_GATED) {  // which has one column a token, 32 at most
+    if (l.nt == 64) return launch<MODE, ACT, 64>(m, p, l, s);
   }
+  return launch<MODE, ACT, 32>(m, p, l, s);
 }
 
 template <int MODE>

@@ -1,6 +1,6 @@
 // fo_few.cuh -- the tcgen05 kernel for products whose token side is short: the weights are
-// the MMA's M side (128 features a tile), the tokens its N side (NT = 16, 32 or 64 columns,
-// all of them in one tile).
+// the MMA's M side (128 features a tile), the tokens its N side (NT = 16, 32 or, but for
+// FEW_GATED, 64 columns, all of them in one tile).
 //
 // With few tokens the time is that of the weights' bytes: an MMA costs by its token columns,
 // so nothing is spent on absent rows, and a SM keeps about 200 KB of weight tiles in flight
@@ -15,8 +15,8 @@
 //   FEW_PLAIN  one weight tile a K block, over one or two K segments
 //   FEW_DGATE  FEW_PLAIN's accumulator is dh: writes dg, du, h from the saved g, u
 // Between the forward pass's two products h travels as two 16-bit parts, high and low, in rows
-// 2 t and 2 t + 1: twice the token columns of an MMA that is not the bound, and h costs no
-// precision.
+// 2 t and 2 t + 1: twice the token columns of an MMA that is not the bound, and h keeps 16
+// significant bits in bf16, 22 in fp16 (there down to steps of 2^-24).
 //
 // Measured, both products of the block, bf16: 4096 x 16384, 403 MB, one token in 67 us (6.0
 // TB/s), 24 tokens in 78 us; 1 x 1024 x 4096, 25 MB in 11.7 us, bound by the launches and the
