@@ -18,9 +18,9 @@
 // 2 t and 2 t + 1: twice the token columns of an MMA that is not the bound, and h keeps 16
 // significant bits in bf16, 22 in fp16 (there down to steps of 2^-24).
 //
-// Measured, both products of the block, bf16: 4096 x 16384, 403 MB, one token in 67 us (6.0
-// TB/s), 24 tokens in 78 us; 1 x 1024 x 4096, 25 MB in 11.7 us, bound by the launches and the
-// first copies' latency.
+// Measured, both products of the block, bf16: 4096 x 16384, 403 MB, one token in 66 us (6.1
+// TB/s), 24 tokens in 78 us; 1 x 1024 x 4096, 25 MB in 12.7 us (10.9 from L2), bound by the
+// launches and the first copies' latency.
 #pragma once
 #include "fo_ffn.cuh"
 

@@ -15,6 +15,11 @@
 //              tiles and long K is cut along K into fp32 parts, which the next launch joins
 // Operands are K-major or MN-major (read transposed) per problem, so every product of the
 // block and its gradients runs on tensors as they are, without a transposition pass.
+// h, dg, du (and h again, backward) are rounded to the operands' 16-bit type between the
+// products: the matrix instructions take both operands in one type, and a second part, high and
+// low, would double these products' work, which is their time.  It costs an output's error
+// against 64 bits 0.0017 -> 0.0023 in bf16, 0.00021 -> 0.00029 in fp16 (2-norms of the error over
+// that of the result; the output's own rounding is the rest).
 //
 // Large products are bound by the matrix units under the power limit: 8192 x 4096 x 16384
 // bf16, gated 1.5-1.7 ms and down 0.75-0.86 ms (1280-1480 TFLOP/s).  A product of a few waves

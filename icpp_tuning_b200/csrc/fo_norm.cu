@@ -24,9 +24,14 @@
 // sum(t), db_post = gate sum(t) are formed once a gate row, in the kernel that joins the
 // CTAs' sums in a fixed order.
 //
-// Measured, 16384 x 4096 bf16 RMS with gate: forward 92 us (5.8 TB/s), backward 143 us (5.6
-// TB/s).  Odd rows cost instructions, one 2-byte shared load and store a value: LayerNorm
-// backward 4680 x 1001 fp16, 43 us (1000 columns: 31).
+// Measured, 16384 x 4096 bf16 with gate: RMS forward 91 us (5.9 TB/s), backward 142 us (5.7
+// TB/s); LayerNorm 114 and 243.  Odd rows cost instructions, one 2-byte shared load and store a
+// value: LayerNorm backward 4680 x 1001 fp16, 42 us (1000 columns: 28).  The LayerNorm-form and
+// odd-row kernels are bound by instructions at 16 warps a SM, and their backward passes spill at
+// the cap of 128 registers: 72 to 104 bytes a thread in the LayerNorm form up to 4096 columns
+// (716 above), 104 to 152 (364) for odd rms rows, 180 to 320 (864) for odd LayerNorm rows; the
+// other rms ones 64 at most.  Forward, odd rows of up to 4096 columns spill 150 to 172, all rows
+// of more than 8192 columns 120 to 690.
 #include "fo_host.cuh"
 #include "fo_math.cuh"
 #include "../../include/b200fo.h"

@@ -31,10 +31,10 @@
 // sums meet in shared memory (distributed across the cluster) and are added in a fixed order.
 //
 // Measured, groups of 128 unless said: one token, bf16, 4096 x 16384 gated block (104 MB of
-// weights and scales) 30 us with its digits' kernels (16-bit operands: 42.1); 16384 x 4096
+// weights and scales) 30 us with its digits' kernels (16-bit operands: 41); 16384 x 4096
 // product 11.3 us; 8 tokens, block 44.2 us; 5 tokens, fp16, groups of 32 with zeros, 52 us (120
 // MB).  That last form is bound by the latencies of a step's chain (copies, table, MMAs, sums)
-// at 14 warps a SM: its integer pipe is busy 47% of the time, issue 39%.  Short products are
+// at 14 warps a SM: its integer pipe is busy 53% of the time, issue 45%.  Short products are
 // bound by the launch and the start and end of their few steps a warp (4096 x 4096, one token:
 // 5.6 us for 8.7 MB; 5.3 in fp16).  More tokens cost MMAs, 32 of them as much as 4 times
 // the bytes: block 64 us at 9 tokens, 122 at 32.
@@ -765,7 +765,8 @@ __global__ void __launch_bounds__(256, 2) fo_w4i_kernel(const __grid_constant__ 
 // Tiles, warps a tile and CTAs a tile: as many warps as fit at once (a fifth more is better
 // than half as many), then CTAs for a tile of long K, or where most SMs would have none.  Of one
 // token 4096 x 4096: 8 warps 5.1 us, 16 in two CTAs 6.5; 16384 x 4096: 4 warps a tile 10.8, 8
-// (two waves) 13.0; 64 tokens 4096 x 4096: 8 warps 23.6, 16 29.4.
+// (two waves) 13.0; 64 tokens 4096 x 4096: 8 warps 23.6 (22.2 since the weights open as q -
+// zero), 16 29.4.
 struct W4Plan {
   int share, q, lg;
   unsigned ctas;
@@ -795,11 +796,12 @@ cudaError_t launch(W4Params p, int sms, cudaStream_t stream) {
 
 int64_t digit_blocks(int64_t T) { return (kPlanes * T + 7) / 8; }
 // Whether x travels as digits: where the tokens' digits fill one block of 8 columns (4096 x
-// 16384 block, one token: groups of 128 42.1 -> 30.6 us, of 64 45.9 -> 34.6, of 32 51 -> 42); up
-// to three where a group is a step or longer (4 tokens 44.1 -> 34.4, 8 tokens 49.7 -> 44.9;
-// groups of 32, 3 tokens: 48.6 -> 54.5).  Up to 2^24 weights a block the second launch costs
-// the caller more (3 us) than the GPU saves (one token 4096 x 4096 5.2 -> 5.8, 8192 x 4096 8.2 ->
-// 7.9, 16384 x 4096 14.7 -> 10.8; 4 tokens 8192 x 4096 8.6 -> 9.9).
+// 16384 block, bf16, one token: groups of 128 41.1 -> 29.8 us, of 64 43.5 -> 31.8, of 32 48.7 ->
+// 39.3); up to three where a group is a step or longer (4 tokens 43.2 -> 33.2, 8 tokens 48.5 ->
+// 43.9; groups of 32, 3 tokens: 49.8 -> 54.5).  Up to 2^24 weights a block the second launch
+// costs the caller more (3 us) than the GPU saves (one token 4096 x 4096 5.6 -> 6.1, 8192 x 4096
+// 8.7 -> 8.2, 16384 x 4096 14.3 -> 11.2; 4 tokens 8192 x 4096 9.1 -> 9.9; 8 tokens 16384 x 4096
+// 15.9 -> 16.4).
 bool as_digits(int64_t T, int64_t N, int64_t K, int per32) {
   return T > 0 && digit_blocks(T) <= (per32 % 4 == 0 ? 3 : 1) && N * K > digit_blocks(T) << 24;
 }

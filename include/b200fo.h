@@ -280,8 +280,10 @@ typedef struct FoW4 {
   int32_t group;
 } FoW4;
 
-/* out[T, N] = x[T, K] w^T (+ bias).  K a multiple of 32.  Any T; the weights are read once
- * for every 32 tokens, so it pays for few.  A few tokens times large weights (those for which
+/* out[T, N] = x[T, K] w^T (+ bias).  K a multiple of 32.  Any T, but made for a few tokens: the
+ * time grows with the tokens from about 8 on (4096 x 16384 gated block, groups of 128: 1 token
+ * 30 us, 8 44, 16 69, 32 122; in 16-bit weights 66, 70, 74, 78), and beyond 16 of them the same
+ * weights in 16 bits are faster.  A few tokens times large weights (those for which
  * a workspace is asked) take x as fixed point of 23 bits relative to the largest magnitude of
  * its 128 k's, with exact integer sums inside a group; a value that is not finite then makes
  * its token's outputs NaN. */
