@@ -17,6 +17,10 @@ import torch
 from . import block
 
 
+def _wants_gradients(*args) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args)
+
+
 class _FirstDerivatives(torch.autograd.Function):
     """Runs a backward pass.  Under create_graph its results depend on every tensor that it
     was given, and differentiating them raises: the operators have no second derivatives."""
@@ -31,7 +35,14 @@ class _FirstDerivatives(torch.autograd.Function):
 
 
 class GatedFFN(torch.autograd.Function):
-    """y = (act(x Wg) * (x Wu)) Wd with its first derivatives; keeps x and the two products."""
+    """y = (act(x Wg) * (x Wu)) Wd with its first derivatives; keeps x and the two products
+    where a gradient is wanted."""
+
+    @classmethod
+    def apply(cls, x, w_gate, w_up, w_down, act, b_layout):
+        if not _wants_gradients(x, w_gate, w_up, w_down):
+            return block.gated_ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout)
+        return super().apply(x, w_gate, w_up, w_down, act, b_layout)
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act, b_layout):
@@ -53,9 +64,8 @@ class BlockNorm(torch.autograd.Function):
 
     @classmethod
     def apply(cls, y, *rest):
-        if y.shape[1] > block.MAX_NORM_BACKWARD and torch.is_grad_enabled() and any(
-                isinstance(t, torch.Tensor) and t.requires_grad for t in (y, *rest)):
-            raise ValueError(f"the norms' backward pass takes rows of at most {block.MAX_NORM_BACKWARD} columns, got {y.shape[1]}")
+        if y.shape[-1] > block.MAX_NORM_BACKWARD and _wants_gradients(y, *rest):
+            raise ValueError(f"the norms' backward pass takes rows of at most {block.MAX_NORM_BACKWARD} columns, got {y.shape[-1]}")
         return super().apply(y, *rest)
 
     @staticmethod

@@ -110,3 +110,21 @@ def test_widths_without_a_backward_pass_are_refused_forward(monkeypatch):
         call()
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+def test_nothing_is_saved_without_gradients(monkeypatch):
+    saves = []
+
+    def ffn(x, w_gate, w_up, w_down, *, act, b_layout, save=False):
+        saves.append(save)
+        out = _ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout, save=True)
+        return out if save else out[0]
+
+    monkeypatch.setattr(block, "gated_ffn", ffn)
+    args = _ffn_inputs()
+    y = gated_block.GatedFFN.apply(*args, "relu", "nk")
+    with torch.no_grad():
+        z = gated_block.GatedFFN.apply(*args, "relu", "nk")
+    w = gated_block.GatedFFN.apply(*(t.detach() for t in args), "relu", "nk")
+    assert saves == [True, False, False] and torch.equal(y, z) and torch.equal(y, w)
+    assert y.requires_grad and not z.requires_grad and not w.requires_grad
