@@ -130,7 +130,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     [F, D] and [N, F] when "nk" (nn.Linear).  act: one of GATE_ACTS.  Returns y [T, N], or with
     save=True (y, g, u): the products before the activation, for gated_ffn_backward.  The
     intermediate act(g) * u is rounded to x's dtype; up to 32 tokens it is held in two parts of
-    that dtype, its high and its low bits.  Row strides must be multiples of 8."""
+    that dtype, its high and its low bits.  Row strides must be multiples of 8; results whose
+    width is no multiple of 8 are views of such wider rows."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn(x, w_gate, w_up, w_down, act=act, b_layout=b_layout, save=save)
@@ -154,7 +155,9 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                        g: torch.Tensor, u: torch.Tensor, *, act: str = "silu", b_layout: str = "kn",
                        stream=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(dx, dw_gate, dw_up, dw_down) of gated_ffn from dy [T, N] and the g, u it saved."""
+    """(dx, dw_gate, dw_up, dw_down) of gated_ffn from dy [T, N] and the g, u it saved, each laid
+    out like its operand in rows whose stride is a multiple of 8.  `aligned_rows` brings a dy of
+    any strides into that form."""
     if stream is not None:
         with torch.cuda.stream(stream):
             return gated_ffn_backward(dy, x, w_gate, w_up, w_down, g, u, act=act, b_layout=b_layout)

@@ -111,3 +111,16 @@ def test_bounds_without_an_offset_as_digits(T, Nn, K, group):
     ref = X @ v.t()
     out = block.matvec_w4(x.cuda(), gpu(w))
     within(out, ref, U[dtype] * ref.abs() * 1.01 + ACC * X.abs() @ v.abs().t() + 2.0 ** -22 * step_most(X) @ v.abs().t())
+
+
+@pytest.mark.parametrize("T,Nn,K,group", [(1, 8200, 2048, 32), (2, 16001, 1056, 64), (8, 12300, 4128, 512)])
+def test_any_zero_of_eight_bits_as_digits(T, Nn, K, group):
+    dtype = torch.float16 if T % 2 else torch.bfloat16
+    w = weight(Nn, K, group, dtype, True, seed=K)
+    w = w._replace(zeros=torch.randint(0, 256, w.zeros.shape, generator=gen(K), dtype=torch.uint8))
+    x = torch.randn(T, K, generator=gen(T)).to(dtype)
+    v, _ = opened(w)
+    X = x.double()
+    ref = X @ v.t()
+    within(block.matvec_w4(x.cuda(), gpu(w)), ref, U[dtype] * ref.abs() * 1.01 + ACC * X.abs() @ v.abs().t() + 2.0 ** -22 * step_most(X) @ v.abs().t())
+    status_clean()
